@@ -358,6 +358,62 @@ int nob200_hadamard128_heads(int tokens, int head_offset, const void* input, voi
                              void* stream);
 
 /*
+ * Attention over packed documents (no counterpart in the reference).  query bf16 [num_rows, heads, 128], key / value bf16
+ * [num_key_rows, kv_heads, 128] (heads a multiple of kv_heads; head h reads key head h / (heads / kv_heads)), output bf16
+ * [num_rows, total_heads, 128] at head_offset.  bounds / key_bounds int32 [documents + 1], ascending: rows
+ * bounds[d] .. bounds[d + 1] attend to key rows key_bounds[d] .. key_bounds[d + 1]; rows outside all documents are left as
+ * they are.  Query i of n stands at position p = i + m - n among its document's m keys.
+ *   score = scale * q.k;  cap > 0: cap * tanh(score / cap);  slopes f32 [heads] not NULL: minus slopes[h] * |p - j|
+ *   causal != 0: key j is seen if j <= p or j < prefix[d] (int32 [documents], NULL: 0); else all keys of the document are.
+ * A row that sees no key gets zeros.  Keys and values that a row does not see may hold anything (infinities, NaN); where a
+ * document's value row is not finite, whole rows that see it under a partial mask become NaN.
+ * unit_rows (128 or 256) query rows of a document and head are a CTA's; kv_splits > 1 divides the keys of each over so
+ * many CTAs, whose fp32 results a second kernel joins: workspace of ..._workspace_bytes().
+ */
+size_t nob200_masked_bf16_attention_d128_workspace_bytes(int num_rows, int heads, int kv_splits);
+int nob200_masked_bf16_attention_d128(int num_rows, int num_key_rows, int documents, int head_offset, const void* query,
+                                      const void* key, const void* value, const void* bounds, const void* key_bounds,
+                                      const void* prefix, const void* slopes, void* output, int heads, int kv_heads,
+                                      int total_heads, int causal, float scale, float cap, int unit_rows, int kv_splits,
+                                      void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * A cache of keys and values in 8 bits (no counterpart in the reference): blocks of 64 tokens, codes int8
+ * [num_blocks, heads, 64, 128], scales f32 [num_blocks, heads] for each of K and V; value = code * scale.
+ * table int32 [sequences, max_blocks]: the block of tokens 64 b .. 64 b + 63 of a sequence; lengths int32 [sequences].
+ * What a block number, length or bound points to outside these tensors is skipped and bit 6 of the status word set.
+ *
+ * append: rows bounds[s] .. bounds[s + 1] (int32 [sequences + 1]) of key / value bf16 [num_rows, heads, 128] become the last
+ * tokens of sequence s, whose `lengths` count them already.  A block's scale is max(largest magnitude / 127, 1e-10); a token
+ * that raises it has the tokens already in the block rounded again on the new grid.  Two sequences must not append to one
+ * block in the same call.
+ * read: the sequences' tokens as bf16 rows [capacity, heads, 128], one sequence behind the other, and where each begins
+ * (bounds int32 [sequences + 1]); rows behind the last are left as they are, tokens past the capacity are not written.
+ */
+int nob200_int8_cache_append_d128(int num_rows, int sequences, int max_blocks, int num_blocks, const void* key,
+                                  const void* value, const void* bounds, const void* table, const void* lengths,
+                                  void* key_codes, void* key_scales, void* value_codes, void* value_scales, int heads,
+                                  void* stream);
+int nob200_int8_cache_read_d128(int capacity, int sequences, int max_blocks, int num_blocks, const void* key_codes,
+                                const void* value_codes, const void* key_scales, const void* value_scales, const void* table,
+                                const void* lengths, void* key, void* value, void* bounds, int heads, void* stream);
+
+/*
+ * Attention of the queries bounds[s] .. bounds[s + 1] over the cached tokens of sequence s, with positions, masks, cap and
+ * slopes as nob200_masked_bf16_attention_d128 (a sequence is a document, lengths[s] its keys).  query bf16
+ * [num_rows, heads, 128], key / value codes int8 [num_blocks, kv_heads, 64, 128], output bf16 [num_rows, total_heads, 128]
+ * at head_offset.  For a few rows per sequence and key head: 16 of them are a CTA's.  kv_splits > 1 divides each
+ * sequence's blocks over so many CTAs (workspace of ..._workspace_bytes()).
+ */
+size_t nob200_int8_cache_attention_d128_workspace_bytes(int num_rows, int heads, int kv_splits);
+int nob200_int8_cache_attention_d128(int num_rows, int sequences, int max_blocks, int num_blocks, int head_offset,
+                                     const void* query, const void* key, const void* value, const void* key_scales,
+                                     const void* value_scales, const void* table, const void* lengths, const void* bounds,
+                                     const void* prefix, const void* slopes, void* output, int heads, int kv_heads,
+                                     int total_heads, int causal, float scale, float cap, int kv_splits, void* workspace,
+                                     size_t workspace_bytes, void* stream);
+
+/*
  * INT8 GEMM with the scaled fused epilogue of the projections around attention.
  * Replaces MatmulInt8Kernel / program matmul_int8 (src/nano_omni/kernels/matmul/matmul_int8.py:53-240; Arguments:
  * input, weight, bias, residual, multiply, output, weight_scale, input_scale, use_silu):

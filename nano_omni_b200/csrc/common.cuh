@@ -31,6 +31,7 @@ enum StatusBit : uint32_t {
   kWaitTimeoutRing = 1u << 3,     // waiting for a free ring stage
   kWaitTimeoutPeer = 1u << 4,     // waiting for another GPU at a cross-rank barrier
   kIndexCheckFailed = 1u << 5,    // checked build only: a store's index lay outside its tensor and was skipped
+  kBadIndex = 1u << 6,            // a block number, length or bound in device memory pointed outside its tensor; skipped
 };
 
 uint32_t* status_word_device_ptr();  // address of the file-scope status word

@@ -1,0 +1,79 @@
+// Ragged batches: which document and which of its rows a CTA works on.
+//
+// Documents (or the sequences of a cache) are packed row behind row; `bounds` [count + 1] on the device holds where each
+// begins and the last one ends.  The host sizes a grid by what all rows and one partly filled unit per document can come to;
+// a CTA looks its unit up and leaves when there is none.  Bounds are clamped to the tensors, so whatever they hold nothing
+// outside is touched.
+#pragma once
+
+#include "common.cuh"
+
+namespace nob200 {
+
+// Units of `unit` items that `rows` items in up to `documents` documents can come to.
+inline long long most_units(long long rows, long long documents, int unit) {
+  const long long most = (rows + documents * (unit - 1)) / unit;
+  return most < rows ? most : rows;
+}
+
+#ifdef __CUDACC__
+
+__device__ __forceinline__ int clamped(int x, int low, int high) { return min(max(x, low), high); }
+
+// Rows [begin, end) of document `d`, inside [0, rows].
+__device__ __forceinline__ int2 document_rows(const int* bounds, int d, int rows) {
+  const int begin = clamped(bounds[d], 0, rows);
+  return make_int2(begin, clamped(bounds[d + 1], begin, rows));
+}
+
+// The `slot`-th unit, counted from the last document's last unit backwards, where document d has units_of(d) of them: of
+// documents of one length the longest key ranges of a causal mask come first, which leaves the short ones for the end of the
+// launch.  Called by a converged warp; (document, unit in it), or (-1, 0) when there are fewer units.
+template <typename UnitsOf>
+__device__ __forceinline__ int2 find_unit(int documents, int slot, const UnitsOf& units_of) {
+  const int lane = threadIdx.x & 31;
+  for (int last = documents - 1; last >= 0; last -= 32) {
+    const int d = last - lane;
+    int through = d >= 0 ? units_of(d) : 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int other = __shfl_up_sync(0xffffffffu, through, o);
+      if (lane >= o) through += other;
+    }
+    const unsigned mine = __ballot_sync(0xffffffffu, slot < through);
+    if (mine) {
+      const int from = __ffs(mine) - 1;
+      return make_int2(last - from, __shfl_sync(0xffffffffu, through, from) - 1 - slot);
+    }
+    slot -= __shfl_sync(0xffffffffu, through, 31);
+  }
+  return make_int2(-1, 0);
+}
+
+// What the queries of a document see: query i of `queries` stands at position i + keys - queries and sees the first
+// visible(i) of its keys - all of them, or under a causal mask those up to its own position and the document's prefix.
+struct Sight {
+  int keys, ahead, prefix;  // ahead: position of query 0
+  bool causal;
+  __device__ __forceinline__ int visible(int query) const {
+    return causal ? clamped(max(prefix, ahead + query + 1), 0, keys) : keys;
+  }
+};
+
+#endif  // __CUDACC__
+
+// Key ranges that were divided over several CTAs: share z of row r of head h is at [z][h][r].
+struct KeyShares {
+  const int* bounds;  // rows outside [bounds[0], bounds[documents]) are left as they are
+  float* partial;     // normalised rows of 128
+  float* lse;         // log2 units; -inf: a share without weight
+  __nv_bfloat16* output;
+  int documents, rows, heads, total_heads, head_offset, splits;
+};
+inline size_t key_shares_bytes(long long rows, long long heads, int splits) {
+  return splits <= 1 ? 0 : static_cast<size_t>(splits) * heads * rows * (512 + 4);
+}
+// Joins them into the output; defined beside the masked attention kernel.
+int launch_join_shares(const KeyShares& shares, void* stream);
+
+}  // namespace nob200

@@ -1,0 +1,673 @@
+// bf16 attention over packed documents for head_dim 128 on sm_100a: document, causal and prefix masks, scores capped by a
+// tanh, a bias that grows with distance, query heads that share key heads.
+//
+//   s(i, j) = scale * q_i . k_j ;  capped: s = cap * tanh(s / cap) ;  biased: s -= slope[head] * |p_i - j|
+//   o_i = sum_{j < visible(i)} softmax_j(s(i, j)) v_j,   p_i = i + keys - queries of the document
+// Every mask leaves a row the first visible(i) keys of its document, so a row carries one number; a row that sees none gets
+// zeros.  No counterpart in the reference, whose attention of this head width is neither masked nor ragged.
+//
+// One CTA owns a unit of 256 (or 128) query rows of one document and head and walks the key tiles of 128 that its last row
+// sees; warps, TMEM columns, hand-overs and issue order are those of the dense kernel (fa_fwd_bf16.cu): two query tiles
+// take turns at one score buffer, softmax with a thread per row, probabilities to the value MMAs through TMEM.  What the
+// masks add:
+//  * tiles that some row of the unit does not see whole are masked in registers, a compare and a select per score;
+//  * rows of V behind the document's end (another document's, or anything at all) and rows of it that are not finite would
+//    spoil rows that do not see them: 0 x NaN.  Warp 11 walks the V tiles that are not seen whole before their value
+//    MMAs start, zeroes such rows and notes the non-finite ones; a query row that does see one of those becomes NaN.
+//  * capped scores: tanh by an odd polynomial while all of a warp's rows stay within the cap (seven FMAs, 2.4e-7 absolute
+//    error), else by 1 - 2 / (1 + e^2x) on the MUFU.
+#include <cuda.h>
+
+#include "common.cuh"
+#include "documents.cuh"
+#include "fa_common.cuh"
+#include "tensor_map.cuh"
+#include "../../include/nano_omni_b200.h"
+
+namespace nob200 {
+namespace {
+
+constexpr int kTile = 128;
+constexpr int kHalfBytes = kTile * 64 * 2;
+constexpr int kTileBytes = 2 * kHalfBytes;
+constexpr int kStages = 4;
+constexpr int kThreads = 384;
+constexpr int kProducerWarp = 8, kMmaWarp = 9, kCleanWarp = 11;  // warp 10 issues the value MMAs
+constexpr uint32_t kTmemCols = 512;
+constexpr float kRescaleThreshold = 8.0f;  // log2 units
+constexpr float kLowestMaximum = -1e38f;   // relative to it a key of score -inf weighs 0
+constexpr int kServiceRegs = 88;
+constexpr int kSoftmaxRegs = (384 * 168 - 128 * kServiceRegs) / 256 / 8 * 8;
+static_assert(256 * kSoftmaxRegs + 128 * kServiceRegs <= 384 * 168, "setmaxnreg split exceeds the registers the CTA owns");
+constexpr uint32_t kColS = 0, kColP = 128, kColO = 256;  // TMEM columns; P_t at kColP + 64 t, O_t at kColO + 128 t
+
+struct Unit {
+  int row0, rows;        // first row, rows of the document from there on (0: no unit)
+  int key0, query0;      // first key row of the document, first row of the unit within the document
+  int kv_begin, kv_end;  // key tiles of this CTA
+  Sight sight;
+};
+
+struct __align__(1024) Shared {
+  uint8_t q[2][kTileBytes];
+  uint8_t kv[kStages][kTileBytes];
+  uint64_t q_full;
+  uint64_t kv_full[kStages];
+  uint64_t kv_empty[kStages];
+  uint64_t s_full[2];
+  uint64_t s_taken[2];
+  uint64_t p_full[2][2];
+  uint64_t pv_done[2];
+  uint64_t v_clean[2];  // the V tile in stage 1 / 3 has been looked through
+  uint32_t bad[2][4];   // and these of its rows were not finite
+  Unit unit;
+  uint32_t tmem_base;
+  uint32_t abort;
+  uint32_t qk_issued;
+};
+
+struct MaskedParams {
+  const int* bounds;
+  const int* key_bounds;
+  const int* prefix;    // or NULL
+  const float* slopes;  // BIAS form
+  __nv_bfloat16* output;
+  float* partial;  // of KeyShares, when the keys are divided
+  float* lse;
+  uint32_t* status;
+  int rows, key_rows, documents, heads, group, total_heads, head_offset;
+  int slots, unit_rows, splits, causal;
+  float scale;     // of a raw score; CAP form: divided by the cap
+  float to_log2;   // from a (capped) scaled score to log2 units
+};
+
+// tanh(x) = x P(x^2) for |x| <= 1: least squares weighted towards the largest deviation, absolute error 2.4e-7.
+__device__ __forceinline__ uint64_t tanh_small2(uint64_t x) {
+  const uint64_t u = mul2(x, x);
+  uint64_t p = pack2(-0.002839462133550424f, -0.002839462133550424f);
+  p = fma2(p, u, pack2(0.01611417175324844f, 0.01611417175324844f));
+  p = fma2(p, u, pack2(-0.05097285427754116f, -0.05097285427754116f));
+  p = fma2(p, u, pack2(0.1325352487392422f, 0.1325352487392422f));
+  p = fma2(p, u, pack2(-0.3332400372594446f, -0.3332400372594446f));
+  p = fma2(p, u, pack2(0.9999968538421297f, 0.9999968538421297f));
+  return mul2(x, p);
+}
+__device__ __forceinline__ float rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// any x: 1 - 2 / (1 + 2^(2 log2(e) x)); absolute error some 2^-22
+__device__ __forceinline__ float tanh_any(float x) { return fmaf(-2.f, rcp(1.f + ex2(x * 2.885390081777927f)), 1.f); }
+
+// The unit of this CTA, by one converged warp.
+__device__ __forceinline__ Unit unit_of(const MaskedParams& P, int slot, int piece) {
+  Unit u = {};
+  const int2 found = find_unit(P.documents, slot, [&](int d) {
+    const int2 r = document_rows(P.bounds, d, P.rows);
+    return (r.y - r.x + P.unit_rows - 1) / P.unit_rows;
+  });
+  if (found.x < 0) return u;
+  const int2 rows = document_rows(P.bounds, found.x, P.rows), keys = document_rows(P.key_bounds, found.x, P.key_rows);
+  u.query0 = found.y * P.unit_rows;
+  u.row0 = rows.x + u.query0;
+  u.rows = rows.y - u.row0;
+  u.key0 = keys.x;
+  u.sight.keys = keys.y - keys.x;
+  u.sight.ahead = u.sight.keys - (rows.y - rows.x);
+  u.sight.prefix = P.prefix ? P.prefix[found.x] : 0;
+  u.sight.causal = P.causal != 0;
+  const int seen = u.sight.visible(u.query0 + min(u.rows, P.unit_rows) - 1);
+  const int tiles = (seen + kTile - 1) / kTile;
+  u.kv_begin = static_cast<int>(static_cast<long long>(tiles) * piece / P.splits);
+  u.kv_end = static_cast<int>(static_cast<long long>(tiles) * (piece + 1) / P.splits);
+  return u;
+}
+
+template <bool CAP, bool BIAS>
+__global__ void __launch_bounds__(kThreads, 1)
+fa_fwd_masked_bf16_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                          const __grid_constant__ CUtensorMap map_v, const MaskedParams P) {
+  extern __shared__ uint8_t smem_raw[];
+  Shared& S = *reinterpret_cast<Shared*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  volatile uint32_t* abort_flag = &S.abort;
+  uint32_t* status = P.status;
+
+  if (threadIdx.x == 0) {
+    mbar_init(&S.q_full, 1);
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&S.kv_full[s], 1);
+      mbar_init(&S.kv_empty[s], 1);
+    }
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&S.s_full[t], 1);
+      mbar_init(&S.s_taken[t], 4);
+      mbar_init(&S.p_full[t][0], 4);
+      mbar_init(&S.p_full[t][1], 4);
+      mbar_init(&S.pv_done[t], 1);
+      mbar_init(&S.v_clean[t], 1);
+    }
+    S.abort = 0;
+    S.qk_issued = 0;
+    mbar_fence_init();
+  }
+  if (warp == kProducerWarp) {
+    tmem_alloc(&S.tmem_base, kTmemCols);
+    tmem_relinquish();
+  }
+  pdl_wait();  // launched as a programmatic dependent: the set-up above overlaps the kernel before
+  const int head = static_cast<int>(blockIdx.x / (P.slots * P.splits));
+  const int piece = static_cast<int>(blockIdx.x % P.splits);
+  if (warp == 0) {
+    const Unit found = unit_of(P, static_cast<int>(blockIdx.x / P.splits) % P.slots, piece);
+    if (lane == 0) S.unit = found;
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = S.tmem_base;
+  pdl_release();
+
+  const int unit_rows = min(S.unit.rows, P.unit_rows);  // 0: no unit
+  const int n_kv = S.unit.kv_end - S.unit.kv_begin;
+  const int kv_begin = S.unit.kv_begin;
+  const bool two = unit_rows > kTile;
+  // key tiles from this one on (of this CTA's) are not seen whole by the unit's first row
+  const int partly = max(0, S.unit.sight.visible(S.unit.query0) / kTile - kv_begin);
+
+  if (warp >= 8) {
+    reg_dealloc<kServiceRegs>();
+    if (n_kv == 0) {
+    } else if (warp == kProducerWarp) {
+      // ------------------------------------------------------------ TMA producer
+      if (lane == 0) {
+        const int key_head = head / P.group, row0 = S.unit.row0, key0 = S.unit.key0;
+        tma_prefetch_desc(&map_q);
+        tma_prefetch_desc(&map_k);
+        tma_prefetch_desc(&map_v);
+        mbar_expect_tx(&S.q_full, two ? 2 * kTileBytes : kTileBytes);
+        tma_load_3d(S.q[0], &map_q, &S.q_full, 0, head, row0);
+        tma_load_3d(S.q[0] + kHalfBytes, &map_q, &S.q_full, 64, head, row0);
+        if (two) {
+          tma_load_3d(S.q[1], &map_q, &S.q_full, 0, head, row0 + kTile);
+          tma_load_3d(S.q[1] + kHalfBytes, &map_q, &S.q_full, 64, head, row0 + kTile);
+        }
+        const int loads = 2 * n_kv;  // K_j at 2j, V_j at 2j+1
+        int issued = 0;
+        for (int i = 0; i < loads; ++i) {
+          const int st = i % kStages;
+          if (i >= kStages) {
+            if (!mbar_wait(&S.kv_empty[st], ((i / kStages) - 1) & 1, abort_flag, status, kWaitTimeoutRing)) break;
+          }
+          mbar_expect_tx(&S.kv_full[st], kTileBytes);
+          const CUtensorMap* map = (i & 1) ? &map_v : &map_k;
+          const int token = key0 + (kv_begin + (i >> 1)) * kTile;
+          tma_load_3d(S.kv[st], map, &S.kv_full[st], 0, key_head, token);
+          tma_load_3d(S.kv[st] + kHalfBytes, map, &S.kv_full[st], 64, key_head, token);
+          issued = i + 1;
+        }
+        if (*abort_flag) {
+          // Gave up: let the copies already in flight land before the CTA exits.
+          for (int i = (issued > kStages ? issued - kStages : 0); i < issued; ++i) {
+            uint64_t* bar = &S.kv_full[i % kStages];
+            const uint32_t parity = (i / kStages) & 1;
+            for (int spin = 0; spin < (1 << 16) && !mbar_try_wait(bar, parity); ++spin) {
+            }
+          }
+        }
+      }
+    } else if (warp == kCleanWarp) {
+      // ---------------------------------------------- V rows that must not reach the value MMAs
+      // Every tile in turn, and the value MMAs wait for it: a wait that skipped some phases of a barrier could not tell them apart.
+      for (int j = 0; j < n_kv; ++j) {
+        const int st = (2 * j + 1) % kStages, which = j & 1;
+        if (!warp_rest(&S.kv_full[st], ((2 * j + 1) / kStages) & 1, abort_flag, status, kWaitTimeoutLoad)) break;
+        const int left = S.unit.sight.keys - (kv_begin + j) * kTile;  // rows of the tile that belong to the document
+        bool wrote = false;
+#pragma unroll 1
+        for (int k = 0; k < 4 && j >= partly; ++k) {
+          const int row = 32 * k + lane;
+          uint8_t* at[2] = {S.kv[st] + row * 128, S.kv[st] + kHalfBytes + row * 128};
+          // x * 0 is NaN for a value that is not finite, else 0
+          __nv_bfloat162 seen[4];
+          const __nv_bfloat162 zero = __floats2bfloat162_rn(0.f, 0.f);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) seen[i] = zero;
+#pragma unroll
+          for (int c = 0; c < 16; ++c) {
+            const uint4 x = *reinterpret_cast<const uint4*>(at[c >> 3] + (((c + lane) & 7) << 4));
+            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) seen[i] = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&w[i]), zero, seen[i]);
+          }
+          const __nv_bfloat162 all = __hadd2(__hadd2(seen[0], seen[1]), __hadd2(seen[2], seen[3]));
+          const bool finite = __low2float(all) == 0.f && __high2float(all) == 0.f;
+          const bool outside = row >= left;
+          const uint32_t bad = __ballot_sync(0xffffffffu, !finite && !outside);
+          if (lane == 0) S.bad[which][k] = bad;
+          if (outside || !finite) {
+            wrote = true;
+#pragma unroll
+            for (int c = 0; c < 16; ++c)
+              *reinterpret_cast<uint4*>(at[c >> 3] + (((c + lane) & 7) << 4)) = make_uint4(0, 0, 0, 0);
+          }
+        }
+        if (__any_sync(0xffffffffu, wrote)) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&S.v_clean[which]);
+      }
+    } else {
+      // --------------------------------------------------------- tcgen05 issuers, as in the dense kernel
+      constexpr uint32_t idesc_qk = umma_idesc(kDF32, kFmtBF16, kFmtBF16, 0, 0, kTile, kTile);
+      constexpr uint32_t idesc_pv = umma_idesc(kDF32, kFmtBF16, kFmtBF16, 0, 1, kTile, 128);
+      auto full_parity = [](int i) { return (uint32_t)((i / kStages) & 1); };
+      auto spin = [&](uint64_t* bar, uint32_t parity, uint32_t bit) { return warp_poll(bar, parity, abort_flag, status, bit); };
+      auto rest = [&](uint64_t* bar, uint32_t parity, uint32_t bit) { return warp_rest(bar, parity, abort_flag, status, bit); };
+      if (warp == kMmaWarp) {
+        const uint64_t desc_k_major = umma_smem_desc(0, 16, 1024, kSwizzle128B);
+        const uint64_t q_desc[2] = {desc_k_major + (smem_u32(S.q[0]) >> 4), desc_k_major + (smem_u32(S.q[1]) >> 4)};
+        const uint64_t kv_k_desc = desc_k_major + (smem_u32(S.kv[0]) >> 4);
+        const uint32_t d = tmem + kColS;
+        uint32_t issued = 0;
+        auto qk = [&](int t, int j, uint64_t* taken, uint32_t taken_parity) -> bool {  // S = Q_t K_j^T
+          const int ik = 2 * j, sk = ik % kStages;
+          const uint64_t a0 = t ? q_desc[1] : q_desc[0], b0 = kv_k_desc + sk * (kTileBytes >> 4);
+          const uint64_t a1 = a0 + 2, a2 = a0 + 4, a3 = a0 + 6, a4 = a0 + (kHalfBytes >> 4), a5 = a4 + 2, a6 = a4 + 4, a7 = a4 + 6;
+          const uint64_t b1 = b0 + 2, b2 = b0 + 4, b3 = b0 + 6, b4 = b0 + (kHalfBytes >> 4), b5 = b4 + 2, b6 = b4 + 4, b7 = b4 + 6;
+          if (t == 0 && !rest(&S.kv_full[sk], full_parity(ik), kWaitTimeoutLoad)) return false;
+          if (taken && !spin(taken, taken_parity, kWaitTimeoutSoftmax)) return false;
+          tc_fence_after();
+          if (elect_one()) {
+            asm volatile(
+                "{\n\t.reg .pred p0, p1;\n\t"
+                "setp.ne.b32 p0, 0, 0;\n\tsetp.eq.b32 p1, 0, 0;\n\t"
+                "tcgen05.mma.cta_group::1.kind::f16 [%0], %2, %10, %1, p0;\n\t"
+                "tcgen05.mma.cta_group::1.kind::f16 [%0], %3, %11, %1, p1;\n\t"
+                "tcgen05.mma.cta_group::1.kind::f16 [%0], %4, %12, %1, p1;\n\t"
+                "tcgen05.mma.cta_group::1.kind::f16 [%0], %5, %13, %1, p1;\n\t"
+                "tcgen05.mma.cta_group::1.kind::f16 [%0], %6, %14, %1, p1;\n\t"
+                "tcgen05.mma.cta_group::1.kind::f16 [%0], %7, %15, %1, p1;\n\t"
+                "tcgen05.mma.cta_group::1.kind::f16 [%0], %8, %16, %1, p1;\n\t"
+                "tcgen05.mma.cta_group::1.kind::f16 [%0], %9, %17, %1, p1;\n\t}" ::"r"(d),
+                "r"(idesc_qk), "l"(a0), "l"(a1), "l"(a2), "l"(a3), "l"(a4), "l"(a5), "l"(a6), "l"(a7), "l"(b0), "l"(b1),
+                "l"(b2), "l"(b3), "l"(b4), "l"(b5), "l"(b6), "l"(b7)
+                : "memory");
+            tc_commit(&S.s_full[t]);
+            if (t == 1 || !two) tc_commit(&S.kv_empty[sk]);  // last reader of K_j
+            *reinterpret_cast<volatile uint32_t*>(&S.qk_issued) = issued + 1;
+          }
+          ++issued;
+          return true;
+        };
+        bool ok = rest(&S.q_full, 0, kWaitTimeoutLoad) && qk(0, 0, nullptr, 0);
+        for (int j = 0; ok && j < n_kv; ++j) {
+          if (two && !(ok = qk(1, j, &S.s_taken[0], j & 1))) break;
+          if (j + 1 < n_kv && !(ok = qk(0, j + 1, &S.s_taken[two ? 1 : 0], j & 1))) break;
+        }
+      } else {
+        const uint64_t desc_n_major = umma_smem_desc(0, kHalfBytes, 1024, kSwizzle128B);
+        const uint64_t kv_n_desc = desc_n_major + (smem_u32(S.kv[0]) >> 4);
+        const uint32_t total_qk = (two ? 2 : 1) * n_kv;
+        // O_t += P_t(j)[:, 64 half : 64 half + 64] V_j[64 half : 64 half + 64, :], after `gate` score groups
+        auto pv_half = [&](int t, int j, int half, uint32_t gate) -> bool {
+          const int iv = 2 * j + 1, sv = iv % kStages;
+          const uint64_t b0 = kv_n_desc + sv * (kTileBytes >> 4) + half * (4 * 2048 >> 4);
+          const uint64_t b1 = b0 + (2048 >> 4), b2 = b0 + 2 * (2048 >> 4), b3 = b0 + 3 * (2048 >> 4);
+          const uint32_t d = tmem + kColO + t * kTile, a0 = tmem + kColP + t * 64 + half * 32;
+          const uint32_t accumulate = (j > 0 || half > 0) ? 1u : 0u;
+          if (gate > total_qk) gate = total_qk;
+          if (half == 0 && !rest(&S.kv_full[sv], full_parity(iv), kWaitTimeoutLoad)) return false;
+          if (half == 0 && !rest(&S.v_clean[j & 1], (j >> 1) & 1, kWaitTimeoutLoad)) return false;
+          if (!spin(&S.p_full[t][half], j & 1, kWaitTimeoutSoftmax)) return false;
+          if (!warp_wait_counter(&S.qk_issued, gate, abort_flag, status, kWaitTimeoutMma)) return false;
+          tc_fence_after();
+          if (elect_one()) {
+            asm volatile(
+                "{\n\t.reg .pred p0, p1;\n\t"
+                "setp.ne.b32 p0, %2, 0;\n\tsetp.eq.b32 p1, 0, 0;\n\t"
+                "tcgen05.mma.cta_group::1.kind::f16 [%0], [%3], %7, %1, p0;\n\t"
+                "tcgen05.mma.cta_group::1.kind::f16 [%0], [%4], %8, %1, p1;\n\t"
+                "tcgen05.mma.cta_group::1.kind::f16 [%0], [%5], %9, %1, p1;\n\t"
+                "tcgen05.mma.cta_group::1.kind::f16 [%0], [%6], %10, %1, p1;\n\t}" ::"r"(d),
+                "r"(idesc_pv), "r"(accumulate), "r"(a0), "r"(a0 + 8), "r"(a0 + 16), "r"(a0 + 24), "l"(b0), "l"(b1), "l"(b2),
+                "l"(b3)
+                : "memory");
+            if (half == 1) {
+              tc_commit(&S.pv_done[t]);
+              if (t == 1 || !two) tc_commit(&S.kv_empty[sv]);  // last reader of V_j
+            }
+          }
+          return true;
+        };
+        bool ok = true;
+        if (two) {
+          for (int j = 0; ok && j < n_kv; ++j) {
+            ok = pv_half(0, j, 0, 2 * j + 3) && pv_half(0, j, 1, 2 * j + 4) && pv_half(1, j, 0, 2 * j + 4) &&
+                 pv_half(1, j, 1, 2 * j + 5);
+          }
+        } else {
+          for (int j = 0; ok && j < n_kv; ++j) ok = pv_half(0, j, 0, j + 2) && pv_half(0, j, 1, j + 2);
+        }
+      }
+    }
+  } else {
+    // ------------------------------------------------- softmax + epilogue warps
+    reg_alloc<kSoftmaxRegs>();
+    auto poll = [&](uint64_t* bar, uint32_t parity, uint32_t bit) { return warp_poll(bar, parity, abort_flag, status, bit); };
+    const int t = warp >> 2;
+    if (unit_rows > 0 && (t == 0 || two)) {
+      const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
+      const uint32_t s_addr = tmem + lane_base + kColS;
+      const uint32_t p_addr = tmem + lane_base + kColP + t * 64;
+      const uint32_t o_addr = tmem + lane_base + kColO + t * kTile;
+      const int query = S.unit.query0 + t * kTile + (warp & 3) * 32 + lane;
+      const int visible = S.unit.sight.visible(query) - kv_begin * kTile;  // keys of this CTA's that the row sees
+      const int whole = S.unit.sight.visible(S.unit.query0 + t * kTile) / kTile - kv_begin;
+      // a capped score stays in units of the cap until the exponential, a biased one is turned into log2 units at once
+      const float sc = BIAS ? (CAP ? P.to_log2 : P.scale * P.to_log2) : 1.f;
+      const float unit_log2 = BIAS ? 1.f : CAP ? P.to_log2 : P.scale * P.to_log2;
+      const float slope = BIAS ? P.slopes[head] * 1.4426950408889634f : 0.f;
+      const int position = BIAS ? S.unit.sight.ahead + query - kv_begin * kTile : 0;  // relative to this CTA's first key
+      float m_used = 0.f;
+      bool spoilt = false;            // the row sees a value that is not finite
+      uint64_t la = 0ull, lb = 0ull;  // four partial row sums as two fp32 pairs
+      bool ok = true;
+      for (int j = 0; j < n_kv; ++j) {
+        ok = warp_rest(&S.s_full[t], j & 1, abort_flag, status, kWaitTimeoutMma);
+        if (!ok) break;
+        tc_fence_after();
+        uint32_t s[128];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld32(s_addr + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&s[32 * c]));
+        tc_wait_ld();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&S.s_taken[t]);
+        if constexpr (CAP) {
+          float most = 0.f;
+#pragma unroll
+          for (int i = 0; i < 128; ++i) most = fmaxf(most, fabsf(__uint_as_float(s[i])));
+          if (__all_sync(0xffffffffu, most * P.scale <= 1.f)) {
+            const uint64_t scale2 = pack2(P.scale, P.scale);
+#pragma unroll
+            for (int i = 0; i < 128; i += 2) {
+              float a, b;
+              unpack2(tanh_small2(mul2(pack2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), scale2)), a, b);
+              s[i] = __float_as_uint(a), s[i + 1] = __float_as_uint(b);
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 128; ++i) s[i] = __float_as_uint(tanh_any(__uint_as_float(s[i]) * P.scale));
+          }
+        }
+        if constexpr (BIAS) {
+          const int key = j * kTile;
+          const int first = __shfl_sync(0xffffffffu, position, 0);  // of the warp's rows
+          const bool below = key + kTile - 1 <= first, above = key >= first + 31;
+          if (below || above) {
+            // all keys on one side of all rows: the distance is linear in the key
+            const float a = below ? slope : -slope;
+            const float base = a * static_cast<float>(key - position);
+            const uint64_t a2 = pack2(a, a), base2 = pack2(base, base), sc2 = pack2(sc, sc);
+#pragma unroll
+            for (int i = 0; i < 128; i += 2) {
+              float x, y;
+              unpack2(fma2(pack2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), sc2, fma2(pack2(i, i + 1), a2, base2)), x, y);
+              s[i] = __float_as_uint(x), s[i + 1] = __float_as_uint(y);
+            }
+          } else {
+            const float from = static_cast<float>(position - key);
+#pragma unroll
+            for (int i = 0; i < 128; ++i) {
+              const float distance = fabsf(from - static_cast<float>(i));
+              s[i] = __float_as_uint(fmaf(__uint_as_float(s[i]), sc, -slope * distance));
+            }
+          }
+        }
+        if (j >= whole) {
+          const int valid = visible - j * kTile;
+#pragma unroll
+          for (int i = 0; i < 128; ++i)
+            if (i >= valid) s[i] = 0xff800000u;  // -inf
+        }
+        float mx0 = __uint_as_float(s[0]), mx1 = __uint_as_float(s[1]);
+        float mx2 = __uint_as_float(s[2]), mx3 = __uint_as_float(s[3]);
+#pragma unroll
+        for (int i = 4; i < 124; i += 8) {
+          mx0 = max3(mx0, __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+          mx1 = max3(mx1, __uint_as_float(s[i + 2]), __uint_as_float(s[i + 3]));
+          mx2 = max3(mx2, __uint_as_float(s[i + 4]), __uint_as_float(s[i + 5]));
+          mx3 = max3(mx3, __uint_as_float(s[i + 6]), __uint_as_float(s[i + 7]));
+        }
+        mx0 = max3(mx0, __uint_as_float(s[124]), __uint_as_float(s[125]));
+        mx1 = max3(mx1, __uint_as_float(s[126]), __uint_as_float(s[127]));
+        const float mx = fmaxf(max3(mx0, mx1, mx2), mx3) * unit_log2;
+        bool pv_waited = j == 0;  // P_t and O_t are untouched by the tensor core before the first PV
+        if (j == 0) {
+          m_used = fmaxf(mx, kLowestMaximum);
+        } else if (__any_sync(0xffffffffu, mx > m_used + kRescaleThreshold)) {
+          const float m_new = fmaxf(m_used, mx);
+          const float alpha = ex2(m_used - m_new);
+          const uint64_t alpha2 = pack2(alpha, alpha);
+          la = fma2(la, alpha2, 0ull);
+          lb = fma2(lb, alpha2, 0ull);
+          // O_t += P_t V_{j-1} must have completed; the next PV waits for our arrival on p_full.
+          ok = poll(&S.pv_done[t], (j - 1) & 1, kWaitTimeoutMma);
+          if (!ok) break;
+          pv_waited = true;
+          tc_fence_after();
+          tmem_scale_rows(o_addr, alpha);
+          m_used = m_new;
+        }
+        if (j >= partly) {
+          // which of the tile's rows of V were not finite; before the probabilities go, as the note is overwritten after them
+          ok = poll(&S.v_clean[j & 1], (j >> 1) & 1, kWaitTimeoutLoad);
+          if (!ok) break;
+          const int valid = visible - j * kTile;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t bad = *const_cast<const volatile uint32_t*>(&S.bad[j & 1][k]);
+            const int seen = clamped(valid - 32 * k, 0, 32);
+            spoilt |= (bad & (seen == 32 ? ~0u : (1u << seen) - 1u)) != 0;
+          }
+        }
+        const uint64_t scale2 = pack2(unit_log2, unit_log2);
+        const uint64_t neg_m2 = pack2(-m_used, -m_used);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          uint32_t p[32];
+#pragma unroll
+          for (int i = 0; i < 64; i += 4) {
+            const int e = half * 64 + i;
+            float x0, x1, x2, x3;
+            unpack2(fma2(pack2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), scale2, neg_m2), x0, x1);
+            unpack2(fma2(pack2(__uint_as_float(s[e + 2]), __uint_as_float(s[e + 3])), scale2, neg_m2), x2, x3);
+            const float a = ex2(x0), b = ex2(x1), c = ex2(x2), d = ex2(x3);
+            la = add2(la, pack2(a, b));
+            lb = add2(lb, pack2(c, d));
+            // probabilities go to bf16 for the value MMAs, as V is; the row sum is taken before the rounding
+            p[i / 2] = pack_bf16(a, b);
+            p[i / 2 + 1] = pack_bf16(c, d);
+          }
+          if (half == 0 && !pv_waited) {
+            // the previous tile's PV still reads P_t until this completes (normally long ago)
+            ok = poll(&S.pv_done[t], (j - 1) & 1, kWaitTimeoutMma);
+            if (!ok) break;
+            tc_fence_after();
+          }
+          tmem_st32(p_addr + 32 * half, p);
+          tc_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&S.p_full[t][half]);
+        }
+        if (!ok) break;
+      }
+      if (ok && n_kv > 0) ok = poll(&S.pv_done[t], (n_kv - 1) & 1, kWaitTimeoutMma);
+      if (ok) {
+        tc_fence_after();
+        float l0, l1, l2, l3;
+        unpack2(la, l0, l1);
+        unpack2(lb, l2, l3);
+        const float l = (l0 + l1) + (l2 + l3);
+        const float inv = spoilt ? __uint_as_float(0x7fffffffu) : l == 0.f ? 0.f : 1.0f / l;
+        const int in_unit = t * kTile + (warp & 3) * 32 + lane;
+        const int row = S.unit.row0 + in_unit;
+        bool store = in_unit < S.unit.rows;
+        const size_t rows = static_cast<size_t>(P.rows);
+        const size_t at = (static_cast<size_t>(piece) * P.heads + head) * rows + row;  // of a partial row
+        store = store && NOB_CHECK(row >= 0 && row < P.rows && head + P.head_offset < P.total_heads, status);
+        if (P.splits > 1 && store) P.lse[at] = spoilt ? __uint_as_float(0x7fffffffu) : m_used + log2f(l);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t o[32];
+          if (n_kv > 0) {
+            tmem_ld32(o_addr + 32 * c, o);
+            tc_wait_ld();
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = 0;
+          }
+          if (store) {
+            float r[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) r[i] = __uint_as_float(o[i]) * inv;
+            if (P.splits > 1) {
+              float4* dst = reinterpret_cast<float4*>(P.partial + at * 128 + 32 * c);
+#pragma unroll
+              for (int i = 0; i < 8; ++i) dst[i] = make_float4(r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
+            } else {
+              __nv_bfloat16* dst = P.output + (static_cast<size_t>(row) * P.total_heads + head + P.head_offset) * 128 + 32 * c;
+#pragma unroll
+              for (int i = 0; i < 32; i += 8)
+                *reinterpret_cast<uint4*>(dst + i) =
+                    make_uint4(pack_bf16(r[i], r[i + 1]), pack_bf16(r[i + 2], r[i + 3]), pack_bf16(r[i + 4], r[i + 5]),
+                               pack_bf16(r[i + 6], r[i + 7]));
+            }
+          }
+        }
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kProducerWarp) tmem_dealloc(tmem, kTmemCols);
+}
+
+// o = sum_z 2^(lse_z - max) o_z / sum_z 2^(lse_z - max).  A thread owns eight channels of a row; a row that no share gave any
+// weight gets zeros.
+__global__ void __launch_bounds__(256)
+join_shares_kernel(const KeyShares P) {
+  pdl_wait();
+  const long long item = blockIdx.x * 256ll + threadIdx.x;
+  const long long all = static_cast<long long>(P.heads) * P.rows;
+  const long long place = item >> 4;
+  if (place >= all) return;
+  const int head = static_cast<int>(place / P.rows), row = static_cast<int>(place - static_cast<long long>(head) * P.rows);
+  if (row < P.bounds[0] || row >= P.bounds[P.documents]) return;
+  float top = -INFINITY;
+  for (int z = 0; z < P.splits; ++z) top = fmaxf(top, P.lse[z * all + place]);
+  float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  float sum = 0.f;
+  for (int z = 0; z < P.splits; ++z) {
+    const long long at = z * all + place;
+    const float lse = P.lse[at];
+    if (lse == -INFINITY) continue;
+    const float w = exp2f(lse - top);
+    sum += w;
+    const float4* src = reinterpret_cast<const float4*>(P.partial + at * 128 + (item & 15) * 8);
+    const float4 x = src[0], y = src[1];
+    const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) acc[i] += w * v[i];
+  }
+  const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+  uint4 v;
+  v.x = pack_bf16(acc[0] * inv, acc[1] * inv);
+  v.y = pack_bf16(acc[2] * inv, acc[3] * inv);
+  v.z = pack_bf16(acc[4] * inv, acc[5] * inv);
+  v.w = pack_bf16(acc[6] * inv, acc[7] * inv);
+  *reinterpret_cast<uint4*>(P.output + (static_cast<size_t>(row) * P.total_heads + head + P.head_offset) * 128 + (item & 15) * 8) = v;
+}
+
+}  // namespace
+
+int launch_join_shares(const KeyShares& shares, void* stream) {
+  const long long items = static_cast<long long>(shares.rows) * shares.heads * 16;
+  return launch_pdl("attention (join of key shares)", join_shares_kernel, static_cast<unsigned>((items + 255) / 256), 256, 0,
+                    stream, shares);
+}
+
+}  // namespace nob200
+
+extern "C" size_t nob200_masked_bf16_attention_d128_workspace_bytes(int num_rows, int heads, int kv_splits) {
+  return num_rows <= 0 || heads <= 0 ? 0 : nob200::key_shares_bytes(num_rows, heads, kv_splits);
+}
+
+extern "C" int nob200_masked_bf16_attention_d128(int num_rows, int num_key_rows, int documents, int head_offset,
+                                                 const void* query, const void* key, const void* value, const void* bounds,
+                                                 const void* key_bounds, const void* prefix, const void* slopes,
+                                                 void* output, int heads, int kv_heads, int total_heads, int causal,
+                                                 float scale, float cap, int unit_rows, int kv_splits, void* workspace,
+                                                 size_t workspace_bytes, void* stream) {
+  using namespace nob200;
+  const char* name = "masked_bf16_attention_d128";
+  NOB_REQUIRE(num_rows > 0 && num_key_rows > 0 && documents > 0 && heads > 0 && kv_heads > 0 && total_heads > 0,
+              "%s: sizes must be positive", name);
+  NOB_REQUIRE(heads % kv_heads == 0, "%s: %d heads cannot share %d key heads evenly", name, heads, kv_heads);
+  NOB_REQUIRE(head_offset >= 0 && head_offset <= total_heads - heads, "%s: head_offset %d outside [0, %d]", name,
+              head_offset, total_heads - heads);
+  NOB_REQUIRE(query && key && value && bounds && key_bounds && output, "%s: NULL tensor", name);
+  NOB_REQUIRE(reinterpret_cast<uintptr_t>(output) % 16 == 0, "%s: output %p is not 16-byte aligned", name, output);
+  NOB_REQUIRE(scale > 0.f && scale <= 1e30f, "%s: scale %g must be positive and finite", name, scale);
+  NOB_REQUIRE(cap >= 0.f && cap <= 1e30f, "%s: cap %g must be finite, 0 for none", name, cap);
+  NOB_REQUIRE(unit_rows == kTile || unit_rows == 2 * kTile, "%s: unit_rows must be 128 or 256 (got %d)", name, unit_rows);
+  NOB_REQUIRE(kv_splits >= 1 && kv_splits <= 64, "%s: kv_splits %d outside [1, 64]", name, kv_splits);
+  const long long slots = most_units(num_rows, documents, unit_rows);
+  const long long blocks = slots * heads * kv_splits;
+  NOB_REQUIRE(blocks <= 0x7fffffffll, "%s: %lld units x %d heads x %d key shares exceed the grid limit", name, slots, heads, kv_splits);
+  const size_t need = key_shares_bytes(num_rows, heads, kv_splits);
+  NOB_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && reinterpret_cast<uintptr_t>(workspace) % 16 == 0),
+              "%s: %zu B of 16-byte aligned workspace required for %d key shares, %zu B given", name, need, kv_splits, workspace_bytes);
+
+  MaskedParams P = {};
+  P.status = status_word_device_ptr();
+  if (!P.status) return fail(kCudaError, "%s: no current CUDA device", name);
+  P.bounds = static_cast<const int*>(bounds), P.key_bounds = static_cast<const int*>(key_bounds);
+  P.prefix = static_cast<const int*>(prefix), P.slopes = static_cast<const float*>(slopes);
+  P.output = static_cast<__nv_bfloat16*>(output);
+  P.rows = num_rows, P.key_rows = num_key_rows, P.documents = documents;
+  P.heads = heads, P.group = heads / kv_heads, P.total_heads = total_heads, P.head_offset = head_offset;
+  P.slots = static_cast<int>(slots), P.unit_rows = unit_rows, P.splits = kv_splits, P.causal = causal != 0;
+  const float log2e = 1.4426950408889634f;
+  P.scale = cap > 0.f ? scale / cap : scale;
+  P.to_log2 = cap > 0.f ? cap * log2e : log2e;
+  if (need) {
+    P.partial = static_cast<float*>(workspace);
+    P.lse = P.partial + static_cast<size_t>(kv_splits) * heads * num_rows * 128;
+  }
+
+  CUtensorMap mq, mk, mv;
+  int rc;
+  const uint64_t pitch = static_cast<uint64_t>(heads) * 256, key_pitch = static_cast<uint64_t>(kv_heads) * 256;
+  if ((rc = make_tensor_map_3d(&mq, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, query, 128, heads, num_rows, 256, pitch, 64, 1, kTile)))
+    return rc;
+  if ((rc = make_tensor_map_3d(&mk, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, key, 128, kv_heads, num_key_rows, 256, key_pitch, 64, 1, kTile)))
+    return rc;
+  if ((rc = make_tensor_map_3d(&mv, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, value, 128, kv_heads, num_key_rows, 256, key_pitch, 64, 1, kTile)))
+    return rc;
+
+  auto kernel = cap > 0.f ? (slopes ? fa_fwd_masked_bf16_kernel<true, true> : fa_fwd_masked_bf16_kernel<true, false>)
+                          : (slopes ? fa_fwd_masked_bf16_kernel<false, true> : fa_fwd_masked_bf16_kernel<false, false>);
+  const size_t smem = sizeof(Shared) + 1024;
+  cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (err != cudaSuccess)
+    return fail(kCudaError, "%s: cannot reserve %zu B of shared memory: %s", name, smem, cudaGetErrorString(err));
+  if ((rc = launch_pdl(name, kernel, static_cast<unsigned>(blocks), kThreads, smem, stream, mq, mk, mv, P))) return rc;
+  if (kv_splits == 1) return kOk;
+  return launch_join_shares({P.bounds, P.partial, P.lse, P.output, documents, num_rows, heads, total_heads, head_offset, kv_splits}, stream);
+}

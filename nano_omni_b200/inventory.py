@@ -39,6 +39,7 @@ def workloads(tokens: int, heads: int) -> list[tuple[str, dict, dict]]:
     """(kernel name, Workload fields, tune options) of the attention path at one shape."""
     t, h = tokens, heads
     sparse = {"mask_density": 0.16}
+    cached = {"sequences": 1, "max_blocks": -(-t // 64), "num_blocks": -(-t // 64), "kv_heads": h}
     return [
         # the projections around attention at the reference's widths (model 5376, 56 heads x 128 = 7168)
         ("int8_rowwise", {"num_tokens": t, "columns": 5376}, {}),
@@ -69,6 +70,15 @@ def workloads(tokens: int, heads: int) -> list[tuple[str, dict, dict]]:
         ("sol_int8_fp8_attention_d128", {"num_tokens": t, "heads": h, "total_heads": h}, sparse),
         ("sol_nvfp4_attention_d128", {"num_query_tokens": t, "num_kv_tokens": t, "heads": h, "total_heads": h}, sparse),
         ("sol_nvfp4_finalize", {"num_tokens": t, "heads": h, "total_heads": h}, sparse),
+        # four packed documents; the same tokens as one cached sequence, appended, read back and attended by one token
+        (
+            "masked_bf16_attention_d128",
+            {"num_rows": t, "num_key_rows": t, "documents": 4, "heads": h, "kv_heads": h, "total_heads": h, "causal": True},
+            {},
+        ),
+        ("int8_cache_append_d128", {"num_rows": t, **cached}, {}),
+        ("int8_cache_read_d128", {"capacity": t, **cached}, {}),
+        ("int8_cache_attention_d128", {"num_rows": 1, "heads": h, "total_heads": h, **cached}, {}),
     ]
 
 

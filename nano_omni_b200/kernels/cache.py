@@ -1,0 +1,293 @@
+"""A cache of keys and values in 8 bits: append, read back, and the attention of a few queries over it.
+
+No counterpart in the reference.  Blocks of 64 tokens, int8 codes ``[num_blocks, kv_heads, 64, 128]`` and one fp32 scale per
+block and head ``[num_blocks, kv_heads]`` for each of K and V; ``table`` int32 ``[sequences, max_blocks]`` names the block
+that holds tokens ``64 b .. 64 b + 63`` of a sequence, ``lengths`` int32 ``[sequences]`` how many tokens it has.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import dataclasses
+
+from pydantic import Field
+
+from nano_omni_b200 import _lib
+from nano_omni_b200.core import Arguments, Config, DType, Kernel, MmaType, TensorDesc, Workload, require_tensor
+from nano_omni_b200.kernels.masked import DEFAULT_SCALE, check_masks, share_workspace_bytes
+
+BLOCK = 64  # tokens of a block
+
+
+def _cache_shape(arguments) -> tuple[int, int, int, int]:
+    """(blocks, key heads, sequences, blocks of a sequence) of the cache tensors, checked against one another."""
+    a = arguments
+    assert len(a.key_codes.shape) == 4 and len(a.table.shape) == 2, "codes have rank 4, the table rank 2"
+    num_blocks, kv_heads = a.key_codes.shape[:2]
+    sequences, max_blocks = a.table.shape
+    for what, codes, scales in (("key", a.key_codes, a.key_scales), ("value", a.value_codes, a.value_scales)):
+        require_tensor(codes, DType.I8, (num_blocks, kv_heads, BLOCK, 128), f"{what} codes")
+        require_tensor(scales, DType.F32, (num_blocks, kv_heads), f"{what} scales")
+    require_tensor(a.table, DType.I32, (sequences, max_blocks), "table")
+    require_tensor(a.lengths, DType.I32, (sequences,), "lengths")
+    return num_blocks, kv_heads, sequences, max_blocks
+
+
+def _empty_cache(w) -> tuple[TensorDesc, ...]:
+    """key codes, value codes, key scales, value scales, table, lengths"""
+    codes = TensorDesc.empty(DType.I8, (w.num_blocks, w.kv_heads, BLOCK, 128))
+    scales = TensorDesc.empty(DType.F32, (w.num_blocks, w.kv_heads))
+    table = TensorDesc.empty(DType.I32, (w.sequences, w.max_blocks))
+    return codes, codes, scales, scales, table, TensorDesc.empty(DType.I32, (w.sequences,))
+
+
+def _full_cache(arguments) -> dict[str, list]:
+    """A table of distinct blocks, as far as there are any, and sequences that fill theirs."""
+    num_blocks, _, sequences, max_blocks = _cache_shape(arguments)
+    table = [[(s * max_blocks + b) % num_blocks for b in range(max_blocks)] for s in range(sequences)]
+    return {"table": table, "lengths": [max_blocks * BLOCK] * sequences}
+
+
+class CacheWorkload(Workload):
+    sequences: int = Field(gt=0)
+    max_blocks: int = Field(gt=0)
+    num_blocks: int = Field(gt=0)
+    kv_heads: int = Field(gt=0)
+
+
+class CacheConfig(Config):
+    pass
+
+
+# ------------------------------------------------------------------ append
+class CacheAppendWorkload(CacheWorkload):
+    num_rows: int = Field(gt=0)
+
+
+@dataclasses.dataclass(frozen=True, slots=True)
+class CacheAppendArguments(Arguments):
+    key: TensorDesc
+    value: TensorDesc
+    bounds: TensorDesc
+    table: TensorDesc
+    lengths: TensorDesc
+    key_codes: TensorDesc
+    key_scales: TensorDesc
+    value_codes: TensorDesc
+    value_scales: TensorDesc
+
+    def dynamic_parameters(self) -> tuple[tuple[str, int], ...]:
+        return (("num_rows", self.key.shape[0]),)
+
+    def index_values(self) -> dict[str, list]:
+        rows, sequences = self.key.shape[0], self.bounds.shape[0] - 1
+        return _full_cache(self) | {"bounds": [rows * s // sequences for s in range(sequences + 1)]}
+
+
+class CacheAppendKernel(Kernel[CacheAppendArguments, CacheAppendWorkload, CacheConfig]):
+    """``key`` and ``value`` bf16 ``[rows, kv_heads, 128]`` become the last tokens of their sequences; ``lengths`` counts them."""
+
+    name = "int8_cache_append_d128"
+    symbol = "nob200_int8_cache_append_d128"
+
+    @classmethod
+    def make_arguments(cls, workload: CacheAppendWorkload) -> CacheAppendArguments:
+        key_codes, value_codes, key_scales, value_scales, table, lengths = _empty_cache(workload)
+        rows = TensorDesc.empty(DType.BF16, (workload.num_rows, workload.kv_heads, 128))
+        bounds = TensorDesc.empty(DType.I32, (workload.sequences + 1,))
+        return CacheAppendArguments(rows, rows, bounds, table, lengths, key_codes, key_scales, value_codes, value_scales)
+
+    @classmethod
+    def make_config(cls, workload: CacheAppendWorkload) -> CacheConfig:
+        return CacheConfig()
+
+    @classmethod
+    def make_workload(cls, arguments: CacheAppendArguments) -> CacheAppendWorkload:
+        num_blocks, kv_heads, sequences, max_blocks = _cache_shape(arguments)
+        rows = arguments.key.shape[0]
+        require_tensor(arguments.key, DType.BF16, (rows, kv_heads, 128), "key")
+        require_tensor(arguments.value, DType.BF16, (rows, kv_heads, 128), "value")
+        require_tensor(arguments.bounds, DType.I32, (sequences + 1,), "bounds")
+        return CacheAppendWorkload(
+            num_rows=rows, sequences=sequences, max_blocks=max_blocks, num_blocks=num_blocks, kv_heads=kv_heads
+        )
+
+    def _launch(self, function, stream: int) -> int:
+        a, w = self.arguments, self.workload
+        return function(
+            ctypes.c_int(w.num_rows), ctypes.c_int(w.sequences), ctypes.c_int(w.max_blocks), ctypes.c_int(w.num_blocks),
+            _lib.ptr(a.key), _lib.ptr(a.value), _lib.ptr(a.bounds), _lib.ptr(a.table), _lib.ptr(a.lengths),
+            _lib.ptr(a.key_codes), _lib.ptr(a.key_scales), _lib.ptr(a.value_codes), _lib.ptr(a.value_scales),
+            ctypes.c_int(w.kv_heads), ctypes.c_void_p(stream),
+        )  # fmt: skip
+
+
+# ------------------------------------------------------------------ read
+class CacheReadWorkload(CacheWorkload):
+    capacity: int = Field(gt=0)
+
+
+@dataclasses.dataclass(frozen=True, slots=True)
+class CacheReadArguments(Arguments):
+    key_codes: TensorDesc
+    value_codes: TensorDesc
+    key_scales: TensorDesc
+    value_scales: TensorDesc
+    table: TensorDesc
+    lengths: TensorDesc
+    key: TensorDesc
+    value: TensorDesc
+    bounds: TensorDesc
+
+    def dynamic_parameters(self) -> tuple[tuple[str, int], ...]:
+        return (("capacity", self.key.shape[0]),)
+
+    def index_values(self) -> dict[str, list]:
+        return _full_cache(self) | {"bounds": [0] * self.bounds.shape[0]}
+
+
+class CacheReadKernel(Kernel[CacheReadArguments, CacheReadWorkload, CacheConfig]):
+    """The sequences' tokens as bf16 rows ``[capacity, kv_heads, 128]``, one sequence behind the other, and their bounds."""
+
+    name = "int8_cache_read_d128"
+    symbol = "nob200_int8_cache_read_d128"
+
+    @classmethod
+    def make_arguments(cls, workload: CacheReadWorkload) -> CacheReadArguments:
+        rows = TensorDesc.empty(DType.BF16, (workload.capacity, workload.kv_heads, 128))
+        return CacheReadArguments(
+            *_empty_cache(workload), rows, rows, TensorDesc.empty(DType.I32, (workload.sequences + 1,))
+        )
+
+    @classmethod
+    def make_config(cls, workload: CacheReadWorkload) -> CacheConfig:
+        return CacheConfig()
+
+    @classmethod
+    def make_workload(cls, arguments: CacheReadArguments) -> CacheReadWorkload:
+        num_blocks, kv_heads, sequences, max_blocks = _cache_shape(arguments)
+        capacity = arguments.key.shape[0]
+        require_tensor(arguments.key, DType.BF16, (capacity, kv_heads, 128), "key")
+        require_tensor(arguments.value, DType.BF16, (capacity, kv_heads, 128), "value")
+        require_tensor(arguments.bounds, DType.I32, (sequences + 1,), "bounds")
+        return CacheReadWorkload(
+            capacity=capacity, sequences=sequences, max_blocks=max_blocks, num_blocks=num_blocks, kv_heads=kv_heads
+        )
+
+    def _launch(self, function, stream: int) -> int:
+        a, w = self.arguments, self.workload
+        return function(
+            ctypes.c_int(w.capacity), ctypes.c_int(w.sequences), ctypes.c_int(w.max_blocks), ctypes.c_int(w.num_blocks),
+            _lib.ptr(a.key_codes), _lib.ptr(a.value_codes), _lib.ptr(a.key_scales), _lib.ptr(a.value_scales),
+            _lib.ptr(a.table), _lib.ptr(a.lengths), _lib.ptr(a.key), _lib.ptr(a.value), _lib.ptr(a.bounds),
+            ctypes.c_int(w.kv_heads), ctypes.c_void_p(stream),
+        )  # fmt: skip
+
+
+# ------------------------------------------------------------------ attention
+class CacheAttentionWorkload(CacheWorkload):
+    num_rows: int = Field(gt=0)
+    heads: int = Field(gt=0)
+    total_heads: int = Field(gt=0)
+    causal: bool = True
+    use_prefix: bool = False
+    use_slopes: bool = False
+    cap: float = Field(default=0.0, ge=0, allow_inf_nan=False)
+    scale: float = Field(default=DEFAULT_SCALE, gt=0, allow_inf_nan=False)
+
+
+def plan_cache_shares(num_rows: int, sequences: int, cached_tokens: int, heads: int, kv_heads: int, sm_count: int = 148) -> int:
+    """Shares of a sequence's blocks, so that the CTAs (two per SM) come to some four rounds of the SMs, and a share still is a
+    block for each of a CTA's four warps."""
+    tiles = max(1, min(num_rows * heads // kv_heads, -(-num_rows * heads // kv_heads // 16) + sequences - 1))
+    blocks = -(-cached_tokens // sequences // BLOCK)
+    return max(1, min(64, blocks // 4, 8 * sm_count // (tiles * kv_heads)))
+
+
+class CacheAttentionConfig(Config):
+    kv_splits: int = Field(default=1, ge=1, le=64)  # > 1: a sequence's blocks over so many CTAs; needs `workspace`
+
+
+@dataclasses.dataclass(frozen=True, slots=True)
+class CacheAttentionArguments(Arguments):
+    query: TensorDesc
+    key_codes: TensorDesc
+    value_codes: TensorDesc
+    key_scales: TensorDesc
+    value_scales: TensorDesc
+    table: TensorDesc
+    lengths: TensorDesc
+    bounds: TensorDesc
+    prefix: TensorDesc | None
+    slopes: TensorDesc | None
+    output: TensorDesc
+    head_offset: int
+    causal: bool
+    scale: float = DEFAULT_SCALE
+    cap: float = 0.0
+    workspace: TensorDesc | None = None
+
+    def dynamic_parameters(self) -> tuple[tuple[str, int], ...]:
+        return (("num_rows", self.query.shape[0]), ("head_offset", self.head_offset))
+
+    def index_values(self) -> dict[str, list]:
+        rows, sequences = self.query.shape[0], self.bounds.shape[0] - 1
+        values = _full_cache(self) | {"bounds": [rows * s // sequences for s in range(sequences + 1)]}
+        return values | ({"prefix": [0] * sequences} if self.prefix is not None else {})
+
+
+class CacheAttentionKernel(Kernel[CacheAttentionArguments, CacheAttentionWorkload, CacheAttentionConfig]):
+    name = "int8_cache_attention_d128"
+    symbol = "nob200_int8_cache_attention_d128"
+
+    @classmethod
+    def make_arguments(cls, workload: CacheAttentionWorkload) -> CacheAttentionArguments:
+        w = workload
+        return CacheAttentionArguments(
+            TensorDesc.empty(DType.BF16, (w.num_rows, w.heads, 128)), *_empty_cache(w),
+            TensorDesc.empty(DType.I32, (w.sequences + 1,)),
+            TensorDesc.empty(DType.I32, (w.sequences,)) if w.use_prefix else None,
+            TensorDesc.empty(DType.F32, (w.heads,)) if w.use_slopes else None,
+            TensorDesc.empty(DType.BF16, (w.num_rows, w.total_heads, 128)), 0, w.causal, w.scale, w.cap,
+        )  # fmt: skip
+
+    @classmethod
+    def make_config(cls, workload: CacheAttentionWorkload) -> CacheAttentionConfig:
+        return CacheAttentionConfig()
+
+    @classmethod
+    def make_workload(cls, arguments: CacheAttentionArguments) -> CacheAttentionWorkload:
+        a = arguments
+        num_blocks, kv_heads, sequences, max_blocks = _cache_shape(a)
+        assert len(a.query.shape) == 3 and len(a.output.shape) == 3, "attention tensors have rank 3"
+        num_rows, heads, _ = a.query.shape
+        total_heads = a.output.shape[1]
+        require_tensor(a.query, DType.BF16, (num_rows, heads, 128), "query")
+        require_tensor(a.output, DType.BF16, (num_rows, total_heads, 128), "output")
+        assert kv_heads > 0 and heads % kv_heads == 0, f"{heads} heads cannot share {kv_heads} key heads evenly"
+        assert 0 <= a.head_offset <= total_heads - heads, "head slice ends past the output's heads"
+        check_masks(cls.name, a, sequences, heads)
+        return CacheAttentionWorkload(
+            num_rows=num_rows, heads=heads, total_heads=total_heads, sequences=sequences, max_blocks=max_blocks,
+            num_blocks=num_blocks, kv_heads=kv_heads, causal=a.causal, use_prefix=a.prefix is not None,
+            use_slopes=a.slopes is not None, cap=a.cap, scale=a.scale,
+        )  # fmt: skip
+
+    @classmethod
+    def tops(cls, arguments: CacheAttentionArguments) -> dict[MmaType, int]:
+        """Of full tables."""
+        w = cls.make_workload(arguments)
+        return {MmaType.F16F16F32: 4 * w.heads * 128 * w.num_rows * w.max_blocks * BLOCK}
+
+    def _launch(self, function, stream: int) -> int:
+        a, w, c = self.arguments, self.workload, self.config
+        need = share_workspace_bytes(w.num_rows, w.heads, c.kv_splits)
+        assert need == 0 or (a.workspace is not None and a.workspace.num_bytes >= need), "kv_splits > 1 needs workspace"
+        return function(
+            ctypes.c_int(w.num_rows), ctypes.c_int(w.sequences), ctypes.c_int(w.max_blocks), ctypes.c_int(w.num_blocks),
+            ctypes.c_int(a.head_offset), _lib.ptr(a.query), _lib.ptr(a.key_codes), _lib.ptr(a.value_codes),
+            _lib.ptr(a.key_scales), _lib.ptr(a.value_scales), _lib.ptr(a.table), _lib.ptr(a.lengths), _lib.ptr(a.bounds),
+            _lib.ptr(a.prefix), _lib.ptr(a.slopes), _lib.ptr(a.output), ctypes.c_int(w.heads), ctypes.c_int(w.kv_heads),
+            ctypes.c_int(w.total_heads), ctypes.c_int(int(a.causal)), ctypes.c_float(a.scale), ctypes.c_float(a.cap),
+            ctypes.c_int(c.kv_splits), _lib.ptr(a.workspace), ctypes.c_size_t(need), ctypes.c_void_p(stream),
+        )  # fmt: skip

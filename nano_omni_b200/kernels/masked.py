@@ -1,0 +1,144 @@
+"""bf16 attention over packed documents, bound to ``nob200_masked_bf16_attention_d128``.
+
+No counterpart in the reference, whose attention of this head width is dense and takes one sequence.  Document, causal
+and prefix masks, capped scores, a bias by distance and shared key heads; see the C header for the definition.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import dataclasses
+from typing import Literal
+
+from pydantic import Field
+
+from nano_omni_b200 import _lib
+from nano_omni_b200.core import Arguments, Config, DType, Kernel, MmaType, TensorDesc, Workload, require_tensor
+
+DEFAULT_SCALE = 128**-0.5
+
+
+class MaskedBf16AttentionWorkload(Workload):
+    num_rows: int = Field(gt=0)
+    num_key_rows: int = Field(gt=0)
+    documents: int = Field(gt=0)
+    heads: int = Field(gt=0)
+    kv_heads: int = Field(gt=0)
+    total_heads: int = Field(gt=0)
+    causal: bool = False
+    use_prefix: bool = False
+    use_slopes: bool = False
+    cap: float = Field(default=0.0, ge=0, allow_inf_nan=False)
+    scale: float = Field(default=DEFAULT_SCALE, gt=0, allow_inf_nan=False)
+
+
+class MaskedBf16AttentionConfig(Config):
+    unit_rows: Literal[128, 256] = 256  # query rows of a CTA
+    kv_splits: int = Field(default=1, ge=1, le=64)  # > 1: the keys of a unit over so many CTAs; needs `workspace`
+
+
+@dataclasses.dataclass(frozen=True, slots=True)
+class MaskedBf16AttentionArguments(Arguments):
+    query: TensorDesc
+    key: TensorDesc
+    value: TensorDesc
+    bounds: TensorDesc
+    key_bounds: TensorDesc
+    prefix: TensorDesc | None
+    slopes: TensorDesc | None
+    output: TensorDesc
+    head_offset: int
+    causal: bool
+    scale: float = DEFAULT_SCALE
+    cap: float = 0.0
+    workspace: TensorDesc | None = None
+
+    def dynamic_parameters(self) -> tuple[tuple[str, int], ...]:
+        return (("num_rows", self.query.shape[0]), ("num_key_rows", self.key.shape[0]), ("head_offset", self.head_offset))
+
+    def index_values(self) -> dict[str, list]:
+        """Plain contents of the index tensors, for launches outside a program: documents of one length."""
+        documents = self.bounds.shape[0] - 1
+        spread = lambda rows: [rows * d // documents for d in range(documents + 1)]  # noqa: E731
+        values = {"bounds": spread(self.query.shape[0]), "key_bounds": spread(self.key.shape[0])}
+        return values | ({"prefix": [0] * documents} if self.prefix is not None else {})
+
+
+def share_workspace_bytes(num_rows: int, heads: int, kv_splits: int) -> int:
+    """Scratch of divided keys: normalised fp32 rows and their log-sum-exp."""
+    return 0 if kv_splits <= 1 else kv_splits * heads * num_rows * 516
+
+
+def check_masks(name: str, arguments, documents: int, heads: int) -> None:
+    """Checks shared with the attention over a cache."""
+    require_tensor(arguments.bounds, DType.I32, (documents + 1,), "bounds")
+    if arguments.prefix is not None:
+        require_tensor(arguments.prefix, DType.I32, (documents,), "prefix")
+        assert arguments.causal, f"{name}: a prefix widens a causal mask; without one every key is seen"
+    if arguments.slopes is not None:
+        require_tensor(arguments.slopes, DType.F32, (heads,), "slopes")
+
+
+class MaskedBf16AttentionKernel(
+    Kernel[MaskedBf16AttentionArguments, MaskedBf16AttentionWorkload, MaskedBf16AttentionConfig]
+):
+    name = "masked_bf16_attention_d128"
+    symbol = "nob200_masked_bf16_attention_d128"
+
+    @classmethod
+    def make_arguments(cls, workload: MaskedBf16AttentionWorkload) -> MaskedBf16AttentionArguments:
+        w = workload
+        keys = TensorDesc.empty(DType.BF16, (w.num_key_rows, w.kv_heads, 128))
+        bounds = TensorDesc.empty(DType.I32, (w.documents + 1,))
+        return MaskedBf16AttentionArguments(
+            TensorDesc.empty(DType.BF16, (w.num_rows, w.heads, 128)), keys, keys, bounds, bounds,
+            TensorDesc.empty(DType.I32, (w.documents,)) if w.use_prefix else None,
+            TensorDesc.empty(DType.F32, (w.heads,)) if w.use_slopes else None,
+            TensorDesc.empty(DType.BF16, (w.num_rows, w.total_heads, 128)), 0, w.causal, w.scale, w.cap,
+        )  # fmt: skip
+
+    @classmethod
+    def make_config(cls, workload: MaskedBf16AttentionWorkload) -> MaskedBf16AttentionConfig:
+        return MaskedBf16AttentionConfig()
+
+    @classmethod
+    def make_workload(cls, arguments: MaskedBf16AttentionArguments) -> MaskedBf16AttentionWorkload:
+        a = arguments
+        for tensor in (a.query, a.key, a.output):
+            assert len(tensor.shape) == 3, "attention tensors have rank 3"
+        num_rows, heads, _ = a.query.shape
+        num_key_rows, kv_heads, _ = a.key.shape
+        total_heads = a.output.shape[1]
+        require_tensor(a.query, DType.BF16, (num_rows, heads, 128), "query")
+        require_tensor(a.key, DType.BF16, (num_key_rows, kv_heads, 128), "key")
+        require_tensor(a.value, DType.BF16, (num_key_rows, kv_heads, 128), "value")
+        require_tensor(a.output, DType.BF16, (num_rows, total_heads, 128), "output")
+        assert kv_heads > 0 and heads % kv_heads == 0, f"{heads} heads cannot share {kv_heads} key heads evenly"
+        assert 0 <= a.head_offset <= total_heads - heads, "head slice ends past the output's heads"
+        documents = a.bounds.shape[0] - 1
+        check_masks(cls.name, a, documents, heads)
+        require_tensor(a.key_bounds, DType.I32, (documents + 1,), "key_bounds")
+        return MaskedBf16AttentionWorkload(
+            num_rows=num_rows, num_key_rows=num_key_rows, documents=documents, heads=heads, kv_heads=kv_heads,
+            total_heads=total_heads, causal=a.causal, use_prefix=a.prefix is not None, use_slopes=a.slopes is not None,
+            cap=a.cap, scale=a.scale,
+        )  # fmt: skip
+
+    @classmethod
+    def tops(cls, arguments: MaskedBf16AttentionArguments) -> dict[MmaType, int]:
+        """Of documents of one length; half of the pairs under a causal mask."""
+        w = cls.make_workload(arguments)
+        return {MmaType.BF16BF16F32: 4 * w.heads * 128 * w.num_rows * w.num_key_rows // w.documents // (2 if w.causal else 1)}
+
+    def _launch(self, function, stream: int) -> int:
+        a, w, c = self.arguments, self.workload, self.config
+        need = share_workspace_bytes(w.num_rows, w.heads, c.kv_splits)
+        assert need == 0 or (a.workspace is not None and a.workspace.num_bytes >= need), "kv_splits > 1 needs workspace"
+        return function(
+            ctypes.c_int(w.num_rows), ctypes.c_int(w.num_key_rows), ctypes.c_int(w.documents), ctypes.c_int(a.head_offset),
+            _lib.ptr(a.query), _lib.ptr(a.key), _lib.ptr(a.value), _lib.ptr(a.bounds), _lib.ptr(a.key_bounds),
+            _lib.ptr(a.prefix), _lib.ptr(a.slopes), _lib.ptr(a.output), ctypes.c_int(w.heads), ctypes.c_int(w.kv_heads),
+            ctypes.c_int(w.total_heads), ctypes.c_int(int(a.causal)), ctypes.c_float(a.scale), ctypes.c_float(a.cap),
+            ctypes.c_int(c.unit_rows), ctypes.c_int(c.kv_splits), _lib.ptr(a.workspace), ctypes.c_size_t(need),
+            ctypes.c_void_p(stream),
+        )  # fmt: skip

@@ -31,6 +31,17 @@ from collections.abc import Iterable
 
 from nano_omni_b200 import _lib
 from nano_omni_b200.core import DType, Kernel, ScratchLayout, TensorDesc, TensorKind
+from nano_omni_b200.kernels.cache import (
+    BLOCK,
+    CacheAppendArguments,
+    CacheAppendKernel,
+    CacheAttentionArguments,
+    CacheAttentionConfig,
+    CacheAttentionKernel,
+    CacheReadArguments,
+    CacheReadKernel,
+    plan_cache_shares,
+)
 from nano_omni_b200.kernels.dense_bf16 import (
     DenseBf16AttentionArguments,
     DenseBf16AttentionConfig,
@@ -46,6 +57,13 @@ from nano_omni_b200.kernels.dense_int8_fp8 import (
     DenseInt8Fp8AttentionKernel,
 )
 from nano_omni_b200.kernels.dense_nvfp4 import DenseNvfp4Arguments, DenseNvfp4Config, DenseNvfp4Kernel
+from nano_omni_b200.kernels.masked import (
+    DEFAULT_SCALE,
+    MaskedBf16AttentionArguments,
+    MaskedBf16AttentionConfig,
+    MaskedBf16AttentionKernel,
+    share_workspace_bytes,
+)
 from nano_omni_b200.kernels.matmul import (
     MAX_ADAPTERS,
     ConvRotInt8Arguments,
@@ -798,6 +816,184 @@ class SolNvfp4Attention(_SolSliceAttention):
             SolNvfp4FinalizeKernel,
             SolNvfp4FinalizeArguments(q3, pooled, selected, attended, state, attended, self.head_offset),
         )
+        return sequence.calls
+
+
+class MaskedBf16Attention(Op):
+    """Attention over packed documents: ``bounds`` I32 ``[documents + 1]`` on the device says where each begins and the last
+    one ends in the rows of Q (and of K and V, unless ``key_bounds`` does).  ``key`` and ``value`` may have fewer heads, which
+    consecutive query heads share, and other rows than ``query``.
+
+    A query stands as far from its document's last key as from its last query.  ``causal`` hides later keys, except the first
+    ``prefix[d]`` (I32 ``[documents]``); ``cap`` > 0 bounds the scores by ``cap * tanh(score / cap)``; ``slopes`` (f32
+    ``[heads]``) take ``slopes[h] * distance`` off them.  A row that sees nothing becomes zeros, rows outside the documents
+    stay as they are.  No counterpart in the reference, whose attention takes one whole sequence.
+    """
+
+    def __init__(self, query: TensorDesc, key: TensorDesc, value: TensorDesc, bounds: TensorDesc, *, total_heads: int,
+                 head_offset: int = 0, key_bounds: TensorDesc | None = None, causal: bool = False,
+                 prefix: TensorDesc | None = None, cap: float = 0.0, slopes: TensorDesc | None = None,
+                 scale: float | None = None, rotation: Rotation | None = None):  # fmt: skip
+        self.rows, self.heads = _rows_and_heads(query)
+        self.key_rows, self.kv_heads = _rows_and_heads(key)
+        assert value.dtype == DType.BF16 and value.shape == key.shape
+        assert key_bounds is not None or self.key_rows >= self.rows, "fewer rows of K than of Q need key_bounds"
+        assert rotation is None or self.key_rows == self.rows, "a Rotation has one row of planes per token"
+        assert 0 <= head_offset <= total_heads - self.heads
+        self.total_heads, self.head_offset = total_heads, head_offset
+        self.documents = bounds.shape[0] - 1
+        self.causal, self.cap, self.scale = causal, cap, DEFAULT_SCALE if scale is None else scale
+        self.key_bounds, self.prefix, self.slopes, self.rotation = key_bounds, prefix, slopes, rotation
+        super().__init__(query, key, value, bounds, outputs=((DType.BF16, (self.rows, total_heads, 128)),))
+
+    def kernels(self, scratch: ScratchLayout) -> list[Kernel]:
+        sequence = KernelSequence(scratch)
+        query, key, value, bounds = self.inputs
+        if self.rotation is not None:
+            query = _rotated(sequence, "query", query, self.rotation.query_norm, self.rotation)
+            key = _rotated(sequence, "key", key, self.rotation.key_norm, self.rotation)
+        _masked(sequence, self, query, key, value, bounds, self.key_bounds or bounds)
+        return sequence.calls
+
+
+def _rows_and_heads(tensor: TensorDesc) -> tuple[int, int]:
+    rows, width = tensor.shape
+    assert tensor.dtype == DType.BF16 and width > 0 and width % 128 == 0
+    return rows, width // 128
+
+
+def _masked(sequence: KernelSequence, op, query, key, value, bounds, key_bounds) -> None:
+    """Emit the masked attention of ``op`` (its masks, scale and output slice) over rows ``key`` and ``value``."""
+    (rows, heads), (key_rows, kv_heads) = _rows_and_heads(query), _rows_and_heads(key)
+    config = MaskedBf16AttentionConfig()
+    need = share_workspace_bytes(rows, heads, config.kv_splits)
+    workspace = sequence.temporary("shares", DType.U8, (need,)) if need else None
+    sequence.emit(
+        MaskedBf16AttentionKernel,
+        MaskedBf16AttentionArguments(
+            query.view((rows, heads, 128)), key.view((key_rows, kv_heads, 128)), value.view((key_rows, kv_heads, 128)),
+            bounds, key_bounds, op.prefix, op.slopes, op.bound_outputs[0], op.head_offset, op.causal, op.scale, op.cap,
+            workspace,
+        ),
+        config,
+    )  # fmt: skip
+
+
+@dataclasses.dataclass(frozen=True, slots=True)
+class BlockCache:
+    """Keys and values in 8 bits: codes I8 ``[blocks, kv_heads, 64, 128]`` and scales F32 ``[blocks, kv_heads]`` of K and V;
+    ``table`` I32 ``[sequences, max_blocks]`` names the block of tokens ``64 b .. 64 b + 63`` of a sequence, ``lengths`` I32
+    ``[sequences]`` how many tokens it holds.  Table and lengths are read when an operator runs: a program changes them in
+    place between runs.  Entries of the table past a sequence's length are not read; one that is and names no block counts as
+    a block without keys and sets bit 6 of the status word."""
+
+    key: TensorDesc
+    value: TensorDesc
+    key_scales: TensorDesc
+    value_scales: TensorDesc
+    table: TensorDesc
+    lengths: TensorDesc
+
+    @property
+    def kv_heads(self) -> int:
+        return self.key.shape[1]
+
+    @property
+    def sequences(self) -> int:
+        return self.table.shape[0]
+
+    @property
+    def capacity(self) -> int:
+        """Tokens that the table has room for."""
+        return self.table.shape[0] * self.table.shape[1] * BLOCK
+
+
+class CacheAppend(Op):
+    """New rows of K and V (``bounds`` I32 ``[sequences + 1]``: which are whose) quantised behind what a cache's sequences hold;
+    ``lengths`` counts them already.  Outputs are the cache's own tensors, changed in place, in the order of ``PrepareKeyValue``:
+    codes and scales of K, codes and scales of V."""
+
+    def __init__(self, key: TensorDesc, value: TensorDesc, bounds: TensorDesc, cache: BlockCache) -> None:
+        self.rows, heads = _rows_and_heads(key)
+        assert value.dtype == DType.BF16 and value.shape == key.shape and heads == cache.kv_heads
+        self.cache = cache
+        outputs = (cache.key, cache.key_scales, cache.value, cache.value_scales)
+        super().__init__(key, value, bounds, outputs=tuple((t.dtype, t.shape) for t in outputs))
+
+    def kernels(self, scratch: ScratchLayout) -> list[Kernel]:
+        key, value, bounds = self.inputs
+        shape = (self.rows, self.cache.kv_heads, 128)
+        sequence = KernelSequence(scratch)
+        sequence.emit(
+            CacheAppendKernel,
+            CacheAppendArguments(
+                key.view(shape), value.view(shape), bounds, self.cache.table, self.cache.lengths, *self.bound_outputs
+            ),
+        )
+        return sequence.calls
+
+
+def _read(sequence: KernelSequence, cache: BlockCache, key: TensorDesc, value: TensorDesc, bounds: TensorDesc) -> None:
+    shape = (key.shape[0], cache.kv_heads, 128)
+    sequence.emit(
+        CacheReadKernel,
+        CacheReadArguments(
+            cache.key, cache.value, cache.key_scales, cache.value_scales, cache.table, cache.lengths,
+            key.view(shape), value.view(shape), bounds,
+        ),
+    )  # fmt: skip
+
+
+class CacheRead(Op):
+    """A cache's sequences as bf16 rows ``[capacity, kv_heads * 128]`` of K and of V, one sequence behind the other, and I32
+    ``[sequences + 1]`` where each begins: the operands of ``MaskedBf16Attention``.  Rows behind the last are left as they are."""
+
+    def __init__(self, cache: BlockCache, capacity: int) -> None:
+        self.cache = cache
+        rows = (DType.BF16, (capacity, cache.kv_heads * 128))
+        super().__init__(cache.key, cache.value, outputs=(rows, rows, (DType.I32, (cache.sequences + 1,))))
+
+    def kernels(self, scratch: ScratchLayout) -> list[Kernel]:
+        sequence = KernelSequence(scratch)
+        _read(sequence, self.cache, *self.bound_outputs)
+        return sequence.calls
+
+
+class CacheAttention(Op):
+    """Queries ``[rows, heads * 128]``, ``bounds`` I32 ``[sequences + 1]``, over the tokens that a cache holds of their sequences;
+    masks, cap and slopes as in ``MaskedBf16Attention`` (causal unless told otherwise: the last query stands at the last
+    cached token).  ``cached_tokens``: how many tokens the sequences hold together at most, for planning the division of
+    long sequences over the SMs (the table's capacity when not given)."""
+
+    def __init__(self, query: TensorDesc, bounds: TensorDesc, cache: BlockCache, *, total_heads: int, head_offset: int = 0,
+                 causal: bool = True, prefix: TensorDesc | None = None, cap: float = 0.0, slopes: TensorDesc | None = None,
+                 scale: float | None = None, cached_tokens: int | None = None):  # fmt: skip
+        self.rows, self.heads = _rows_and_heads(query)
+        assert 0 <= head_offset <= total_heads - self.heads
+        assert self.heads % cache.kv_heads == 0
+        self.total_heads, self.head_offset = total_heads, head_offset
+        self.cache = cache
+        self.cached_tokens = cache.capacity if cached_tokens is None else min(cached_tokens, cache.capacity)
+        assert self.cached_tokens > 0
+        self.causal, self.cap, self.scale = causal, cap, DEFAULT_SCALE if scale is None else scale
+        self.prefix, self.slopes = prefix, slopes
+        super().__init__(query, bounds, outputs=((DType.BF16, (self.rows, total_heads, 128)),))
+
+    def kernels(self, scratch: ScratchLayout) -> list[Kernel]:
+        query, bounds = self.inputs
+        cache = self.cache
+        sequence = KernelSequence(scratch)
+        splits = plan_cache_shares(self.rows, cache.sequences, self.cached_tokens, self.heads, cache.kv_heads)
+        need = share_workspace_bytes(self.rows, self.heads, splits)
+        sequence.emit(
+            CacheAttentionKernel,
+            CacheAttentionArguments(
+                query.view((self.rows, self.heads, 128)), cache.key, cache.value, cache.key_scales, cache.value_scales,
+                cache.table, cache.lengths, bounds, self.prefix, self.slopes, self.bound_outputs[0], self.head_offset,
+                self.causal, self.scale, self.cap, sequence.temporary("shares", DType.U8, (need,)) if need else None,
+            ),
+            CacheAttentionConfig(kv_splits=splits),
+        )  # fmt: skip
         return sequence.calls
 
 

@@ -30,6 +30,8 @@ def _fill(desc: TensorDesc, generator: torch.Generator, scale: float) -> TensorD
         t = torch.rand(shape, generator=generator, device="cuda") * 0.1 + 0.01
     elif desc.dtype == DType.I8:
         t = torch.randint(-3, 4, shape, generator=generator, device="cuda", dtype=torch.int8)
+    elif desc.dtype == DType.I32:
+        t = torch.zeros(shape, dtype=torch.int32, device="cuda")  # indices: see ``address``
     elif desc.dtype == DType.FP8_UE4M3:
         t = (torch.rand(shape, generator=generator, device="cuda") + 0.125).to(torch.float8_e4m3fn)
     elif desc.dtype == DType.FP8_E4M3:
@@ -41,7 +43,11 @@ def _fill(desc: TensorDesc, generator: torch.Generator, scale: float) -> TensorD
 
 def address(arguments, seed: int = 0, scale: float = 1.0):
     generator = torch.Generator(device="cuda").manual_seed(seed)
-    return arguments.map(lambda d: _fill(d, generator, scale) if d.kind == TensorKind.EMPTY else d)
+    arguments = arguments.map(lambda d: _fill(d, generator, scale) if d.kind == TensorKind.EMPTY else d)
+    # kernels that follow indices in device memory say what makes sense there
+    for name, values in getattr(arguments, "index_values", dict)().items():
+        getattr(arguments, name).tensor.copy_(torch.tensor(values, dtype=torch.int32))
+    return arguments
 
 
 def measure(kernel, repeat: int, warmup: int) -> list[float]:

@@ -1,0 +1,203 @@
+"""Planning and refusals of the masked attention and the 8-bit cache (no GPU)."""
+
+import ctypes
+
+import pytest
+
+from nano_omni_b200 import kernels, ops
+from nano_omni_b200.core import DType, TensorDesc
+
+
+def at(dtype, *shape):
+    at.next += 1 << 30
+    return TensorDesc.from_pointer(at.next, dtype, shape)
+
+
+at.next = 1 << 40
+
+
+def cache(blocks=20, kv_heads=2, sequences=3, max_blocks=8):
+    codes, scales = (blocks, kv_heads, 64, 128), (blocks, kv_heads)
+    return ops.BlockCache(
+        at(DType.I8, *codes), at(DType.I8, *codes), at(DType.F32, *scales), at(DType.F32, *scales),
+        at(DType.I32, sequences, max_blocks), at(DType.I32, sequences),
+    )  # fmt: skip
+
+
+def masked(heads=4, kv_heads=2, rows=300, key_rows=300, documents=3, total_heads=6, **options):
+    return ops.MaskedBf16Attention(
+        at(DType.BF16, rows, heads * 128), at(DType.BF16, key_rows, kv_heads * 128), at(DType.BF16, key_rows, kv_heads * 128),
+        at(DType.I32, documents + 1), total_heads=total_heads, **options,
+    )  # fmt: skip
+
+
+def test_masked_attention_plans_one_launch_of_its_kernel():
+    op = masked(causal=True, prefix=at(DType.I32, 3), slopes=at(DType.F32, 4), cap=20.0, head_offset=2)
+    op.to(at(DType.BF16, 300, 6, 128))
+    call = op.prepare()[0][0]
+    assert call.name == "masked_bf16_attention_d128"
+    w = call.workload
+    assert (w.heads, w.kv_heads, w.documents, w.causal, w.use_prefix, w.use_slopes, w.cap) == (4, 2, 3, True, True, True, 20.0)
+    assert call.arguments.key_bounds is call.arguments.bounds
+
+
+def test_rotation_comes_in_front():
+    rotation = ops.Rotation(at(DType.BF16, 128), at(DType.BF16, 128), at(DType.F32, 300, 48), at(DType.F32, 300, 48))
+    op = masked(rotation=rotation).to(at(DType.BF16, 300, 6, 128))
+    assert [c.name for c in op.prepare()[0]] == ["h3_head_norm_rope", "h3_head_norm_rope", "masked_bf16_attention_d128"]
+
+
+@pytest.mark.parametrize(
+    "options",
+    [
+        {"kv_heads": 3},  # does not divide the heads
+        {"head_offset": 3},
+        {"key_rows": 200},  # fewer keys than queries need bounds of their own
+        {"prefix": (DType.I32, 3)},  # a prefix without a causal mask
+        {"causal": True, "prefix": (DType.I32, 2)},
+        {"causal": True, "prefix": (DType.F32, 3)},
+        {"slopes": (DType.F32, 2)},
+        {"slopes": (DType.BF16, 4)},
+        {"key_bounds": (DType.I32, 5)},
+    ],
+    ids=str,
+)
+def test_masked_attention_refuses(options):
+    options = {n: at(x[0], *x[1:]) if isinstance(x, tuple) else x for n, x in options.items()}
+    with pytest.raises(AssertionError):
+        masked(**options).to(at(DType.BF16, 300, 6, 128)).prepare()
+
+
+@pytest.mark.parametrize("options", [{"cap": -1.0}, {"cap": float("inf")}, {"scale": 0.0}, {"scale": float("nan")}], ids=str)
+def test_masked_attention_refuses_numbers(options):
+    with pytest.raises(ValueError):
+        masked(**options).to(at(DType.BF16, 300, 6, 128)).prepare()
+    op = ops.CacheAttention(at(DType.BF16, 3, 512), at(DType.I32, 4), cache(), total_heads=4, **options)
+    with pytest.raises(ValueError):
+        op.to(at(DType.BF16, 3, 4, 128)).prepare()
+
+
+def test_cache_operators_plan_their_kernels():
+    c = cache()
+    append = ops.CacheAppend(at(DType.BF16, 9, 256), at(DType.BF16, 9, 256), at(DType.I32, 4), c)
+    append.to(c.key, c.key_scales, c.value, c.value_scales)
+    assert [k.name for k in append.prepare()[0]] == ["int8_cache_append_d128"]
+    read = ops.CacheRead(c, 900).to(at(DType.BF16, 900, 256), at(DType.BF16, 900, 256), at(DType.I32, 4))
+    assert [k.name for k in read.prepare()[0]] == ["int8_cache_read_d128"]
+    attend = ops.CacheAttention(at(DType.BF16, 3, 512), at(DType.I32, 4), c, total_heads=4).to(at(DType.BF16, 3, 4, 128))
+    assert [k.name for k in attend.prepare()[0]] == ["int8_cache_attention_d128"]
+    assert c.capacity == 3 * 8 * 64
+
+
+def test_cache_operators_refuse():
+    c = cache()
+    rows = at(DType.BF16, 9, 256)
+    with pytest.raises(AssertionError):  # heads of the rows and of the cache
+        ops.CacheAppend(at(DType.BF16, 9, 512), at(DType.BF16, 9, 512), at(DType.I32, 4), c)
+    with pytest.raises(AssertionError):  # bounds of another number of sequences
+        op = ops.CacheAppend(rows, rows, at(DType.I32, 5), c).to(c.key, c.key_scales, c.value, c.value_scales)
+        op.prepare()
+    with pytest.raises(AssertionError):  # outputs in another order
+        ops.CacheAppend(rows, rows, at(DType.I32, 4), c).to(c.key, c.value, c.key_scales, c.value_scales)
+    with pytest.raises(AssertionError):
+        ops.CacheRead(c, 900).to(at(DType.BF16, 800, 256), at(DType.BF16, 900, 256), at(DType.I32, 4))
+    with pytest.raises(AssertionError):  # heads that cannot share two key heads
+        ops.CacheAttention(at(DType.BF16, 3, 384), at(DType.I32, 4), c, total_heads=3)
+    with pytest.raises(AssertionError):  # a prefix without a causal mask
+        op = ops.CacheAttention(at(DType.BF16, 3, 512), at(DType.I32, 4), c, total_heads=4, causal=False, prefix=at(DType.I32, 3))
+        op.to(at(DType.BF16, 3, 4, 128)).prepare()
+    for field, wrong in (("key_scales", (DType.F32, 20, 3)), ("table", (DType.F32, 3, 8)), ("lengths", (DType.I32, 2)),
+                         ("value", (DType.I8, 20, 2, 32, 128))):  # fmt: skip
+        fields = {n: getattr(c, n) for n in ("key", "value", "key_scales", "value_scales", "table", "lengths")}
+        broken = ops.BlockCache(**fields | {field: at(wrong[0], *wrong[1:])})
+        with pytest.raises(AssertionError):
+            op = ops.CacheAttention(at(DType.BF16, 3, 512), at(DType.I32, 4), broken, total_heads=4)
+            op.to(at(DType.BF16, 3, 4, 128)).prepare()
+
+
+def test_workloads_survive_the_round_trip():
+    from nano_omni_b200.kernels.cache import CacheAppendWorkload, CacheAttentionWorkload, CacheReadWorkload
+    from nano_omni_b200.kernels.masked import MaskedBf16AttentionWorkload
+
+    common = {"sequences": 3, "max_blocks": 5, "num_blocks": 11, "kv_heads": 2}
+    for workload, name in (
+        (MaskedBf16AttentionWorkload(num_rows=9, num_key_rows=70, documents=4, heads=6, kv_heads=2, total_heads=7, causal=True,
+                                     use_prefix=True, use_slopes=True, cap=3.0), "masked_bf16_attention_d128"),
+        (CacheAppendWorkload(num_rows=9, **common), "int8_cache_append_d128"),
+        (CacheReadWorkload(capacity=90, **common), "int8_cache_read_d128"),
+        (CacheAttentionWorkload(num_rows=9, heads=4, total_heads=4, use_slopes=True, **common), "int8_cache_attention_d128"),
+    ):  # fmt: skip
+        cls = kernels.classes()[name]
+        arguments = cls.make_arguments(workload)
+        assert cls.make_workload(arguments) == workload
+        for field, values in arguments.index_values().items():
+            shape = getattr(arguments, field).shape
+            assert len(values) == shape[0] and (len(shape) == 1 or len(values[0]) == shape[1])
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from nano_omni_b200 import _lib, build
+
+    build.build()
+    lib = _lib.library()
+    lib.nob200_last_error.restype = ctypes.c_char_p
+    return lib
+
+
+def test_c_entries_refuse_before_any_launch(lib):
+    p, null, z = ctypes.c_void_p(1 << 20), ctypes.c_void_p(0), ctypes.c_size_t(0)
+    f = ctypes.c_float
+
+    def refused(function, arguments, text):
+        function.restype = ctypes.c_int
+        assert function(*arguments) == -1 and text in lib.nob200_last_error(), lib.nob200_last_error()
+
+    def attention(rows=9, heads=4, kv_heads=2, offset=0, query=p, output=p, scale=0.1, cap=0.0, unit=256, splits=1, workspace=null,
+                  size=z):  # fmt: skip
+        return (rows, 70, 3, offset, query, p, p, p, p, null, null, output, heads, kv_heads, 4, 1, f(scale), f(cap), unit, splits,
+                workspace, size, null)  # fmt: skip
+
+    fn = lib.nob200_masked_bf16_attention_d128
+    refused(fn, attention(rows=0), b"positive")
+    refused(fn, attention(kv_heads=3), b"cannot share 3 key heads")
+    refused(fn, attention(offset=1), b"head_offset")
+    refused(fn, attention(query=null), b"NULL")
+    refused(fn, attention(output=ctypes.c_void_p(8)), b"16-byte aligned")
+    refused(fn, attention(scale=float("nan")), b"scale")
+    refused(fn, attention(cap=-1.0), b"cap")
+    refused(fn, attention(unit=192), b"unit_rows")
+    refused(fn, attention(splits=65), b"kv_splits")
+    refused(fn, attention(splits=2), b"workspace required")
+    refused(fn, attention(rows=0x7FFFFFFF, heads=4, splits=64, workspace=p, size=ctypes.c_size_t(1 << 62)), b"grid limit")
+
+    fn = lib.nob200_int8_cache_append_d128
+    refused(fn, (0, 3, 5, 11, p, p, p, p, p, p, p, p, p, 2, null), b"positive")
+    refused(fn, (9, 3, 5, 11, p, p, p, p, null, p, p, p, p, 2, null), b"NULL")
+    refused(fn, (9, 3, 1 << 26, 11, p, p, p, p, p, p, p, p, p, 2, null), b"exceed the limit")
+    refused(fn, (9, 3, 5, 11, ctypes.c_void_p(8), p, p, p, p, p, p, p, p, 2, null), b"aligned")
+    fn = lib.nob200_int8_cache_read_d128
+    refused(fn, (0, 3, 5, 11, p, p, p, p, p, p, p, p, p, 2, null), b"positive")
+    refused(fn, (90, 3, 5, 11, p, p, p, p, p, p, p, p, null, 2, null), b"NULL")
+
+    def cached(rows=3, blocks=11, kv_heads=2, splits=1, lengths=p, cap=0.0):
+        return (rows, 3, 5, blocks, 0, p, p, p, p, p, p, lengths, p, null, null, p, 4, kv_heads, 4, 1, f(0.1), f(cap), splits, null, z,
+                null)  # fmt: skip
+
+    fn = lib.nob200_int8_cache_attention_d128
+    refused(fn, cached(rows=0), b"positive")
+    refused(fn, cached(kv_heads=3), b"cannot share")
+    refused(fn, cached(lengths=null), b"NULL")
+    refused(fn, cached(cap=float("inf")), b"cap")
+    refused(fn, cached(blocks=1 << 28), b"exceed the limit")
+    refused(fn, cached(splits=2), b"workspace required")
+
+
+def test_workspace_sizes_are_the_planned_ones(lib):
+    from nano_omni_b200.kernels.masked import share_workspace_bytes
+
+    for name in ("masked_bf16", "int8_cache"):
+        fn = getattr(lib, f"nob200_{name}_attention_d128_workspace_bytes")
+        fn.restype = ctypes.c_size_t
+        for rows, heads, splits in ((1, 1, 1), (1, 14, 21), (32768, 28, 8), (4096, 56, 64)):
+            assert fn(rows, heads, splits) == share_workspace_bytes(rows, heads, splits)
