@@ -61,6 +61,8 @@ struct __align__(1024) Shared {
   uint64_t v_clean[2];  // the V tile in stage 1 / 3 has been looked through
   uint32_t bad[2][4];   // and these of its rows were not finite
   Unit unit;
+  int units[kThreads / 32];
+  __align__(16) uint8_t staging[8][32 * 64];  // of the softmax warps: 64 bytes of each of their rows
   uint32_t tmem_base;
   uint32_t abort;
   uint32_t qk_issued;
@@ -100,28 +102,54 @@ __device__ __forceinline__ float rcp(float x) {
 // any x: 1 - 2 / (1 + 2^(2 log2(e) x)); absolute error some 2^-22
 __device__ __forceinline__ float tanh_any(float x) { return fmaf(-2.f, rcp(1.f + ex2(x * 2.885390081777927f)), 1.f); }
 
-// The unit of this CTA, by one converged warp.
-__device__ __forceinline__ Unit unit_of(const MaskedParams& P, int slot, int piece) {
-  Unit u = {};
-  const int2 found = find_unit(P.documents, slot, [&](int d) {
-    const int2 r = document_rows(P.bounds, d, P.rows);
-    return (r.y - r.x + P.unit_rows - 1) / P.unit_rows;
-  });
-  if (found.x < 0) return u;
-  const int2 rows = document_rows(P.bounds, found.x, P.rows), keys = document_rows(P.key_bounds, found.x, P.key_rows);
-  u.query0 = found.y * P.unit_rows;
-  u.row0 = rows.x + u.query0;
-  u.rows = rows.y - u.row0;
-  u.key0 = keys.x;
-  u.sight.keys = keys.y - keys.x;
-  u.sight.ahead = u.sight.keys - (rows.y - rows.x);
-  u.sight.prefix = P.prefix ? P.prefix[found.x] : 0;
-  u.sight.causal = P.causal != 0;
-  const int seen = u.sight.visible(u.query0 + min(u.rows, P.unit_rows) - 1);
-  const int tiles = (seen + kTile - 1) / kTile;
-  u.kv_begin = static_cast<int>(static_cast<long long>(tiles) * piece / P.splits);
-  u.kv_end = static_cast<int>(static_cast<long long>(tiles) * (piece + 1) / P.splits);
-  return u;
+// The unit of this CTA, by all its threads: a document each, from the last one backwards, so that everything about 384
+// documents is one load's latency away.  Units are numbered from the last document's last one on.
+__device__ __forceinline__ void find_own_unit(const MaskedParams& P, Shared& S, int slot, int piece) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int last = P.documents - 1; last >= 0; last -= kThreads) {
+    const int d = last - static_cast<int>(threadIdx.x);
+    int2 rows = {}, keys = {};
+    int prefix = 0, units = 0;
+    if (d >= 0) {
+      keys = document_rows(P.key_bounds, d, P.key_rows);
+      prefix = P.prefix ? P.prefix[d] : 0;
+      rows = document_rows(P.bounds, d, P.rows);
+      units = (rows.y - rows.x + P.unit_rows - 1) / P.unit_rows;
+    }
+    int through = units;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int other = __shfl_up_sync(0xffffffffu, through, o);
+      if (lane >= o) through += other;
+    }
+    if (lane == 31) S.units[warp] = through;
+    __syncthreads();
+    int total = 0;
+#pragma unroll
+    for (int w = 0; w < kThreads / 32; ++w) {
+      if (w == warp) through += total;
+      total += S.units[w];
+    }
+    if (slot < through && slot >= through - units) {
+      Unit u;
+      u.query0 = (through - 1 - slot) * P.unit_rows;
+      u.row0 = rows.x + u.query0;
+      u.rows = rows.y - u.row0;
+      u.key0 = keys.x;
+      u.sight.keys = keys.y - keys.x;
+      u.sight.ahead = u.sight.keys - (rows.y - rows.x);
+      u.sight.prefix = prefix;
+      u.sight.causal = P.causal != 0;
+      const int seen = u.sight.visible(u.query0 + min(u.rows, P.unit_rows) - 1);
+      const int tiles = (seen + kTile - 1) / kTile;
+      u.kv_begin = static_cast<int>(static_cast<long long>(tiles) * piece / P.splits);
+      u.kv_end = static_cast<int>(static_cast<long long>(tiles) * (piece + 1) / P.splits);
+      S.unit = u;
+    }
+    __syncthreads();
+    if (slot < total) return;
+    slot -= total;
+  }
 }
 
 template <bool CAP, bool BIAS>
@@ -150,6 +178,7 @@ fa_fwd_masked_bf16_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
       mbar_init(&S.pv_done[t], 1);
       mbar_init(&S.v_clean[t], 1);
     }
+    S.unit = Unit{};
     S.abort = 0;
     S.qk_issued = 0;
     mbar_fence_init();
@@ -158,16 +187,15 @@ fa_fwd_masked_bf16_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
     tmem_alloc(&S.tmem_base, kTmemCols);
     tmem_relinquish();
   }
-  pdl_wait();  // launched as a programmatic dependent: the set-up above overlaps the kernel before
-  const int head = static_cast<int>(blockIdx.x / (P.slots * P.splits));
-  const int piece = static_cast<int>(blockIdx.x % P.splits);
-  if (warp == 0) {
-    const Unit found = unit_of(P, static_cast<int>(blockIdx.x / P.splits) % P.slots, piece);
-    if (lane == 0) S.unit = found;
-  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  pdl_wait();  // launched as a programmatic dependent: the set-up above overlaps the kernel before
+  // All heads of a unit are neighbours in the grid, and the units with the longest key ranges come first: the short ones are
+  // left for its end (8192 causal rows x 14 heads 341 us head by head, so 270).
+  const int piece = static_cast<int>(blockIdx.x % P.splits), place = static_cast<int>(blockIdx.x / P.splits);
+  const int head = place % P.heads;
+  find_own_unit(P, S, place / P.heads, piece);
   const uint32_t tmem = S.tmem_base;
   pdl_release();
 
@@ -365,14 +393,12 @@ fa_fwd_masked_bf16_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
       const uint32_t o_addr = tmem + lane_base + kColO + t * kTile;
       const int query = S.unit.query0 + t * kTile + (warp & 3) * 32 + lane;
       const int visible = S.unit.sight.visible(query) - kv_begin * kTile;  // keys of this CTA's that the row sees
-      const int whole = S.unit.sight.visible(S.unit.query0 + t * kTile) / kTile - kv_begin;
       // a capped score stays in units of the cap until the exponential, a biased one is turned into log2 units at once
       const float sc = BIAS ? (CAP ? P.to_log2 : P.scale * P.to_log2) : 1.f;
       const float unit_log2 = BIAS ? 1.f : CAP ? P.to_log2 : P.scale * P.to_log2;
       const float slope = BIAS ? P.slopes[head] * 1.4426950408889634f : 0.f;
       const int position = BIAS ? S.unit.sight.ahead + query - kv_begin * kTile : 0;  // relative to this CTA's first key
       float m_used = 0.f;
-      bool spoilt = false;            // the row sees a value that is not finite
       uint64_t la = 0ull, lb = 0ull;  // four partial row sums as two fp32 pairs
       bool ok = true;
       for (int j = 0; j < n_kv; ++j) {
@@ -427,7 +453,7 @@ fa_fwd_masked_bf16_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
             }
           }
         }
-        if (j >= whole) {
+        if (j >= partly && __any_sync(0xffffffffu, visible < (j + 1) * kTile)) {
           const int valid = visible - j * kTile;
 #pragma unroll
           for (int i = 0; i < 128; ++i)
@@ -467,12 +493,13 @@ fa_fwd_masked_bf16_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
           ok = poll(&S.v_clean[j & 1], (j >> 1) & 1, kWaitTimeoutLoad);
           if (!ok) break;
           const int valid = visible - j * kTile;
+          uint32_t bad = 0;
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            const uint32_t bad = *const_cast<const volatile uint32_t*>(&S.bad[j & 1][k]);
             const int seen = clamped(valid - 32 * k, 0, 32);
-            spoilt |= (bad & (seen == 32 ? ~0u : (1u << seen) - 1u)) != 0;
+            bad |= *const_cast<const volatile uint32_t*>(&S.bad[j & 1][k]) & (seen == 32 ? ~0u : (1u << seen) - 1u);
           }
+          if (bad) la = ~0ull;  // the row sees one: its sum, and with it the row, is not a number
         }
         const uint64_t scale2 = pack2(unit_log2, unit_log2);
         const uint64_t neg_m2 = pack2(-m_used, -m_used);
@@ -513,14 +540,33 @@ fa_fwd_masked_bf16_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
         unpack2(la, l0, l1);
         unpack2(lb, l2, l3);
         const float l = (l0 + l1) + (l2 + l3);
-        const float inv = spoilt ? __uint_as_float(0x7fffffffu) : l == 0.f ? 0.f : 1.0f / l;
-        const int in_unit = t * kTile + (warp & 3) * 32 + lane;
-        const int row = S.unit.row0 + in_unit;
-        bool store = in_unit < S.unit.rows;
-        const size_t rows = static_cast<size_t>(P.rows);
-        const size_t at = (static_cast<size_t>(piece) * P.heads + head) * rows + row;  // of a partial row
-        store = store && NOB_CHECK(row >= 0 && row < P.rows && head + P.head_offset < P.total_heads, status);
-        if (P.splits > 1 && store) P.lse[at] = spoilt ? __uint_as_float(0x7fffffffu) : m_used + log2f(l);
+        const float inv = l == 0.f ? 0.f : 1.0f / l;
+        const int in_unit = t * kTile + (warp & 3) * 32 + lane, row = S.unit.row0 + in_unit;
+        const bool live = NOB_CHECK(in_unit >= S.unit.rows || (row >= 0 && row < P.rows && head + P.head_offset < P.total_heads), status) &&
+                          in_unit < S.unit.rows;
+        const size_t share = static_cast<size_t>(piece) * P.heads + head;  // of divided keys
+        if (P.splits > 1 && live) P.lse[share * P.rows + row] = m_used + log2f(l);
+        // Rows leave through shared memory, 64 bytes of each at a time, so that four lanes write one row's piece: a lane per row
+        // touches 32 lines with every store (packed documents 140 us, so 128).
+        uint8_t* mine = S.staging[warp];
+        const uint32_t rows_live = __ballot_sync(0xffffffffu, live);
+        uint4 part[4];
+        auto flush = [&](int byte) {  // `part`, the bytes from `byte` on of every lane's row
+          __syncwarp();
+#pragma unroll
+          for (int g = 0; g < 4; ++g) *reinterpret_cast<uint4*>(mine + lane * 64 + ((g ^ ((lane >> 1) & 3)) << 4)) = part[g];
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int r = 8 * i + (lane >> 2);
+            if (!(rows_live >> r & 1)) continue;
+            const uint4 x = *reinterpret_cast<const uint4*>(mine + r * 64 + (((lane & 3) ^ ((r >> 1) & 3)) << 4));
+            const size_t to = row - lane + r;
+            char* dst = P.splits > 1 ? reinterpret_cast<char*>(P.partial) + (share * P.rows + to) * 512
+                                     : reinterpret_cast<char*>(P.output) + (to * P.total_heads + head + P.head_offset) * 256;
+            *reinterpret_cast<uint4*>(dst + byte + 16 * (lane & 3)) = x;
+          }
+        };
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           uint32_t o[32];
@@ -531,22 +577,26 @@ fa_fwd_masked_bf16_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
 #pragma unroll
             for (int i = 0; i < 32; ++i) o[i] = 0;
           }
-          if (store) {
-            float r[32];
+          auto value = [&](int i) { return __uint_as_float(o[i]) * inv; };
+          if (P.splits > 1) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) r[i] = __uint_as_float(o[i]) * inv;
-            if (P.splits > 1) {
-              float4* dst = reinterpret_cast<float4*>(P.partial + at * 128 + 32 * c);
+            for (int k = 0; k < 2; ++k) {
 #pragma unroll
-              for (int i = 0; i < 8; ++i) dst[i] = make_float4(r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
-            } else {
-              __nv_bfloat16* dst = P.output + (static_cast<size_t>(row) * P.total_heads + head + P.head_offset) * 128 + 32 * c;
-#pragma unroll
-              for (int i = 0; i < 32; i += 8)
-                *reinterpret_cast<uint4*>(dst + i) =
-                    make_uint4(pack_bf16(r[i], r[i + 1]), pack_bf16(r[i + 2], r[i + 3]), pack_bf16(r[i + 4], r[i + 5]),
-                               pack_bf16(r[i + 6], r[i + 7]));
+              for (int g = 0; g < 4; ++g) {
+                const int i = 16 * k + 4 * g;
+                part[g] = make_uint4(__float_as_uint(value(i)), __float_as_uint(value(i + 1)), __float_as_uint(value(i + 2)),
+                                     __float_as_uint(value(i + 3)));
+              }
+              flush(128 * c + 64 * k);
             }
+          } else {
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              const int i = 8 * g;
+              part[g] = make_uint4(pack_bf16(value(i), value(i + 1)), pack_bf16(value(i + 2), value(i + 3)),
+                                   pack_bf16(value(i + 4), value(i + 5)), pack_bf16(value(i + 6), value(i + 7)));
+            }
+            flush(64 * c);
           }
         }
       }

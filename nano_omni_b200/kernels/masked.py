@@ -8,7 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import dataclasses
-from typing import Literal
+from typing import Literal, NamedTuple
 
 from pydantic import Field
 
@@ -62,6 +62,43 @@ class MaskedBf16AttentionArguments(Arguments):
         spread = lambda rows: [rows * d // documents for d in range(documents + 1)]  # noqa: E731
         values = {"bounds": spread(self.query.shape[0]), "key_bounds": spread(self.key.shape[0])}
         return values | ({"prefix": [0] * documents} if self.prefix is not None else {})
+
+
+class MaskedUnits(NamedTuple):
+    """How a launch becomes units: query rows of a unit, CTAs over which its keys are divided."""
+
+    unit_rows: int
+    kv_splits: int
+
+
+def plan_masked_units(num_rows: int, num_key_rows: int, documents: int, heads: int, causal: bool, sm_count: int = 148) -> MaskedUnits:
+    """Units of a launch whose documents are taken to be of one length (the device alone knows their bounds).
+
+    Times are counted in key tiles of a 256-row unit (1.9 us); a 128-row unit takes 0.72 of one per key tile, a CTA 2 beside
+    its tiles, the join of shares 2.5 and 0.025 per 256-row share.  Units of one length run in whole rounds of the SMs, others
+    fill the last round to about a half.  One unit of 256 rows stays unless the estimate falls by 2 %: 1024 rows x 14 heads
+    18.9 us in 128-row units, 21.9 in 256; 1560 rows against 31560 keys x 14 heads 364 us in three shares, 510 whole; 8192 rows
+    x 14 heads 475 us whole, 505 in two shares."""
+    rows, keys = -(-num_rows // documents), -(-num_key_rows // documents)
+    seen = keys - min(rows, keys) / 2 if causal else keys
+    tiles = max(1.0, seen / 128)
+    alike = documents == 1 and not causal
+    best, plan = None, MaskedUnits(256, 1)
+    for unit_rows, step in ((256, 1.0), (128, 0.72)):
+        units = -(-rows // unit_rows) * documents * heads
+        for splits in range(1, 65):
+            if splits > 1 and tiles / splits < 2:
+                break
+            pieces = units * splits
+            rounds = -(-pieces // sm_count) if alike or pieces <= sm_count else pieces / sm_count + 0.5
+            cost = rounds * (tiles / splits * step + 2)
+            if splits > 1:
+                cost += 2.5 + 0.025 * pieces * unit_rows / 256
+            if best is None:
+                best = 0.98 * cost
+            elif cost < best:
+                best, plan = cost, MaskedUnits(unit_rows, splits)
+    return plan
 
 
 def share_workspace_bytes(num_rows: int, heads: int, kv_splits: int) -> int:

@@ -62,6 +62,8 @@ from nano_omni_b200.kernels.masked import (
     MaskedBf16AttentionArguments,
     MaskedBf16AttentionConfig,
     MaskedBf16AttentionKernel,
+    MaskedUnits,
+    plan_masked_units,
     share_workspace_bytes,
 )
 from nano_omni_b200.kernels.matmul import (
@@ -844,6 +846,7 @@ class MaskedBf16Attention(Op):
         self.documents = bounds.shape[0] - 1
         self.causal, self.cap, self.scale = causal, cap, DEFAULT_SCALE if scale is None else scale
         self.key_bounds, self.prefix, self.slopes, self.rotation = key_bounds, prefix, slopes, rotation
+        self.units = plan_masked_units(self.rows, self.key_rows, self.documents, self.heads, causal)
         super().__init__(query, key, value, bounds, outputs=((DType.BF16, (self.rows, total_heads, 128)),))
 
     def kernels(self, scratch: ScratchLayout) -> list[Kernel]:
@@ -852,7 +855,7 @@ class MaskedBf16Attention(Op):
         if self.rotation is not None:
             query = _rotated(sequence, "query", query, self.rotation.query_norm, self.rotation)
             key = _rotated(sequence, "key", key, self.rotation.key_norm, self.rotation)
-        _masked(sequence, self, query, key, value, bounds, self.key_bounds or bounds)
+        _masked(sequence, self, self.units, query, key, value, bounds, self.key_bounds or bounds)
         return sequence.calls
 
 
@@ -862,10 +865,10 @@ def _rows_and_heads(tensor: TensorDesc) -> tuple[int, int]:
     return rows, width // 128
 
 
-def _masked(sequence: KernelSequence, op, query, key, value, bounds, key_bounds) -> None:
+def _masked(sequence: KernelSequence, op, units: MaskedUnits, query, key, value, bounds, key_bounds) -> None:
     """Emit the masked attention of ``op`` (its masks, scale and output slice) over rows ``key`` and ``value``."""
     (rows, heads), (key_rows, kv_heads) = _rows_and_heads(query), _rows_and_heads(key)
-    config = MaskedBf16AttentionConfig()
+    config = MaskedBf16AttentionConfig(**units._asdict())
     need = share_workspace_bytes(rows, heads, config.kv_splits)
     workspace = sequence.temporary("shares", DType.U8, (need,)) if need else None
     sequence.emit(
