@@ -402,16 +402,18 @@ int nob200_int8_cache_read_d128(int capacity, int sequences, int max_blocks, int
  * Attention of the queries bounds[s] .. bounds[s + 1] over the cached tokens of sequence s, with positions, masks, cap and
  * slopes as nob200_masked_bf16_attention_d128 (a sequence is a document, lengths[s] its keys).  query bf16
  * [num_rows, heads, 128], key / value codes int8 [num_blocks, kv_heads, 64, 128], output bf16 [num_rows, total_heads, 128]
- * at head_offset.  For a few rows per sequence and key head: 16 of them are a CTA's.  kv_splits > 1 divides each
- * sequence's blocks over so many CTAs (workspace of ..._workspace_bytes()).
+ * at head_offset.  For a few rows per sequence and key head (new tokens x query heads of a key head): `columns`, 8 or 16, of
+ * them are a CTA's.  kv_splits > 1 divides each sequence's keys over so many CTAs, whose
+ * fp32 results a second kernel joins (workspace of ..._workspace_bytes()); without workspace up to eight are a cluster that
+ * joins them itself.
  */
 size_t nob200_int8_cache_attention_d128_workspace_bytes(int num_rows, int heads, int kv_splits);
 int nob200_int8_cache_attention_d128(int num_rows, int sequences, int max_blocks, int num_blocks, int head_offset,
                                      const void* query, const void* key, const void* value, const void* key_scales,
                                      const void* value_scales, const void* table, const void* lengths, const void* bounds,
                                      const void* prefix, const void* slopes, void* output, int heads, int kv_heads,
-                                     int total_heads, int causal, float scale, float cap, int kv_splits, void* workspace,
-                                     size_t workspace_bytes, void* stream);
+                                     int total_heads, int causal, float scale, float cap, int columns, int kv_splits,
+                                     void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * INT8 GEMM with the scaled fused epilogue of the projections around attention.

@@ -4,20 +4,22 @@
 // in fa_fwd_masked_bf16.cu.  No counterpart in the reference.
 //
 // One token reads every cached byte once and computes 2 x 128 multiply-adds per 256 bytes and head, so the call is bound by
-// HBM and the kernel by how many bytes it keeps in flight.  The query heads that share a key head, of all new tokens of a
-// sequence, are rows of one 16-row matrix instruction (mma.sync: a tcgen05 tile of 128 rows would stand empty, and its
-// operands would have to go through shared memory once more after they are widened).
+// HBM, and the kernel by the bytes it keeps in flight and the instructions it spends on a byte (an SM has some 700 cycles for
+// the 16 KiB of a block).  Keys are the 16 rows of the matrix instructions (mma.sync m16n8k16) and queries their 8 columns: the
+// query heads that share a key head, of all new tokens of a sequence, are 8 or 16 columns of a CTA.  (Queries as 16 rows took
+// twice the instructions for one token of up to eight heads, and 242 registers: 64 contexts x 32 heads 253 us.)
 //
-// A CTA owns 16 such rows of one sequence and key head and a contiguous share of its blocks; its four warps take blocks in turn,
-// each with a running maximum, sum and 16 x 128 accumulator of its own, joined at the end.  A warp feeds itself: its lane 0
-// issues TMA loads of K and V blocks (64 x 128 bytes, 128-byte swizzle) into a ring of three, two of which are in flight while
-// one is worked on; two CTAs per SM make 128 KiB in flight, well over the 45 KiB that latency x bandwidth asks for.
-//  * scores: A = the queries as f16, scaled by a power of two to a row maximum in [1, 2) (exact down to 2^-24 of it);
-//    B = codes, which f16 holds exactly: byte -> f16 by a permute onto 1024 + (code + 128) and a subtraction.  The channels
-//    of an instruction's k index are chosen so that a lane reads 32 consecutive bytes of a key.
-//  * values: V's bytes come through ldmatrix.trans, which delivers two channels of two keys per register; a permute
-//    separates the channels into two n tiles.  The probabilities are rounded to f16 (2^-11), their sum is taken before;
-//    the block's scale of V multiplies the block's product as it joins the accumulator.
+// A CTA's four warps take steps of 32 keys in turn from its share of the sequence, each with a running maximum, sum and
+// accumulator of its own, joined at the end.  A warp feeds itself: its lane 0 issues TMA loads of K and V (32 x 128 bytes,
+// 128-byte swizzle) into a ring of three, two of which are in flight while one is worked on; sixteen warps per SM make
+// 128 KiB in flight, well over the 45 KiB that latency x bandwidth asks for.
+//  * scores: A = codes, which f16 holds exactly (byte -> f16 by a permute onto 1024 + (code + 128) and a subtraction); B = the
+//    queries as f16, scaled by a power of two to a row maximum in [1, 2) (exact down to 2^-24 of it).  The channels of an
+//    instruction's k index are chosen so that a lane reads 32 consecutive bytes of a key.
+//  * values: A = V transposed by ldmatrix.trans, which delivers two channels of two keys per register; a permute puts the even
+//    channels in rows 0-7 and the odd ones in rows 8-15.  B = the probabilities, from the scores' layout by movmatrix,
+//    rounded to f16 (2^-11; their sum is taken before); the block's scale of V multiplies the step's product as it joins
+//    the accumulator.
 #include <cuda.h>
 #include <cuda_fp16.h>
 
@@ -30,15 +32,24 @@
 namespace nob200 {
 namespace {
 
-constexpr int kBlock = 64, kDim = 128, kBlockBytes = kBlock * kDim;
-constexpr int kWarps = 4, kThreads = 32 * kWarps, kRows = 16, kStages = 3;
+constexpr int kBlock = 64, kDim = 128, kStep = 32, kStepBytes = kStep * kDim;
+constexpr int kWarps = 4, kThreads = 32 * kWarps, kStages = 3;
+constexpr float kRescaleThreshold = 8.0f;  // log2 units: the running maximum is raised, and what is there rescaled, past this growth
+constexpr int kMaxCluster = 8;            // shares that a cluster can hold
 constexpr float kLowestMaximum = -1e38f;  // relative to it a key of score -inf weighs 0
 
+struct Unit {
+  int sequence, index;   // -1: none; which group of columns of it
+  int row0, tokens;      // its new tokens
+  int length, prefix;
+};
+
 struct __align__(1024) Shared {
-  uint8_t ring[kWarps][kStages][kBlockBytes];  // after the last block: the warps' accumulators [16][128] f32
+  uint8_t ring[kWarps][kStages][kStepBytes];  // after the last step: the warps' accumulators [columns][128] f32
   uint64_t full[kWarps][kStages];
-  float top[kWarps][kRows], sum[kWarps][kRows];
-  int unit[2];
+  float top[kWarps][16], sum[kWarps][16];
+  float share_top[16], share_sum[16];  // of the CTA, for the other CTAs of its cluster
+  Unit unit;
   uint32_t abort;
 };
 
@@ -56,7 +67,7 @@ struct CacheParams {
   float* lse;
   uint32_t* status;
   int rows, sequences, max_blocks, num_blocks, heads, kv_heads, group, total_heads, head_offset;
-  int slots, splits, causal;
+  int slots, splits, causal, joined;  // joined: the shares of a unit are a cluster, which joins them itself
   float scale;    // of a raw score; CAP form: divided by the cap
   float to_log2;  // from a (capped) scaled score to log2 units
 };
@@ -87,13 +98,45 @@ __device__ __forceinline__ float rcp(float x) {
 // 1 - 2 / (1 + e^2x): absolute error some 2^-22 for any x
 __device__ __forceinline__ float tanh_any(float x) { return fmaf(-2.f, rcp(1.f + ex2(x * 2.885390081777927f)), 1.f); }
 
-template <bool CAP, bool BIAS>
-__global__ void __launch_bounds__(kThreads, 2)
+// An 8 x 8 matrix of f16 transposed: a lane's two elements of a row become two elements of a column.
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+// ---- clusters: a float of another CTA's shared memory, at this CTA's address of it
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t remote_address(uint32_t mine, int rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(mine), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ float remote_float(uint32_t mine, int rank) {
+  float x;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(remote_address(mine, rank)) : "memory");
+  return x;
+}
+__device__ __forceinline__ float4 remote_float4(uint32_t mine, int rank) {
+  float4 x;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w)
+               : "r"(remote_address(mine, rank))
+               : "memory");
+  return x;
+}
+
+// NT: columns of a CTA in eights.
+template <bool CAP, bool BIAS, int NT>
+__global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3)
 cache_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const CacheParams P) {
+  constexpr int kColumns = 8 * NT;
   extern __shared__ uint8_t smem_raw[];
   Shared& S = *reinterpret_cast<Shared*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int quad = lane >> 2, part = lane & 3;  // row (and key / channel) of a fragment, quarter of its columns
+  const int quad = lane >> 2, part = lane & 3;  // of a fragment: row of A, column of B; and which pair of the other index
   volatile uint32_t* abort_flag = &S.abort;
   if (threadIdx.x == 0) {
     for (int w = 0; w < kWarps; ++w)
@@ -106,50 +149,69 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
   const int key_head = static_cast<int>(blockIdx.x) / P.splits / P.slots;
   pdl_wait();
   if (warp == 0) {
-    const int2 found = find_unit(P.sequences, slot, [&](int s) {
-      const int2 r = document_rows(P.bounds, s, P.rows);
-      return ((r.y - r.x) * P.group + kRows - 1) / kRows;
-    });
-    if (lane == 0) S.unit[0] = found.x, S.unit[1] = found.y;
+    if (lane == 0) S.unit.sequence = -1;
+    __syncwarp();
+    // a lane per sequence, so that all that is to be known about 32 of them is one load's latency away
+    for (int last = P.sequences - 1, before = 0; last >= 0; last -= 32) {
+      const int d = last - lane;
+      int2 r = {};
+      int length = 0, prefix = 0, units = 0;
+      if (d >= 0) {
+        length = P.lengths[d];
+        prefix = P.prefix ? P.prefix[d] : 0;
+        r = document_rows(P.bounds, d, P.rows);
+        units = ((r.y - r.x) * P.group + kColumns - 1) / kColumns;
+      }
+      int through = before + units;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int other = __shfl_up_sync(0xffffffffu, through - before, o);
+        if (lane >= o) through += other;
+      }
+      const bool mine = slot < through && slot >= through - units;
+      if (mine) S.unit = {d, through - 1 - slot, r.x, r.y - r.x, length, prefix};
+      if (__any_sync(0xffffffffu, mine)) break;
+      before = __shfl_sync(0xffffffffu, through, 31);
+    }
   }
   __syncthreads();
   pdl_release();
-  const int sequence = S.unit[0];
-  if (sequence < 0) return;
+  const Unit unit = S.unit;
+  const int sequence = unit.sequence;
+  if (sequence < 0) return;  // the whole cluster
 
-  const int2 rows = document_rows(P.bounds, sequence, P.rows);
-  const int given = P.lengths[sequence];
   Sight sight;
-  sight.keys = clamped(given, 0, P.max_blocks * kBlock);
-  if (given != sight.keys && threadIdx.x == 0) atomicOr(P.status, kBadIndex);
-  sight.ahead = sight.keys - (rows.y - rows.x);
-  sight.prefix = P.prefix ? P.prefix[sequence] : 0;
+  sight.keys = clamped(unit.length, 0, P.max_blocks * kBlock);
+  if (unit.length != sight.keys && threadIdx.x == 0) atomicOr(P.status, kBadIndex);
+  sight.ahead = sight.keys - unit.tokens;
+  sight.prefix = unit.prefix;
   sight.causal = P.causal != 0;
-  const int items = (rows.y - rows.x) * P.group;  // (token, head of the group) pairs
-  const int item0 = S.unit[1] * kRows;
-  const int blocks = (sight.visible((min(items, item0 + kRows) - 1) / P.group) + kBlock - 1) / kBlock;
-  const int begin = static_cast<int>(static_cast<long long>(blocks) * piece / P.splits);
-  const int end = static_cast<int>(static_cast<long long>(blocks) * (piece + 1) / P.splits);
-  const int mine = (end - begin - warp + kWarps - 1) / kWarps;  // blocks of this warp: begin + warp, + kWarps, ...
+  const int items = unit.tokens * P.group;  // (token, head of the group) pairs
+  const int item0 = unit.index * kColumns;
+  const int steps = (sight.visible((min(items, item0 + kColumns) - 1) / P.group) + kStep - 1) / kStep;
+  const int begin = static_cast<int>(static_cast<long long>(steps) * piece / P.splits);
+  const int end = static_cast<int>(static_cast<long long>(steps) * (piece + 1) / P.splits);
+  const int first_step = begin + warp, mine = (end - first_step + kWarps - 1) / kWarps;  // first_step, + kWarps, ...
 
-  // ---- the table two blocks ahead of the loads, the scales one block ahead of their use
-  const int* table = P.table + static_cast<size_t>(sequence) * P.max_blocks + begin + warp;
+  // ---- the table two steps ahead of the loads, the scales one step ahead of their use
+  const int* table = P.table + static_cast<size_t>(sequence) * P.max_blocks;
   auto entry = [&](int i) {
-    int block = i < mine ? table[i * kWarps] : 0;
+    int block = i < mine ? table[(first_step + i * kWarps) / 2] : 0;
     if (block < 0 || block >= P.num_blocks) {
       if (lane == 0) atomicOr(P.status, kBadIndex);
       block = -1;
     }
     return block;
   };
-  uint8_t(*ring)[kBlockBytes] = S.ring[warp];
+  uint8_t(*ring)[kStepBytes] = S.ring[warp];
   uint64_t* full = S.full[warp];
-  auto load = [&](int i, int which, int block) {  // K (0) or V (1) of this warp's i-th block
+  auto load = [&](int i, int which, int block) {  // K (0) or V (1) of this warp's i-th step
     const int n = 2 * i + which;
     if (i < mine && lane == 0) {
-      mbar_expect_tx(&full[n % kStages], kBlockBytes);
+      mbar_expect_tx(&full[n % kStages], kStepBytes);
       // a block that is not there: any block, whose scores are masked
-      tma_load_3d(ring[n % kStages], which ? &map_v : &map_k, &full[n % kStages], 0, (max(block, 0) * P.kv_heads + key_head) * kBlock, 0);
+      tma_load_3d(ring[n % kStages], which ? &map_v : &map_k, &full[n % kStages], 0,
+                  (max(block, 0) * P.kv_heads + key_head) * kBlock + ((first_step + i * kWarps) & 1) * kStep, 0);
     }
   };
   int e0 = entry(0), e1 = entry(1), e2 = entry(2);
@@ -157,21 +219,18 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
   load(0, 1, e0);
   load(1, 0, e1);
 
-  // ---- the 16 rows
-  uint32_t q[kDim / 16][4];
-  float factor[2];  // raw score of the row's f16 form and a key's codes, without the key's scale -> scaled score
-  int visible[2], position[2];
-  float slope[2];
+  // ---- the columns: a lane reads a quarter of column quad of each eight and works on columns 2 part and 2 part + 1
+  uint32_t q[NT][kDim / 16][2];
+  float factor[NT][2];  // raw product of a column's f16 form with a key's codes, without the key's scale -> scaled score
+  int visible[NT][2], position[NT][2];
+  float slope[NT][2];
 #pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    const int item = item0 + quad + 8 * r;
+  for (int n = 0; n < NT; ++n) {
+    const int item = item0 + 8 * n + quad;
     const bool live = item < items;
     const int token = live ? item / P.group : 0, head = key_head * P.group + (live ? item - token * P.group : 0);
-    visible[r] = live ? sight.visible(token) : 0;
-    position[r] = sight.ahead + token;
-    slope[r] = BIAS ? P.slopes[head] * 1.4426950408889634f : 0.f;
     uint32_t w[16];
-    const uint4* src = reinterpret_cast<const uint4*>(P.query + (static_cast<size_t>(rows.x + token) * P.heads + head) * kDim + 32 * part);
+    const uint4* src = reinterpret_cast<const uint4*>(P.query + (static_cast<size_t>(unit.row0 + token) * P.heads + head) * kDim + 32 * part);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const uint4 x = live ? src[i] : make_uint4(0, 0, 0, 0);
@@ -185,22 +244,37 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
     const uint32_t exponent = min(max(__float_as_uint(top) >> 23, 1u), 253u);
     const float down = __uint_as_float((254u - exponent) << 23);
-    factor[r] = __uint_as_float(exponent << 23) * P.scale;
 #pragma unroll
     for (int t = 0; t < 8; ++t)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const uint32_t x = w[2 * t + h];
-        q[t][2 * h + r] = pack_f16(__uint_as_float(x << 16) * down, __uint_as_float(x & 0xffff0000u) * down);
+        q[n][t][h] = pack_f16(__uint_as_float(x << 16) * down, __uint_as_float(x & 0xffff0000u) * down);
       }
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const int from = 4 * (2 * part + c);  // a lane that read the column
+      factor[n][c] = __shfl_sync(0xffffffffu, __uint_as_float(exponent << 23) * P.scale, from);
+      visible[n][c] = __shfl_sync(0xffffffffu, live ? sight.visible(token) : 0, from);
+      position[n][c] = BIAS ? __shfl_sync(0xffffffffu, sight.ahead + token, from) : 0;
+      slope[n][c] = BIAS ? __shfl_sync(0xffffffffu, P.slopes[head] * 1.4426950408889634f, from) : 0.f;
+    }
   }
+  int fewest = visible[0][0];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) fewest = min(fewest, min(visible[n][0], visible[n][1]));
+  fewest = __reduce_min_sync(0xffffffffu, fewest);
 
-  float o[kDim / 8][4];
+  float o[kDim / 16][NT][4];  // channels 16 m + 2 quad (+ 1: the second two), columns 2 part and 2 part + 1
 #pragma unroll
-  for (int n = 0; n < kDim / 8; ++n)
+  for (int m = 0; m < kDim / 16; ++m)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o[n][i] = 0.f;
-  float top[2] = {kLowestMaximum, kLowestMaximum}, sum[2] = {0.f, 0.f};
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) o[m][n][c] = 0.f;
+  float top[NT][2], sum[NT][2];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) top[n][0] = top[n][1] = kLowestMaximum, sum[n][0] = sum[n][1] = 0.f;
   auto scale_of = [&](const float* scales, int block) { return scales[static_cast<size_t>(max(block, 0)) * P.kv_heads + key_head]; };
   float key_scale = mine > 0 ? scale_of(P.key_scales, e0) : 0.f, value_scale = mine > 0 ? scale_of(P.value_scales, e0) : 0.f;
   bool ok = true;
@@ -213,103 +287,143 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     const int nk = 2 * i, nv = 2 * i + 1;
     ok = warp_rest(&full[nk % kStages], (nk / kStages) & 1, abort_flag, P.status, kWaitTimeoutLoad);
     if (!ok) break;
-    float s[kBlock / 8][4];
+    float s[kStep / 16][NT][4];  // keys 16 m + quad (+ 8: the second two), columns 2 part and 2 part + 1
     const uint8_t* k_at = ring[nk % kStages] + quad * kDim;
 #pragma unroll
-    for (int n = 0; n < kBlock / 8; ++n) {
+    for (int m = 0; m < kStep / 16; ++m) {
 #pragma unroll
-      for (int c = 0; c < 4; ++c) s[n][c] = 0.f;
-      uint32_t w[8];  // 32 channels of key 8 n + quad; the swizzle leaves the eight lanes of a phase on different banks
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint4 x = *reinterpret_cast<const uint4*>(k_at + n * 8 * kDim + (((2 * part + h) ^ quad) << 4));
-        w[4 * h] = x.x, w[4 * h + 1] = x.y, w[4 * h + 2] = x.z, w[4 * h + 3] = x.w;
-      }
+        for (int c = 0; c < 4; ++c) s[m][n][c] = 0.f;
 #pragma unroll
-      for (int t = 0; t < 8; ++t) {
-        const uint32_t u = w[t] ^ 0x80808080u;
-        mma_f16(s[n], q[t], widen<0x4140>(u), widen<0x4342>(u));
+      for (int h = 0; h < 2; ++h) {  // 16 of the lane's 32 channels; the swizzle puts the lanes of a phase on different banks
+        const int at = ((2 * part + h) ^ quad) << 4;
+        const uint4 x = *reinterpret_cast<const uint4*>(k_at + (16 * m) * kDim + at);
+        const uint4 y = *reinterpret_cast<const uint4*>(k_at + (16 * m + 8) * kDim + at);
+        const uint32_t w[2][4] = {{x.x, x.y, x.z, x.w}, {y.x, y.y, y.z, y.w}};
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const uint32_t u = w[0][t] ^ 0x80808080u, v = w[1][t] ^ 0x80808080u;
+          const uint32_t a[4] = {widen<0x4140>(u), widen<0x4140>(v), widen<0x4342>(u), widen<0x4342>(v)};
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma_f16(s[m][n], a, q[n][4 * h + t][0], q[n][4 * h + t][1]);
+        }
       }
     }
-    __syncwarp();  // all lanes have read the K block
+    __syncwarp();  // all lanes have read K
     load(i + 1, 1, e1);
 
-    const int key0 = (begin + warp + i * kWarps) * kBlock;
-    const int first = key0 + 2 * part;  // the lane's keys: first + 8 n, first + 8 n + 1
-    float mx[2] = {kLowestMaximum, kLowestMaximum};
-    float alpha[2];
-    const bool whole = e0 >= 0 && __all_sync(0xffffffffu, min(visible[0], visible[1]) >= key0 + kBlock);
+    const int key0 = (first_step + i * kWarps) * kStep;
+    const bool whole = e0 >= 0 && fewest >= key0 + kStep;
+    uint32_t p[kStep / 16][NT][2];
+    float mx[NT][2];
+    bool grown = false;
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const float f = factor[r] * key_scale * (CAP ? 1.f : P.to_log2);
-      const int seen = e0 < 0 ? 0 : visible[r] - first;
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int n = 0; n < kBlock / 8; ++n)
+      for (int c = 0; c < 2; ++c) {
+        const float f = factor[n][c] * key_scale * (CAP ? 1.f : P.to_log2);
+#pragma unroll
+        for (int m = 0; m < kStep / 16; ++m)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float x = s[m][n][2 * h + c] * f;
+            if constexpr (CAP) x = tanh_any(x) * P.to_log2;
+            if constexpr (BIAS) x -= slope[n][c] * static_cast<float>(abs(position[n][c] - (key0 + quad + 16 * m + 8 * h)));
+            s[m][n][2 * h + c] = x;
+          }
+      }
+    if (!whole) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          float x = s[n][2 * r + c] * f;
-          if constexpr (CAP) x = tanh_any(x) * P.to_log2;
-          if constexpr (BIAS) x -= slope[r] * static_cast<float>(abs(position[r] - (first + 8 * n + c)));
-          if (!whole && 8 * n + c >= seen) x = -INFINITY;
-          s[n][2 * r + c] = x;
-          mx[r] = fmaxf(mx[r], x);
+          const int seen = e0 < 0 ? 0 : visible[n][c] - key0 - quad;
+#pragma unroll
+          for (int m = 0; m < kStep / 16; ++m)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              if (16 * m + 8 * h >= seen) s[m][n][2 * h + c] = -INFINITY;
         }
-      mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
-      mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
-      const float now = fmaxf(top[r], mx[r]);
-      alpha[r] = ex2(top[r] - now);
-      top[r] = now;
-      sum[r] *= alpha[r];
     }
-    uint32_t p[kBlock / 16][4];
 #pragma unroll
-    for (int n = 0; n < kBlock / 8; ++n)
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const float a = ex2(s[n][2 * r] - top[r]), b = ex2(s[n][2 * r + 1] - top[r]);
-        sum[r] += a + b;
-        p[n >> 1][2 * (n & 1) + r] = pack_f16(a, b);
+      for (int c = 0; c < 2; ++c) {
+        mx[n][c] = fmaxf(fmaxf(s[0][n][c], s[0][n][2 + c]), fmaxf(s[1][n][c], s[1][n][2 + c]));
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) mx[n][c] = fmaxf(mx[n][c], __shfl_xor_sync(0xffffffffu, mx[n][c], d));
+        grown |= mx[n][c] > top[n][c] + kRescaleThreshold;
       }
+    if (__any_sync(0xffffffffu, grown)) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float alpha[2];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const float now = fmaxf(top[n][c], mx[n][c]);
+          alpha[c] = ex2(top[n][c] - now);
+          top[n][c] = now;
+          sum[n][c] *= alpha[c];
+        }
+#pragma unroll
+        for (int m = 0; m < kDim / 16; ++m)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) o[m][n][c] *= alpha[c & 1];
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int m = 0; m < kStep / 16; ++m)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float a = ex2(s[m][n][2 * h] - top[n][0]), b = ex2(s[m][n][2 * h + 1] - top[n][1]);
+          sum[n][0] += a, sum[n][1] += b;
+          p[m][n][h] = transposed(pack_f16(a, b));
+        }
 
     // ---- values
     ok = warp_rest(&full[nv % kStages], (nv / kStages) & 1, abort_flag, P.status, kWaitTimeoutLoad);
     if (!ok) break;
-    // rows that see nothing of the block take nothing of it, whatever its scale is
-    const float take[2] = {e0 >= 0 && visible[0] > key0 ? value_scale : 0.f, e0 >= 0 && visible[1] > key0 ? value_scale : 0.f};
+    float take[NT][2];  // a column that sees nothing of the step has probabilities of 0 and takes 0 of it, whatever its scale is
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) take[n][c] = e0 >= 0 && visible[n][c] > key0 ? value_scale : 0.f;
     const uint32_t v_at = smem_u32(ring[nv % kStages]);
     const int v_key = ((lane >> 3) & 1) * 8 + (lane & 7);  // ldmatrix: the row whose address this lane gives
 #pragma unroll
-    for (int cc = 0; cc < 4; ++cc) {  // 32 channels
-      float d[4][4];
+    for (int mm = 0; mm < kDim / 32; ++mm) {  // 32 channels
+      float d[2][NT][4];
 #pragma unroll
-      for (int n = 0; n < 4; ++n)
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) d[n][c] = 0.f;
+        for (int c = 0; c < 4; ++c) d[0][n][c] = d[1][n][c] = 0.f;
 #pragma unroll
-      for (int kt = 0; kt < kBlock / 16; ++kt) {
+      for (int kt = 0; kt < kStep / 16; ++kt) {
         const int key = kt * 16 + v_key;
         uint32_t w[4];
         asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
                      : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
-                     : "r"(v_at + key * kDim + (((2 * cc + (lane >> 4)) ^ (key & 7)) << 4))
+                     : "r"(v_at + key * kDim + (((2 * mm + (lane >> 4)) ^ (key & 7)) << 4))
                      : "memory");
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const uint32_t u0 = w[2 * h] ^ 0x80808080u, u1 = w[2 * h + 1] ^ 0x80808080u;
-          mma_f16(d[2 * h], p[kt], widen<0x4240>(u0), widen<0x4240>(u1));      // even channels
-          mma_f16(d[2 * h + 1], p[kt], widen<0x4341>(u0), widen<0x4341>(u1));  // odd channels
+          const uint32_t u = w[2 * h] ^ 0x80808080u, v = w[2 * h + 1] ^ 0x80808080u;
+          const uint32_t a[4] = {widen<0x4240>(u), widen<0x4341>(u), widen<0x4240>(v), widen<0x4341>(v)};
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma_f16(d[h][n], a, p[kt][n][0], p[kt][n][1]);
         }
       }
 #pragma unroll
-      for (int n = 0; n < 4; ++n)
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const int r = c >> 1;
-          const float kept = o[4 * cc + n][c] * alpha[r];
-          o[4 * cc + n][c] = take[r] != 0.f ? fmaf(d[n][c], take[r], kept) : kept;
-        }
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) o[2 * mm + h][n][c] = fmaf(d[h][n][c], take[n][c & 1], o[2 * mm + h][n][c]);
     }
-    __syncwarp();  // all lanes have read the V block
+    __syncwarp();  // all lanes have read V
     load(i + 2, 0, e2);
     e0 = e1, e1 = e2, e2 = e3;
     key_scale = next_key_scale, value_scale = next_value_scale;
@@ -320,54 +434,89 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
   }
 
   // ---- join of the four warps
-#pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 1);
-    sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 2);
-    if (part == 0) S.top[warp][quad + 8 * r] = top[r], S.sum[warp][quad + 8 * r] = sum[r];
-  }
   float* joined = reinterpret_cast<float*>(ring[0]);
 #pragma unroll
-  for (int n = 0; n < 8; ++n)  // a lane's columns of an even / odd pair of n tiles are four consecutive channels
+  for (int n = 0; n < NT; ++n)
 #pragma unroll
-    for (int r = 0; r < 2; ++r)
-      *reinterpret_cast<float4*>(joined + (quad + 8 * r) * kDim + 16 * n + 4 * part) =
-          make_float4(o[2 * n][2 * r], o[2 * n + 1][2 * r], o[2 * n][2 * r + 1], o[2 * n + 1][2 * r + 1]);
+    for (int c = 0; c < 2; ++c) {
+      const int column = 8 * n + 2 * part + c;
+#pragma unroll
+      for (int d = 4; d < 32; d <<= 1) sum[n][c] += __shfl_xor_sync(0xffffffffu, sum[n][c], d);
+      if (quad == 0) S.top[warp][column] = top[n][c], S.sum[warp][column] = sum[n][c];
+#pragma unroll
+      for (int m = 0; m < kDim / 16; ++m)
+        *reinterpret_cast<float2*>(joined + column * kDim + 16 * m + 2 * quad) = make_float2(o[m][n][c], o[m][n][2 + c]);
+    }
   __syncthreads();
-  if (*abort_flag) return;
-  const int row = threadIdx.x >> 3, channel = (threadIdx.x & 7) * 16;
-  const int item = item0 + row;
-  if (item >= items) return;
-  float most = S.top[0][row];
+  constexpr int kLanes = kThreads / kColumns, kEach = kDim / kLanes;  // threads of a column, channels of each
+  const int column = threadIdx.x / kLanes, channel = (threadIdx.x % kLanes) * kEach;
+  float most = S.top[0][column];
 #pragma unroll
-  for (int w = 1; w < kWarps; ++w) most = fmaxf(most, S.top[w][row]);
-  float total = 0.f, acc[16] = {};
+  for (int w = 1; w < kWarps; ++w) most = fmaxf(most, S.top[w][column]);
+  float total = 0.f, acc[kEach] = {};
 #pragma unroll
   for (int w = 0; w < kWarps; ++w) {
-    const float weight = ex2(S.top[w][row] - most);
-    total += weight * S.sum[w][row];
-    const float4* src = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(S.ring[w][0]) + row * kDim + channel);
+    const float weight = ex2(S.top[w][column] - most);
+    total += weight * S.sum[w][column];
+    const float4* src = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(S.ring[w][0]) + column * kDim + channel);
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
+    for (int c = 0; c < kEach / 4; ++c) {
       const float4 x = src[c];
       acc[4 * c] = fmaf(weight, x.x, acc[4 * c]), acc[4 * c + 1] = fmaf(weight, x.y, acc[4 * c + 1]);
       acc[4 * c + 2] = fmaf(weight, x.z, acc[4 * c + 2]), acc[4 * c + 3] = fmaf(weight, x.w, acc[4 * c + 3]);
     }
   }
+  // where a column's output goes; nullptr for a column that is none, or after a wait that gave up
+  auto output_of = [&](int column) -> __nv_bfloat16* {
+    const int item = item0 + column;
+    if (item >= items) return nullptr;
+    const int token = item / P.group, head = key_head * P.group + item - token * P.group, row = unit.row0 + token;
+    if (!NOB_CHECK(row < P.rows && head + P.head_offset < P.total_heads, P.status)) return nullptr;
+    return P.output + (static_cast<size_t>(row) * P.total_heads + head + P.head_offset) * kDim;
+  };
+  if (P.joined) {
+    // every CTA of the cluster leaves its result in its shared memory and joins some channels of all of them
+    float* share = reinterpret_cast<float*>(S.ring[column >> 3][2]) + (column & 7) * kDim + channel;
+#pragma unroll
+    for (int c = 0; c < kEach / 4; ++c)
+      *reinterpret_cast<float4*>(share + 4 * c) = make_float4(acc[4 * c], acc[4 * c + 1], acc[4 * c + 2], acc[4 * c + 3]);
+    if (channel == 0) S.share_top[column] = most, S.share_sum[column] = *abort_flag ? __uint_as_float(0x7fffffffu) : total;
+    cluster_sync();
+    for (int at = piece * kThreads + threadIdx.x; at < kColumns * (kDim / 4); at += P.splits * kThreads) {
+      const int column = at / (kDim / 4), channel = at % (kDim / 4) * 4;
+      const uint32_t tops = smem_u32(&S.share_top[column]), sums = smem_u32(&S.share_sum[column]);
+      const uint32_t from = smem_u32(reinterpret_cast<const float*>(S.ring[column >> 3][2]) + (column & 7) * kDim + channel);
+      float most = kLowestMaximum;
+      for (int z = 0; z < P.splits; ++z) most = fmaxf(most, remote_float(tops, z));
+      float total = 0.f;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int z = 0; z < P.splits; ++z) {
+        const float weight = ex2(remote_float(tops, z) - most);
+        const float4 x = remote_float4(from, z);
+        total = fmaf(weight, remote_float(sums, z), total);
+        acc.x = fmaf(weight, x.x, acc.x), acc.y = fmaf(weight, x.y, acc.y), acc.z = fmaf(weight, x.z, acc.z), acc.w = fmaf(weight, x.w, acc.w);
+      }
+      const float inv = total == 0.f ? 0.f : 1.0f / total;
+      if (__nv_bfloat16* dst = output_of(column))
+        *reinterpret_cast<uint2*>(dst + channel) = make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
+    }
+    cluster_sync();  // nobody reads this CTA's shared memory any more
+    return;
+  }
+  __nv_bfloat16* out = output_of(column);
+  if (!out || *abort_flag) return;
   const float inv = total == 0.f ? 0.f : 1.0f / total;
-  const int token = item / P.group, head = key_head * P.group + item - token * P.group;
-  const size_t out_row = rows.x + token;
-  if (!NOB_CHECK(static_cast<int>(out_row) < P.rows && head + P.head_offset < P.total_heads, P.status)) return;
   if (P.splits > 1) {
-    const size_t at = (static_cast<size_t>(piece) * P.heads + head) * P.rows + out_row;
+    const int item = item0 + column, token = item / P.group, head = key_head * P.group + item - token * P.group;
+    const size_t at = (static_cast<size_t>(piece) * P.heads + head) * P.rows + unit.row0 + token;
     float4* dst = reinterpret_cast<float4*>(P.partial + at * kDim + channel);
 #pragma unroll
-    for (int c = 0; c < 4; ++c) dst[c] = make_float4(acc[4 * c] * inv, acc[4 * c + 1] * inv, acc[4 * c + 2] * inv, acc[4 * c + 3] * inv);
+    for (int c = 0; c < kEach / 4; ++c) dst[c] = make_float4(acc[4 * c] * inv, acc[4 * c + 1] * inv, acc[4 * c + 2] * inv, acc[4 * c + 3] * inv);
     if (channel == 0) P.lse[at] = most + log2f(total);
   } else {
-    uint4* dst = reinterpret_cast<uint4*>(P.output + (out_row * P.total_heads + head + P.head_offset) * kDim + channel);
+    uint4* dst = reinterpret_cast<uint4*>(out + channel);
 #pragma unroll
-    for (int c = 0; c < 2; ++c)
+    for (int c = 0; c < kEach / 8; ++c)
       dst[c] = make_uint4(pack_bf16(acc[8 * c] * inv, acc[8 * c + 1] * inv), pack_bf16(acc[8 * c + 2] * inv, acc[8 * c + 3] * inv),
                           pack_bf16(acc[8 * c + 4] * inv, acc[8 * c + 5] * inv), pack_bf16(acc[8 * c + 6] * inv, acc[8 * c + 7] * inv));
   }
@@ -385,7 +534,7 @@ extern "C" int nob200_int8_cache_attention_d128(int num_rows, int sequences, int
                                                 const void* key_scales, const void* value_scales, const void* table,
                                                 const void* lengths, const void* bounds, const void* prefix,
                                                 const void* slopes, void* output, int heads, int kv_heads, int total_heads,
-                                                int causal, float scale, float cap, int kv_splits, void* workspace,
+                                                int causal, float scale, float cap, int columns, int kv_splits, void* workspace,
                                                 size_t workspace_bytes, void* stream) {
   using namespace nob200;
   const char* name = "int8_cache_attention_d128";
@@ -402,14 +551,16 @@ extern "C" int nob200_int8_cache_attention_d128(int num_rows, int sequences, int
               "%s: a tensor is not 16-byte aligned", name);
   NOB_REQUIRE(scale > 0.f && scale <= 1e30f, "%s: scale %g must be positive and finite", name, scale);
   NOB_REQUIRE(cap >= 0.f && cap <= 1e30f, "%s: cap %g must be finite, 0 for none", name, cap);
+  NOB_REQUIRE(columns == 8 || columns == 16, "%s: columns must be 8 or 16 (got %d)", name, columns);
   NOB_REQUIRE(kv_splits >= 1 && kv_splits <= 64, "%s: kv_splits %d outside [1, 64]", name, kv_splits);
   const int group = heads / kv_heads;
   const long long items = static_cast<long long>(num_rows) * group;
-  NOB_REQUIRE(items + kRows <= 0x7fffffffll, "%s: %d rows x %d heads a key head exceed the limit of 2^31", name, num_rows, group);
-  const long long slots = most_units(items, sequences, kRows);
+  NOB_REQUIRE(items + columns <= 0x7fffffffll, "%s: %d rows x %d heads a key head exceed the limit of 2^31", name, num_rows, group);
+  const long long slots = most_units(items, sequences, columns);
   const long long grid = slots * kv_heads * kv_splits;
   NOB_REQUIRE(grid <= 0x7fffffffll, "%s: %lld units x %d key heads x %d key shares exceed the grid limit", name, slots, kv_heads, kv_splits);
-  const size_t need = key_shares_bytes(num_rows, heads, kv_splits);
+  const bool joined = kv_splits > 1 && kv_splits <= kMaxCluster && !workspace;
+  const size_t need = joined ? 0 : key_shares_bytes(num_rows, heads, kv_splits);
   NOB_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && reinterpret_cast<uintptr_t>(workspace) % 16 == 0),
               "%s: %zu B of 16-byte aligned workspace required for %d key shares, %zu B given", name, need, kv_splits, workspace_bytes);
 
@@ -423,7 +574,7 @@ extern "C" int nob200_int8_cache_attention_d128(int num_rows, int sequences, int
   P.slopes = static_cast<const float*>(slopes);
   P.rows = num_rows, P.sequences = sequences, P.max_blocks = max_blocks, P.num_blocks = num_blocks;
   P.heads = heads, P.kv_heads = kv_heads, P.group = group, P.total_heads = total_heads, P.head_offset = head_offset;
-  P.slots = static_cast<int>(slots), P.splits = kv_splits, P.causal = causal != 0;
+  P.slots = static_cast<int>(slots), P.splits = kv_splits, P.causal = causal != 0, P.joined = joined;
   const float log2e = 1.4426950408889634f;
   P.scale = cap > 0.f ? scale / cap : scale;
   P.to_log2 = cap > 0.f ? cap * log2e : log2e;
@@ -435,15 +586,19 @@ extern "C" int nob200_int8_cache_attention_d128(int num_rows, int sequences, int
   CUtensorMap mk, mv;
   int rc;
   const uint64_t lines = static_cast<uint64_t>(num_blocks) * kv_heads * kBlock;
-  if ((rc = make_tensor_map_3d(&mk, CU_TENSOR_MAP_DATA_TYPE_UINT8, key, kDim, lines, 1, kDim, kDim * lines, kDim, kBlock, 1))) return rc;
-  if ((rc = make_tensor_map_3d(&mv, CU_TENSOR_MAP_DATA_TYPE_UINT8, value, kDim, lines, 1, kDim, kDim * lines, kDim, kBlock, 1))) return rc;
-  auto kernel = cap > 0.f ? (slopes ? cache_attention_kernel<true, true> : cache_attention_kernel<true, false>)
-                          : (slopes ? cache_attention_kernel<false, true> : cache_attention_kernel<false, false>);
+  if ((rc = make_tensor_map_3d(&mk, CU_TENSOR_MAP_DATA_TYPE_UINT8, key, kDim, lines, 1, kDim, kDim * lines, kDim, kStep, 1))) return rc;
+  if ((rc = make_tensor_map_3d(&mv, CU_TENSOR_MAP_DATA_TYPE_UINT8, value, kDim, lines, 1, kDim, kDim * lines, kDim, kStep, 1))) return rc;
+  const bool capped = cap > 0.f;
+  auto kernel = columns == 8 ? (capped ? (slopes ? cache_attention_kernel<true, true, 1> : cache_attention_kernel<true, false, 1>)
+                                       : (slopes ? cache_attention_kernel<false, true, 1> : cache_attention_kernel<false, false, 1>))
+                             : (capped ? (slopes ? cache_attention_kernel<true, true, 2> : cache_attention_kernel<true, false, 2>)
+                                       : (slopes ? cache_attention_kernel<false, true, 2> : cache_attention_kernel<false, false, 2>));
   const size_t smem = sizeof(Shared) + 1024;
   cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (err != cudaSuccess)
     return fail(kCudaError, "%s: cannot reserve %zu B of shared memory: %s", name, smem, cudaGetErrorString(err));
-  if ((rc = launch_pdl(name, kernel, static_cast<unsigned>(grid), kThreads, smem, stream, mk, mv, P))) return rc;
-  if (kv_splits == 1) return kOk;
+  if ((rc = launch_pdl_clusters(name, kernel, static_cast<unsigned>(grid), joined ? kv_splits : 1, kThreads, smem, stream, mk, mv, P)))
+    return rc;
+  if (!need) return kOk;
   return launch_join_shares({P.bounds, P.partial, P.lse, P.output, sequences, num_rows, heads, total_heads, head_offset, kv_splits}, stream);
 }

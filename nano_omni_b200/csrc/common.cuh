@@ -57,6 +57,22 @@ int launch_pdl(const char* what, void (*kernel)(Params...), dim3 grid, dim3 bloc
   (void)cudaLaunchKernelEx(&config, kernel, static_cast<Params>(args)...);
   return check_launch(what);
 }
+// The same with clusters of `cluster` neighbouring CTAs.
+template <typename... Params, typename... Args>
+int launch_pdl_clusters(const char* what, void (*kernel)(Params...), dim3 grid, int cluster, dim3 block, size_t smem, void* stream,
+                        Args&&... args) {
+  cudaLaunchAttribute attributes[2] = {};
+  attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attributes[0].val.programmaticStreamSerializationAllowed = 1;
+  attributes[1].id = cudaLaunchAttributeClusterDimension;
+  attributes[1].val.clusterDim.x = cluster, attributes[1].val.clusterDim.y = 1, attributes[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = grid, config.blockDim = block, config.dynamicSmemBytes = smem;
+  config.stream = static_cast<cudaStream_t>(stream);
+  config.attrs = attributes, config.numAttrs = 2;
+  (void)cudaLaunchKernelEx(&config, kernel, static_cast<Params>(args)...);
+  return check_launch(what);
+}
 }  // namespace nob200
 #endif
 

@@ -608,48 +608,74 @@ fa_fwd_masked_bf16_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
   if (warp == kProducerWarp) tmem_dealloc(tmem, kTmemCols);
 }
 
-// o = sum_z 2^(lse_z - max) o_z / sum_z 2^(lse_z - max).  A thread owns eight channels of a row; a row that no share gave any
-// weight gets zeros.
+// o = sum_z 2^(lse_z - max) o_z / sum_z 2^(lse_z - max).  A thread owns eight channels of a row and every LANES-th share of it, so
+// that many shares of few rows are not read one after the other (42 shares of 14 rows: 12 us by one thread each).  A row that
+// no share gave any weight gets zeros.
+template <int LANES>
 __global__ void __launch_bounds__(256)
 join_shares_kernel(const KeyShares P) {
+  __shared__ float tops[16], sums[16];
+  __shared__ float parts[LANES > 1 ? 256 : 1][8];
   pdl_wait();
-  const long long item = blockIdx.x * 256ll + threadIdx.x;
+  const int group = threadIdx.x >> 4, piece = threadIdx.x & 15, lane = group % LANES;  // a group: one row, one set of shares
   const long long all = static_cast<long long>(P.heads) * P.rows;
-  const long long place = item >> 4;
-  if (place >= all) return;
+  const long long place = blockIdx.x * static_cast<long long>(16 / LANES) + group / LANES;
   const int head = static_cast<int>(place / P.rows), row = static_cast<int>(place - static_cast<long long>(head) * P.rows);
-  if (row < P.bounds[0] || row >= P.bounds[P.documents]) return;
+  const bool live = place < all && row >= P.bounds[0] && row < P.bounds[P.documents];
   float top = -INFINITY;
-  for (int z = 0; z < P.splits; ++z) top = fmaxf(top, P.lse[z * all + place]);
+  if (live)
+    for (int z = lane; z < P.splits; z += LANES) top = fmaxf(top, P.lse[z * all + place]);
+  if (LANES > 1) {
+    if (piece == 0) tops[group] = top;
+    __syncthreads();
+#pragma unroll
+    for (int l = 0; l < LANES; ++l) top = fmaxf(top, tops[group - lane + l]);
+  }
   float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
   float sum = 0.f;
-  for (int z = 0; z < P.splits; ++z) {
-    const long long at = z * all + place;
-    const float lse = P.lse[at];
-    if (lse == -INFINITY) continue;
-    const float w = exp2f(lse - top);
-    sum += w;
-    const float4* src = reinterpret_cast<const float4*>(P.partial + at * 128 + (item & 15) * 8);
-    const float4 x = src[0], y = src[1];
-    const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+  if (live)
+    for (int z = lane; z < P.splits; z += LANES) {
+      const long long at = z * all + place;
+      const float4* src = reinterpret_cast<const float4*>(P.partial + at * 128 + piece * 8);
+      const float4 x = src[0], y = src[1];
+      const float lse = P.lse[at];
+      if (lse == -INFINITY) continue;
+      const float w = exp2f(lse - top);
+      sum += w;
+      const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) acc[i] += w * v[i];
+      for (int i = 0; i < 8; ++i) acc[i] += w * v[i];
+    }
+  if (LANES > 1) {
+    if (piece == 0) sums[group] = sum;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) parts[threadIdx.x][i] = acc[i];
+    __syncthreads();
+    if (lane > 0) return;
+#pragma unroll
+    for (int l = 1; l < LANES; ++l) {
+      sum += sums[group + l];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) acc[i] += parts[threadIdx.x + 16 * l][i];
+    }
   }
+  if (!live) return;
   const float inv = sum == 0.f ? 0.f : 1.0f / sum;
   uint4 v;
   v.x = pack_bf16(acc[0] * inv, acc[1] * inv);
   v.y = pack_bf16(acc[2] * inv, acc[3] * inv);
   v.z = pack_bf16(acc[4] * inv, acc[5] * inv);
   v.w = pack_bf16(acc[6] * inv, acc[7] * inv);
-  *reinterpret_cast<uint4*>(P.output + (static_cast<size_t>(row) * P.total_heads + head + P.head_offset) * 128 + (item & 15) * 8) = v;
+  *reinterpret_cast<uint4*>(P.output + (static_cast<size_t>(row) * P.total_heads + head + P.head_offset) * 128 + piece * 8) = v;
 }
 
 }  // namespace
 
 int launch_join_shares(const KeyShares& shares, void* stream) {
-  const long long items = static_cast<long long>(shares.rows) * shares.heads * 16;
-  return launch_pdl("attention (join of key shares)", join_shares_kernel, static_cast<unsigned>((items + 255) / 256), 256, 0,
-                    stream, shares);
+  const int lanes = shares.splits <= 4 ? 1 : shares.splits <= 16 ? 4 : 16;
+  const long long rows = static_cast<long long>(shares.rows) * shares.heads;
+  auto kernel = lanes == 1 ? join_shares_kernel<1> : lanes == 4 ? join_shares_kernel<4> : join_shares_kernel<16>;
+  return launch_pdl("attention (join of key shares)", kernel, static_cast<unsigned>((rows * lanes + 15) / 16), 256, 0, stream, shares);
 }
 
 }  // namespace nob200

@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import dataclasses
+from typing import Literal, NamedTuple
 
 from pydantic import Field
 
@@ -196,16 +197,39 @@ class CacheAttentionWorkload(CacheWorkload):
     scale: float = Field(default=DEFAULT_SCALE, gt=0, allow_inf_nan=False)
 
 
-def plan_cache_shares(num_rows: int, sequences: int, cached_tokens: int, heads: int, kv_heads: int, sm_count: int = 148) -> int:
-    """Shares of a sequence's blocks, so that the CTAs (two per SM) come to some four rounds of the SMs, and a share still is a
-    block for each of a CTA's four warps."""
-    tiles = max(1, min(num_rows * heads // kv_heads, -(-num_rows * heads // kv_heads // 16) + sequences - 1))
-    blocks = -(-cached_tokens // sequences // BLOCK)
-    return max(1, min(64, blocks // 4, 8 * sm_count // (tiles * kv_heads)))
+MAX_CLUSTER = 8  # up to so many shares need no workspace: their CTAs are a cluster and join them themselves
+
+
+class CacheUnits(NamedTuple):
+    """How a launch becomes CTAs: rows of a sequence and key head (new tokens x query heads) of one, shares of its keys, and
+    whether the shares of a unit are a cluster."""
+
+    columns: int
+    kv_splits: int
+    clusters: bool
+
+
+def plan_cache_units(num_rows: int, sequences: int, cached_tokens: int, heads: int, kv_heads: int, sm_count: int = 148) -> CacheUnits:
+    """Units of a launch whose sequences are taken to be of one length (the device alone knows).
+
+    Eight columns where they hold a sequence's rows.  An SM holds four CTAs of eight columns or three of sixteen.  A launch
+    that has room for all its shares at once takes clusters where eight shares do: 1021 keys x 14 heads 9.2 us, 11.5 with the
+    second launch; one that comes in rounds does not, as a cluster's CTAs wait for room together (64 contexts x 8 key
+    heads 181 us, 200 in clusters of eight)."""
+    group = heads // kv_heads
+    each = -(-num_rows * group // sequences)
+    columns = 8 if each <= 8 else 16
+    units = -(-each // columns) * sequences * kv_heads
+    tokens = -(-cached_tokens // sequences)
+    room = (4 if columns == 8 else 3) * sm_count
+    shares = max(1, min(64, tokens // 128, room // units if 4 * units <= room else -(-8 * room // units)))
+    clusters = 1 < shares and units * min(shares, MAX_CLUSTER) <= room and shares < 12
+    return CacheUnits(columns, min(shares, MAX_CLUSTER) if clusters else shares, clusters)
 
 
 class CacheAttentionConfig(Config):
-    kv_splits: int = Field(default=1, ge=1, le=64)  # > 1: a sequence's blocks over so many CTAs; needs `workspace`
+    columns: Literal[8, 16] = 16  # rows of a CTA
+    kv_splits: int = Field(default=1, ge=1, le=64)  # > 1: a sequence's keys over so many CTAs, clusters of up to 8 without `workspace`
 
 
 @dataclasses.dataclass(frozen=True, slots=True)
@@ -281,13 +305,15 @@ class CacheAttentionKernel(Kernel[CacheAttentionArguments, CacheAttentionWorkloa
 
     def _launch(self, function, stream: int) -> int:
         a, w, c = self.arguments, self.workload, self.config
-        need = share_workspace_bytes(w.num_rows, w.heads, c.kv_splits)
-        assert need == 0 or (a.workspace is not None and a.workspace.num_bytes >= need), "kv_splits > 1 needs workspace"
+        need = share_workspace_bytes(w.num_rows, w.heads, c.kv_splits) if a.workspace is not None else 0
+        assert need or c.kv_splits <= MAX_CLUSTER, f"more than {MAX_CLUSTER} kv_splits need workspace"
+        assert need == 0 or a.workspace.num_bytes >= need, "workspace too small"
         return function(
             ctypes.c_int(w.num_rows), ctypes.c_int(w.sequences), ctypes.c_int(w.max_blocks), ctypes.c_int(w.num_blocks),
             ctypes.c_int(a.head_offset), _lib.ptr(a.query), _lib.ptr(a.key_codes), _lib.ptr(a.value_codes),
             _lib.ptr(a.key_scales), _lib.ptr(a.value_scales), _lib.ptr(a.table), _lib.ptr(a.lengths), _lib.ptr(a.bounds),
             _lib.ptr(a.prefix), _lib.ptr(a.slopes), _lib.ptr(a.output), ctypes.c_int(w.heads), ctypes.c_int(w.kv_heads),
             ctypes.c_int(w.total_heads), ctypes.c_int(int(a.causal)), ctypes.c_float(a.scale), ctypes.c_float(a.cap),
-            ctypes.c_int(c.kv_splits), _lib.ptr(a.workspace), ctypes.c_size_t(need), ctypes.c_void_p(stream),
+            ctypes.c_int(c.columns), ctypes.c_int(c.kv_splits), _lib.ptr(a.workspace), ctypes.c_size_t(need),
+            ctypes.c_void_p(stream),
         )  # fmt: skip

@@ -40,7 +40,7 @@ from nano_omni_b200.kernels.cache import (
     CacheAttentionKernel,
     CacheReadArguments,
     CacheReadKernel,
-    plan_cache_shares,
+    plan_cache_units,
 )
 from nano_omni_b200.kernels.dense_bf16 import (
     DenseBf16AttentionArguments,
@@ -986,8 +986,8 @@ class CacheAttention(Op):
         query, bounds = self.inputs
         cache = self.cache
         sequence = KernelSequence(scratch)
-        splits = plan_cache_shares(self.rows, cache.sequences, self.cached_tokens, self.heads, cache.kv_heads)
-        need = share_workspace_bytes(self.rows, self.heads, splits)
+        units = plan_cache_units(self.rows, cache.sequences, self.cached_tokens, self.heads, cache.kv_heads)
+        need = 0 if units.clusters else share_workspace_bytes(self.rows, self.heads, units.kv_splits)
         sequence.emit(
             CacheAttentionKernel,
             CacheAttentionArguments(
@@ -995,7 +995,7 @@ class CacheAttention(Op):
                 cache.table, cache.lengths, bounds, self.prefix, self.slopes, self.bound_outputs[0], self.head_offset,
                 self.causal, self.scale, self.cap, sequence.temporary("shares", DType.U8, (need,)) if need else None,
             ),
-            CacheAttentionConfig(kv_splits=splits),
+            CacheAttentionConfig(columns=units.columns, kv_splits=units.kv_splits),
         )  # fmt: skip
         return sequence.calls
 

@@ -237,8 +237,10 @@ def test_queries_of_any_size():
             causal=False)  # fmt: skip
 
 
-@pytest.mark.parametrize("splits", [1, 2, 5, 64])
-def test_shares(splits):
+@pytest.mark.parametrize("splits", [1, 2, 5, 8, 9, 17, 64])
+@pytest.mark.parametrize("columns", [8, 16])
+@pytest.mark.parametrize("clusters", [False, True])
+def test_shares(splits, columns, clusters):
     """Every division of the blocks, empty shares among them."""
     from nano_omni_b200.core import DType
     from nano_omni_b200.kernels.cache import CacheAttentionArguments, CacheAttentionConfig, CacheAttentionKernel
@@ -249,14 +251,16 @@ def test_shares(splits):
     cache, c = (x := Cache([900, 0, 70], 2, seed=22)), x.desc()
     q = random_rows(23, 9, 4)
     out = torch.full_like(q, float("nan"))
-    need = share_workspace_bytes(9, 4, splits)
+    if clusters and splits > 8:
+        pytest.skip("more shares than a cluster holds")
+    need = 0 if clusters else share_workspace_bytes(9, 4, splits)
     workspace = desc(torch.empty(need, dtype=torch.uint8, device="cuda"), DType.U8) if need else None
     bounds = ints([0, 4, 6, 9])
     arguments = CacheAttentionArguments(
         desc(q), c.key, c.value, c.key_scales, c.value_scales, c.table, c.lengths, desc(bounds), None, None, desc(out), 0, True,
         workspace=workspace,
     )  # fmt: skip
-    run(CacheAttentionKernel(arguments, CacheAttentionConfig(kv_splits=splits)))
+    run(CacheAttentionKernel(arguments, CacheAttentionConfig(columns=columns, kv_splits=splits)))
     for s, (a, b) in enumerate(((0, 4), (4, 6), (6, 9))):
         want, size = attend(q[a:b], cache.rows(0, s), cache.rows(1, s), causal=True)
         assert ((out[a:b].double() - want).abs() <= HALF * (0.3 * size + want.abs()) + 1e-3).all()

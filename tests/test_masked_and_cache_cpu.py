@@ -180,8 +180,8 @@ def test_c_entries_refuse_before_any_launch(lib):
     refused(fn, (0, 3, 5, 11, p, p, p, p, p, p, p, p, p, 2, null), b"positive")
     refused(fn, (90, 3, 5, 11, p, p, p, p, p, p, p, p, null, 2, null), b"NULL")
 
-    def cached(rows=3, blocks=11, kv_heads=2, splits=1, lengths=p, cap=0.0):
-        return (rows, 3, 5, blocks, 0, p, p, p, p, p, p, lengths, p, null, null, p, 4, kv_heads, 4, 1, f(0.1), f(cap), splits, null, z,
+    def cached(rows=3, blocks=11, kv_heads=2, splits=1, lengths=p, cap=0.0, columns=16):
+        return (rows, 3, 5, blocks, 0, p, p, p, p, p, p, lengths, p, null, null, p, 4, kv_heads, 4, 1, f(0.1), f(cap), columns, splits, null, z,
                 null)  # fmt: skip
 
     fn = lib.nob200_int8_cache_attention_d128
@@ -190,7 +190,8 @@ def test_c_entries_refuse_before_any_launch(lib):
     refused(fn, cached(lengths=null), b"NULL")
     refused(fn, cached(cap=float("inf")), b"cap")
     refused(fn, cached(blocks=1 << 28), b"exceed the limit")
-    refused(fn, cached(splits=2), b"workspace required")
+    refused(fn, cached(splits=9), b"workspace required")
+    refused(fn, cached(columns=12), b"columns")
 
 
 def test_workspace_sizes_are_the_planned_ones(lib):
@@ -199,5 +200,5 @@ def test_workspace_sizes_are_the_planned_ones(lib):
     for name in ("masked_bf16", "int8_cache"):
         fn = getattr(lib, f"nob200_{name}_attention_d128_workspace_bytes")
         fn.restype = ctypes.c_size_t
-        for rows, heads, splits in ((1, 1, 1), (1, 14, 21), (32768, 28, 8), (4096, 56, 64)):
+        for rows, heads, splits in ((1, 1, 1), (1, 14, 21), (32768, 28, 8), (100, 8, 9), (4096, 56, 64)):
             assert fn(rows, heads, splits) == share_workspace_bytes(rows, heads, splits)
