@@ -1,4 +1,5 @@
-// Attention of a few queries per sequence over the 8-bit cache of kv_cache.cu, head_dim 128, sm_100a.
+// Attention of a few queries per sequence over the 8-bit cache of kv_cache.cu, head_dim 128, sm_100a; of many in
+// cache_attention_tiles.cu.
 //
 //   s = scale * q . (code_k * scale_k[block]);  o = sum_j softmax_j(s) code_v * scale_v[block], masks, cap and distance bias as
 // in fa_fwd_masked_bf16.cu.  No counterpart in the reference.
@@ -23,6 +24,7 @@
 #include <cuda.h>
 #include <cuda_fp16.h>
 
+#include "cache_attention.cuh"
 #include "common.cuh"
 #include "documents.cuh"
 #include "fa_common.cuh"
@@ -53,25 +55,6 @@ struct __align__(1024) Shared {
   uint32_t abort;
 };
 
-struct CacheParams {
-  const __nv_bfloat16* query;
-  const float* key_scales;
-  const float* value_scales;
-  const int* table;
-  const int* lengths;
-  const int* bounds;
-  const int* prefix;    // or NULL
-  const float* slopes;  // BIAS form
-  __nv_bfloat16* output;
-  float* partial;  // of KeyShares, when the keys are divided
-  float* lse;
-  uint32_t* status;
-  int rows, sequences, max_blocks, num_blocks, heads, kv_heads, group, total_heads, head_offset;
-  int slots, splits, causal, joined;  // joined: the shares of a unit are a cluster, which joins them itself
-  float scale;    // of a raw score; CAP form: divided by the cap
-  float to_log2;  // from a (capped) scaled score to log2 units
-};
-
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -90,14 +73,6 @@ __device__ __forceinline__ uint32_t widen(uint32_t offset_word) {
   const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&with_exponent), __float2half2_rn(1152.f));
   return *reinterpret_cast<const uint32_t*>(&r);
 }
-__device__ __forceinline__ float rcp(float x) {
-  float y;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-// 1 - 2 / (1 + e^2x): absolute error some 2^-22 for any x
-__device__ __forceinline__ float tanh_any(float x) { return fmaf(-2.f, rcp(1.f + ex2(x * 2.885390081777927f)), 1.f); }
-
 // An 8 x 8 matrix of f16 transposed: a lane's two elements of a row become two elements of a column.
 __device__ __forceinline__ uint32_t transposed(uint32_t x) {
   uint32_t y;
@@ -551,7 +526,7 @@ extern "C" int nob200_int8_cache_attention_d128(int num_rows, int sequences, int
               "%s: a tensor is not 16-byte aligned", name);
   NOB_REQUIRE(scale > 0.f && scale <= 1e30f, "%s: scale %g must be positive and finite", name, scale);
   NOB_REQUIRE(cap >= 0.f && cap <= 1e30f, "%s: cap %g must be finite, 0 for none", name, cap);
-  NOB_REQUIRE(columns == 8 || columns == 16, "%s: columns must be 8 or 16 (got %d)", name, columns);
+  NOB_REQUIRE(columns == 8 || columns == 16 || columns == 128, "%s: columns must be 8, 16 or 128 (got %d)", name, columns);
   NOB_REQUIRE(kv_splits >= 1 && kv_splits <= 64, "%s: kv_splits %d outside [1, 64]", name, kv_splits);
   const int group = heads / kv_heads;
   const long long items = static_cast<long long>(num_rows) * group;
@@ -559,7 +534,7 @@ extern "C" int nob200_int8_cache_attention_d128(int num_rows, int sequences, int
   const long long slots = most_units(items, sequences, columns);
   const long long grid = slots * kv_heads * kv_splits;
   NOB_REQUIRE(grid <= 0x7fffffffll, "%s: %lld units x %d key heads x %d key shares exceed the grid limit", name, slots, kv_heads, kv_splits);
-  const bool joined = kv_splits > 1 && kv_splits <= kMaxCluster && !workspace;
+  const bool joined = kv_splits > 1 && kv_splits <= kMaxCluster && columns < 128 && !workspace;
   const size_t need = joined ? 0 : key_shares_bytes(num_rows, heads, kv_splits);
   NOB_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && reinterpret_cast<uintptr_t>(workspace) % 16 == 0),
               "%s: %zu B of 16-byte aligned workspace required for %d key shares, %zu B given", name, need, kv_splits, workspace_bytes);
@@ -583,8 +558,15 @@ extern "C" int nob200_int8_cache_attention_d128(int num_rows, int sequences, int
     P.lse = P.partial + static_cast<size_t>(kv_splits) * heads * num_rows * kDim;
   }
 
-  CUtensorMap mk, mv;
   int rc;
+  if (columns == 128) {
+    NOB_REQUIRE(static_cast<long long>(num_rows) * total_heads <= 0x7fffffffll, "%s: %d rows x %d heads exceed the limit of 2^31", name,
+                num_rows, total_heads);
+    rc = launch_cache_tiles(P, key, value, cap > 0.f, stream);
+    if (rc || !need) return rc;
+    return launch_join_shares({P.bounds, P.partial, P.lse, P.output, sequences, num_rows, heads, total_heads, head_offset, kv_splits}, stream);
+  }
+  CUtensorMap mk, mv;
   const uint64_t lines = static_cast<uint64_t>(num_blocks) * kv_heads * kBlock;
   if ((rc = make_tensor_map_3d(&mk, CU_TENSOR_MAP_DATA_TYPE_UINT8, key, kDim, lines, 1, kDim, kDim * lines, kDim, kStep, 1))) return rc;
   if ((rc = make_tensor_map_3d(&mv, CU_TENSOR_MAP_DATA_TYPE_UINT8, value, kDim, lines, 1, kDim, kDim * lines, kDim, kStep, 1))) return rc;

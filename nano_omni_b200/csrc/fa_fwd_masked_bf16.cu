@@ -14,8 +14,8 @@
 //  * rows of V behind the document's end (another document's, or anything at all) and rows of it that are not finite would
 //    spoil rows that do not see them: 0 x NaN.  Warp 11 walks the V tiles that are not seen whole before their value
 //    MMAs start, zeroes such rows and notes the non-finite ones; a query row that does see one of those becomes NaN.
-//  * capped scores: tanh by an odd polynomial while all of a warp's rows stay within the cap (seven FMAs, 2.4e-7 absolute
-//    error), else by 1 - 2 / (1 + e^2x) on the MUFU.
+//  * capped scores: tanh by odd polynomials while all of a warp's rows stay within a third of the cap, or within the cap, else
+//    by 1 - 2 / (1 + e^2x) on the MUFU (cap_scores).
 #include <cuda.h>
 
 #include "common.cuh"
@@ -79,28 +79,9 @@ struct MaskedParams {
   uint32_t* status;
   int rows, key_rows, documents, heads, group, total_heads, head_offset;
   int slots, unit_rows, splits, causal;
-  float scale;     // of a raw score; CAP form: divided by the cap
-  float to_log2;   // from a (capped) scaled score to log2 units
+  float scale;    // of a raw score; CAP form: divided by the cap
+  float to_log2;  // from a raw or capped score to log2 units
 };
-
-// tanh(x) = x P(x^2) for |x| <= 1: least squares weighted towards the largest deviation, absolute error 2.4e-7.
-__device__ __forceinline__ uint64_t tanh_small2(uint64_t x) {
-  const uint64_t u = mul2(x, x);
-  uint64_t p = pack2(-0.002839462133550424f, -0.002839462133550424f);
-  p = fma2(p, u, pack2(0.01611417175324844f, 0.01611417175324844f));
-  p = fma2(p, u, pack2(-0.05097285427754116f, -0.05097285427754116f));
-  p = fma2(p, u, pack2(0.1325352487392422f, 0.1325352487392422f));
-  p = fma2(p, u, pack2(-0.3332400372594446f, -0.3332400372594446f));
-  p = fma2(p, u, pack2(0.9999968538421297f, 0.9999968538421297f));
-  return mul2(x, p);
-}
-__device__ __forceinline__ float rcp(float x) {
-  float y;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-// any x: 1 - 2 / (1 + 2^(2 log2(e) x)); absolute error some 2^-22
-__device__ __forceinline__ float tanh_any(float x) { return fmaf(-2.f, rcp(1.f + ex2(x * 2.885390081777927f)), 1.f); }
 
 // The unit of this CTA, by all its threads: a document each, from the last one backwards, so that everything about 384
 // documents is one load's latency away.  Units are numbered from the last document's last one on.
@@ -393,9 +374,8 @@ fa_fwd_masked_bf16_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
       const uint32_t o_addr = tmem + lane_base + kColO + t * kTile;
       const int query = S.unit.query0 + t * kTile + (warp & 3) * 32 + lane;
       const int visible = S.unit.sight.visible(query) - kv_begin * kTile;  // keys of this CTA's that the row sees
-      // a capped score stays in units of the cap until the exponential, a biased one is turned into log2 units at once
-      const float sc = BIAS ? (CAP ? P.to_log2 : P.scale * P.to_log2) : 1.f;
-      const float unit_log2 = BIAS ? 1.f : CAP ? P.to_log2 : P.scale * P.to_log2;
+      // from a raw score to log2 units; capped and biased ones are turned into them at once
+      const float sc = CAP ? 1.f : P.to_log2, unit_log2 = CAP || BIAS ? 1.f : P.to_log2;
       const float slope = BIAS ? P.slopes[head] * 1.4426950408889634f : 0.f;
       const int position = BIAS ? S.unit.sight.ahead + query - kv_begin * kTile : 0;  // relative to this CTA's first key
       float m_used = 0.f;
@@ -412,23 +392,7 @@ fa_fwd_masked_bf16_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&S.s_taken[t]);
-        if constexpr (CAP) {
-          float most = 0.f;
-#pragma unroll
-          for (int i = 0; i < 128; ++i) most = fmaxf(most, fabsf(__uint_as_float(s[i])));
-          if (__all_sync(0xffffffffu, most * P.scale <= 1.f)) {
-            const uint64_t scale2 = pack2(P.scale, P.scale);
-#pragma unroll
-            for (int i = 0; i < 128; i += 2) {
-              float a, b;
-              unpack2(tanh_small2(mul2(pack2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), scale2)), a, b);
-              s[i] = __float_as_uint(a), s[i + 1] = __float_as_uint(b);
-            }
-          } else {
-#pragma unroll
-            for (int i = 0; i < 128; ++i) s[i] = __float_as_uint(tanh_any(__uint_as_float(s[i]) * P.scale));
-          }
-        }
+        if constexpr (CAP) cap_scores(s, P.scale, P.to_log2);
         if constexpr (BIAS) {
           const int key = j * kTile;
           const int first = __shfl_sync(0xffffffffu, position, 0);  // of the warp's rows
@@ -721,7 +685,7 @@ extern "C" int nob200_masked_bf16_attention_d128(int num_rows, int num_key_rows,
   P.slots = static_cast<int>(slots), P.unit_rows = unit_rows, P.splits = kv_splits, P.causal = causal != 0;
   const float log2e = 1.4426950408889634f;
   P.scale = cap > 0.f ? scale / cap : scale;
-  P.to_log2 = cap > 0.f ? cap * log2e : log2e;
+  P.to_log2 = cap > 0.f ? cap * log2e : scale * log2e;
   if (need) {
     P.partial = static_cast<float*>(workspace);
     P.lse = P.partial + static_cast<size_t>(kv_splits) * heads * num_rows * 128;

@@ -212,23 +212,37 @@ class CacheUnits(NamedTuple):
 def plan_cache_units(num_rows: int, sequences: int, cached_tokens: int, heads: int, kv_heads: int, sm_count: int = 148) -> CacheUnits:
     """Units of a launch whose sequences are taken to be of one length (the device alone knows).
 
-    Eight columns where they hold a sequence's rows.  An SM holds four CTAs of eight columns or three of sixteen.  A launch
-    that has room for all its shares at once takes clusters where eight shares do: 1021 keys x 14 heads 9.2 us, 11.5 with the
-    second launch; one that comes in rounds does not, as a cluster's CTAs wait for room together (64 contexts x 8 key
-    heads 181 us, 200 in clusters of eight)."""
-    group = heads // kv_heads
-    each = -(-num_rows * group // sequences)
-    columns = 8 if each <= 8 else 16
+    Up to sixteen rows of a sequence and key head are columns of the small kernel, eight where they do; more take the kernel
+    of 128-row tiles (24 rows against 30000 keys x 8 key heads 34 us, 39 in two groups of columns; 16 rows against 8192 x 4
+    x 16 sequences 62, 41 as columns).  Shares: as many as have room at once - four CTAs of eight columns an SM, two of sixteen,
+    one of tiles - and where less than two have, eight rounds' worth, with 128 or 512 keys each at least.  Clusters where
+    eight shares do: 1021 keys x 14 heads 9.2 us, 11.5 with the second launch; not in rounds, as a cluster's CTAs wait for
+    room together (64 contexts x 8 key heads 181 us, 200 in clusters of eight)."""
+    each = -(-num_rows * (heads // kv_heads) // sequences)
+    columns = 8 if each <= 8 else 16 if each <= 16 else 128
     units = -(-each // columns) * sequences * kv_heads
     tokens = -(-cached_tokens // sequences)
-    room = (4 if columns == 8 else 3) * sm_count
-    shares = max(1, min(64, tokens // 128, room // units if 4 * units <= room else -(-8 * room // units)))
-    clusters = 1 < shares and units * min(shares, MAX_CLUSTER) <= room and shares < 12
-    return CacheUnits(columns, min(shares, MAX_CLUSTER) if clusters else shares, clusters)
+    if columns == 128:
+        # in key tiles of 128: a CTA takes 6 tiles' time beside its own, the join 3.  One sequence's CTAs run in whole rounds;
+        # of several, the longest is taken to hold twice the average, and its CTA to be the last.
+        tiles = max(1, tokens // 128)
+
+        def cost(n: int) -> float:
+            work = units * (tiles + 6 * n) / sm_count + 2 * tiles / n
+            whole = -(-units * n // sm_count) * (tiles / n + 6)
+            return (whole if sequences == 1 else work) + 3 * (n > 1)
+
+        return CacheUnits(columns, min(range(1, max(1, min(64, tiles // 4)) + 1), key=cost), False)
+    room = (4 if columns == 8 else 2) * sm_count
+    if room >= 2 * units:
+        shares = max(1, min(64, tokens // 128, room // units))
+        clusters = 1 < shares < 12 and units * min(shares, MAX_CLUSTER) <= room
+        return CacheUnits(columns, min(shares, MAX_CLUSTER) if clusters else shares, clusters)
+    return CacheUnits(columns, max(1, min(64, tokens // 512, -(-8 * room // units))), False)
 
 
 class CacheAttentionConfig(Config):
-    columns: Literal[8, 16] = 16  # rows of a CTA
+    columns: Literal[8, 16, 128] = 16  # rows of a CTA
     kv_splits: int = Field(default=1, ge=1, le=64)  # > 1: a sequence's keys over so many CTAs, clusters of up to 8 without `workspace`
 
 
@@ -290,7 +304,7 @@ class CacheAttentionKernel(Kernel[CacheAttentionArguments, CacheAttentionWorkloa
         require_tensor(a.output, DType.BF16, (num_rows, total_heads, 128), "output")
         assert kv_heads > 0 and heads % kv_heads == 0, f"{heads} heads cannot share {kv_heads} key heads evenly"
         assert 0 <= a.head_offset <= total_heads - heads, "head slice ends past the output's heads"
-        check_masks(cls.name, a, sequences, heads)
+        check_masks(a, sequences, heads)
         return CacheAttentionWorkload(
             num_rows=num_rows, heads=heads, total_heads=total_heads, sequences=sequences, max_blocks=max_blocks,
             num_blocks=num_blocks, kv_heads=kv_heads, causal=a.causal, use_prefix=a.prefix is not None,

@@ -106,12 +106,11 @@ def share_workspace_bytes(num_rows: int, heads: int, kv_splits: int) -> int:
     return 0 if kv_splits <= 1 else kv_splits * heads * num_rows * 516
 
 
-def check_masks(name: str, arguments, documents: int, heads: int) -> None:
+def check_masks(arguments, documents: int, heads: int) -> None:
     """Checks shared with the attention over a cache."""
     require_tensor(arguments.bounds, DType.I32, (documents + 1,), "bounds")
     if arguments.prefix is not None:
         require_tensor(arguments.prefix, DType.I32, (documents,), "prefix")
-        assert arguments.causal, f"{name}: a prefix widens a causal mask; without one every key is seen"
     if arguments.slopes is not None:
         require_tensor(arguments.slopes, DType.F32, (heads,), "slopes")
 
@@ -153,7 +152,7 @@ class MaskedBf16AttentionKernel(
         assert kv_heads > 0 and heads % kv_heads == 0, f"{heads} heads cannot share {kv_heads} key heads evenly"
         assert 0 <= a.head_offset <= total_heads - heads, "head slice ends past the output's heads"
         documents = a.bounds.shape[0] - 1
-        check_masks(cls.name, a, documents, heads)
+        check_masks(a, documents, heads)
         require_tensor(a.key_bounds, DType.I32, (documents + 1,), "key_bounds")
         return MaskedBf16AttentionWorkload(
             num_rows=num_rows, num_key_rows=num_key_rows, documents=documents, heads=heads, kv_heads=kv_heads,

@@ -827,7 +827,7 @@ class MaskedBf16Attention(Op):
     consecutive query heads share, and other rows than ``query``.
 
     A query stands as far from its document's last key as from its last query.  ``causal`` hides later keys, except the first
-    ``prefix[d]`` (I32 ``[documents]``); ``cap`` > 0 bounds the scores by ``cap * tanh(score / cap)``; ``slopes`` (f32
+    ``prefix[d]`` (I32 ``[documents]``; of no effect without it); ``cap`` > 0 bounds the scores by ``cap * tanh(score / cap)``; ``slopes`` (f32
     ``[heads]``) take ``slopes[h] * distance`` off them.  A row that sees nothing becomes zeros, rows outside the documents
     stay as they are.  No counterpart in the reference, whose attention takes one whole sequence.
     """

@@ -98,10 +98,12 @@ def test_other_keys_than_queries(heads, kv_heads, queries, keys, causal):
 
 
 @pytest.mark.parametrize("prefix", [[1, 0, 0], [200, 129, 5000], [128, 128, 300]])
-def test_prefix(prefix):
+@pytest.mark.parametrize("causal", [True, False])
+def test_prefix(prefix, causal):
+    """Without a causal mask a prefix changes nothing."""
     lengths = [390, 200, 300]
     q, k, v = rows(7, 890, 2), rows(8, 890, 2), rows(9, 890, 2)
-    compare(q, k, v, ends(lengths), causal=True, prefix=prefix)
+    compare(q, k, v, ends(lengths), causal=causal, prefix=prefix)
 
 
 @pytest.mark.parametrize("spread,cap", [(1.0, 50.0), (6.0, 20.0), (6.0, 1.0), (40.0, 30.0), (1.0, 0.05)])

@@ -53,7 +53,6 @@ def test_rotation_comes_in_front():
         {"kv_heads": 3},  # does not divide the heads
         {"head_offset": 3},
         {"key_rows": 200},  # fewer keys than queries need bounds of their own
-        {"prefix": (DType.I32, 3)},  # a prefix without a causal mask
         {"causal": True, "prefix": (DType.I32, 2)},
         {"causal": True, "prefix": (DType.F32, 3)},
         {"slopes": (DType.F32, 2)},
@@ -103,8 +102,8 @@ def test_cache_operators_refuse():
         ops.CacheRead(c, 900).to(at(DType.BF16, 800, 256), at(DType.BF16, 900, 256), at(DType.I32, 4))
     with pytest.raises(AssertionError):  # heads that cannot share two key heads
         ops.CacheAttention(at(DType.BF16, 3, 384), at(DType.I32, 4), c, total_heads=3)
-    with pytest.raises(AssertionError):  # a prefix without a causal mask
-        op = ops.CacheAttention(at(DType.BF16, 3, 512), at(DType.I32, 4), c, total_heads=4, causal=False, prefix=at(DType.I32, 3))
+    with pytest.raises(AssertionError):  # a prefix for another number of sequences
+        op = ops.CacheAttention(at(DType.BF16, 3, 512), at(DType.I32, 4), c, total_heads=4, prefix=at(DType.I32, 2))
         op.to(at(DType.BF16, 3, 4, 128)).prepare()
     for field, wrong in (("key_scales", (DType.F32, 20, 3)), ("table", (DType.F32, 3, 8)), ("lengths", (DType.I32, 2)),
                          ("value", (DType.I8, 20, 2, 32, 128))):  # fmt: skip
