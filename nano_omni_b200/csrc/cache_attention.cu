@@ -52,6 +52,7 @@ struct __align__(1024) Shared {
   float top[kWarps][16], sum[kWarps][16];
   float share_top[16], share_sum[16];  // of the CTA, for the other CTAs of its cluster
   Unit unit;
+  int units[kWarps];
   uint32_t abort;
 };
 
@@ -116,40 +117,32 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
   if (threadIdx.x == 0) {
     for (int w = 0; w < kWarps; ++w)
       for (int s = 0; s < kStages; ++s) mbar_init(&S.full[w][s], 1);
+    S.unit.sequence = -1;
     S.abort = 0;
     mbar_fence_init();
   }
+  __syncthreads();
   const int piece = static_cast<int>(blockIdx.x) % P.splits;
   const int slot = static_cast<int>(blockIdx.x) / P.splits % P.slots;
   const int key_head = static_cast<int>(blockIdx.x) / P.splits / P.slots;
   pdl_wait();
-  if (warp == 0) {
-    if (lane == 0) S.unit.sequence = -1;
-    __syncwarp();
-    // a lane per sequence, so that all that is to be known about 32 of them is one load's latency away
-    for (int last = P.sequences - 1, before = 0; last >= 0; last -= 32) {
-      const int d = last - lane;
-      int2 r = {};
-      int length = 0, prefix = 0, units = 0;
-      if (d >= 0) {
-        length = P.lengths[d];
-        prefix = P.prefix ? P.prefix[d] : 0;
-        r = document_rows(P.bounds, d, P.rows);
-        units = ((r.y - r.x) * P.group + kColumns - 1) / kColumns;
-      }
-      int through = before + units;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int other = __shfl_up_sync(0xffffffffu, through - before, o);
-        if (lane >= o) through += other;
-      }
-      const bool mine = slot < through && slot >= through - units;
-      if (mine) S.unit = {d, through - 1 - slot, r.x, r.y - r.x, length, prefix};
-      if (__any_sync(0xffffffffu, mine)) break;
-      before = __shfl_sync(0xffffffffu, through, 31);
-    }
-  }
-  __syncthreads();
+  struct Sequence {
+    int2 rows;
+    int length, prefix, units;
+  };
+  find_unit<kThreads, true>(
+      P.sequences, slot, S.units,
+      [&](int d, bool live) {
+        Sequence r = {};
+        if (live) {
+          r.length = P.lengths[d];
+          r.prefix = P.prefix ? P.prefix[d] : 0;
+          r.rows = document_rows(P.bounds, d, P.rows);
+          r.units = ((r.rows.y - r.rows.x) * P.group + kColumns - 1) / kColumns;
+        }
+        return r;
+      },
+      [&](const Sequence& r, int d, int index) { S.unit = {d, index, r.rows.x, r.rows.y - r.rows.x, r.length, r.prefix}; });
   pdl_release();
   const Unit unit = S.unit;
   const int sequence = unit.sequence;

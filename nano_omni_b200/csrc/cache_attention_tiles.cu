@@ -73,55 +73,42 @@ struct __align__(1024) Shared {
 };
 static_assert(sizeof(Shared) + 1024 <= 227 * 1024, "shared memory of an SM");
 
-// The unit of this CTA, by all its threads: a sequence each, from the last one backwards.
+// The unit of this CTA, into shared memory.
 __device__ __forceinline__ void find_own_unit(const CacheParams& P, Shared& S, int slot, int piece) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int last = P.sequences - 1; last >= 0; last -= kThreads) {
-    const int d = last - static_cast<int>(threadIdx.x);
-    int2 rows = {};
-    int length = 0, prefix = 0, units = 0;
-    if (d >= 0) {
-      length = P.lengths[d];
-      prefix = P.prefix ? P.prefix[d] : 0;
-      rows = document_rows(P.bounds, d, P.rows);
-      units = ((rows.y - rows.x) * P.group + kTile - 1) / kTile;
-    }
-    int through = units;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int other = __shfl_up_sync(0xffffffffu, through, o);
-      if (lane >= o) through += other;
-    }
-    if (lane == 31) S.units[warp] = through;
-    __syncthreads();
-    int total = 0;
-#pragma unroll
-    for (int w = 0; w < kThreads / 32; ++w) {
-      if (w == warp) through += total;
-      total += S.units[w];
-    }
-    if (slot < through && slot >= through - units) {
-      Unit u;
-      const int tokens = rows.y - rows.x;
-      u.sequence = d;
-      u.item0 = (through - 1 - slot) * kTile;
-      u.items = tokens * P.group - u.item0;
-      u.row0 = rows.x;
-      u.sight.keys = clamped(length, 0, P.max_blocks * kBlock);
-      if (u.sight.keys != length) atomicOr(P.status, kBadIndex);
-      u.sight.ahead = u.sight.keys - tokens;
-      u.sight.prefix = prefix;
-      u.sight.causal = P.causal != 0;
-      const int seen = u.sight.visible((u.item0 + min(u.items, kTile) - 1) / P.group);
-      const int tiles = (seen + kTile - 1) / kTile;
-      u.kv_begin = static_cast<int>(static_cast<long long>(tiles) * piece / P.splits);
-      u.kv_end = static_cast<int>(static_cast<long long>(tiles) * (piece + 1) / P.splits);
-      S.unit = u;
-    }
-    __syncthreads();
-    if (slot < total) return;
-    slot -= total;
-  }
+  struct Sequence {
+    int2 rows;
+    int length, prefix, units;
+  };
+  find_unit<kThreads, true>(
+      P.sequences, slot, S.units,
+      [&](int d, bool live) {
+        Sequence r = {};
+        if (live) {
+          r.length = P.lengths[d];
+          r.prefix = P.prefix ? P.prefix[d] : 0;
+          r.rows = document_rows(P.bounds, d, P.rows);
+          r.units = ((r.rows.y - r.rows.x) * P.group + kTile - 1) / kTile;
+        }
+        return r;
+      },
+      [&](const Sequence& r, int d, int index) {
+        Unit u;
+        const int tokens = r.rows.y - r.rows.x;
+        u.sequence = d;
+        u.item0 = index * kTile;
+        u.items = tokens * P.group - u.item0;
+        u.row0 = r.rows.x;
+        u.sight.keys = clamped(r.length, 0, P.max_blocks * kBlock);
+        if (u.sight.keys != r.length) atomicOr(P.status, kBadIndex);
+        u.sight.ahead = u.sight.keys - tokens;
+        u.sight.prefix = r.prefix;
+        u.sight.causal = P.causal != 0;
+        const int seen = u.sight.visible((u.item0 + min(u.items, kTile) - 1) / P.group);
+        const int tiles = (seen + kTile - 1) / kTile;
+        u.kv_begin = static_cast<int>(static_cast<long long>(tiles) * piece / P.splits);
+        u.kv_end = static_cast<int>(static_cast<long long>(tiles) * (piece + 1) / P.splits);
+        S.unit = u;
+      });
 }
 
 // The block of keys 64 b .. 64 b + 63; -1 and a note for one that is not there, -1 without past the table.

@@ -26,28 +26,37 @@ __device__ __forceinline__ int2 document_rows(const int* bounds, int d, int rows
   return make_int2(begin, clamped(bounds[d + 1], begin, rows));
 }
 
-// The `slot`-th unit, counted from the last document's last unit backwards, where document d has units_of(d) of them: of
-// documents of one length the longest key ranges of a causal mask come first, which leaves the short ones for the end of the
-// launch.  Called by a converged warp; (document, unit in it), or (-1, 0) when there are fewer units.
-template <typename UnitsOf>
-__device__ __forceinline__ int2 find_unit(int documents, int slot, const UnitsOf& units_of) {
-  const int lane = threadIdx.x & 31;
-  for (int last = documents - 1; last >= 0; last -= 32) {
-    const int d = last - lane;
-    int through = d >= 0 ? units_of(d) : 0;
+// Finds the `slot`-th unit of `count` documents with all THREADS threads of a CTA, a document each, so that what is to be known of
+// THREADS documents is one load's latency away: load(d) brings a document's record to its thread and returns its units, and
+// the thread of the document that the unit is in is told (record, document, unit in it) before the barrier.  `totals` is shared
+// memory of THREADS / 32 words.  BACKWARDS: documents, and the units of each, are counted from the last one on - of documents
+// of one length the longest key ranges of a causal mask come first, and the short ones are left for the end of the launch.
+template <int THREADS, bool BACKWARDS, typename Load, typename Found>
+__device__ __forceinline__ void find_unit(int count, int slot, int* totals, const Load& load, const Found& found) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int base = 0; base < count; base += THREADS) {
+    const int at = base + static_cast<int>(threadIdx.x), d = BACKWARDS ? count - 1 - at : at;
+    const auto record = load(d, at < count);
+    const int units = record.units;
+    int through = units;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int other = __shfl_up_sync(0xffffffffu, through, o);
       if (lane >= o) through += other;
     }
-    const unsigned mine = __ballot_sync(0xffffffffu, slot < through);
-    if (mine) {
-      const int from = __ffs(mine) - 1;
-      return make_int2(last - from, __shfl_sync(0xffffffffu, through, from) - 1 - slot);
+    if (lane == 31) totals[warp] = through;
+    __syncthreads();
+    int total = 0;
+#pragma unroll
+    for (int w = 0; w < THREADS / 32; ++w) {
+      if (w == warp) through += total;
+      total += totals[w];
     }
-    slot -= __shfl_sync(0xffffffffu, through, 31);
+    if (slot < through && slot >= through - units) found(record, d, BACKWARDS ? through - 1 - slot : slot - (through - units));
+    __syncthreads();
+    if (slot < total) return;
+    slot -= total;
   }
-  return make_int2(-1, 0);
 }
 
 // What the queries of a document see: query i of `queries` stands at position i + keys - queries and sees the first

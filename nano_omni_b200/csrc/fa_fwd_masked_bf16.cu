@@ -83,54 +83,40 @@ struct MaskedParams {
   float to_log2;  // from a raw or capped score to log2 units
 };
 
-// The unit of this CTA, by all its threads: a document each, from the last one backwards, so that everything about 384
-// documents is one load's latency away.  Units are numbered from the last document's last one on.
+// The unit of this CTA, into shared memory.
 __device__ __forceinline__ void find_own_unit(const MaskedParams& P, Shared& S, int slot, int piece) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int last = P.documents - 1; last >= 0; last -= kThreads) {
-    const int d = last - static_cast<int>(threadIdx.x);
-    int2 rows = {}, keys = {};
-    int prefix = 0, units = 0;
-    if (d >= 0) {
-      keys = document_rows(P.key_bounds, d, P.key_rows);
-      prefix = P.prefix ? P.prefix[d] : 0;
-      rows = document_rows(P.bounds, d, P.rows);
-      units = (rows.y - rows.x + P.unit_rows - 1) / P.unit_rows;
-    }
-    int through = units;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int other = __shfl_up_sync(0xffffffffu, through, o);
-      if (lane >= o) through += other;
-    }
-    if (lane == 31) S.units[warp] = through;
-    __syncthreads();
-    int total = 0;
-#pragma unroll
-    for (int w = 0; w < kThreads / 32; ++w) {
-      if (w == warp) through += total;
-      total += S.units[w];
-    }
-    if (slot < through && slot >= through - units) {
-      Unit u;
-      u.query0 = (through - 1 - slot) * P.unit_rows;
-      u.row0 = rows.x + u.query0;
-      u.rows = rows.y - u.row0;
-      u.key0 = keys.x;
-      u.sight.keys = keys.y - keys.x;
-      u.sight.ahead = u.sight.keys - (rows.y - rows.x);
-      u.sight.prefix = prefix;
-      u.sight.causal = P.causal != 0;
-      const int seen = u.sight.visible(u.query0 + min(u.rows, P.unit_rows) - 1);
-      const int tiles = (seen + kTile - 1) / kTile;
-      u.kv_begin = static_cast<int>(static_cast<long long>(tiles) * piece / P.splits);
-      u.kv_end = static_cast<int>(static_cast<long long>(tiles) * (piece + 1) / P.splits);
-      S.unit = u;
-    }
-    __syncthreads();
-    if (slot < total) return;
-    slot -= total;
-  }
+  struct Document {
+    int2 rows, keys;
+    int prefix, units;
+  };
+  find_unit<kThreads, true>(
+      P.documents, slot, S.units,
+      [&](int d, bool live) {
+        Document r = {};
+        if (live) {
+          r.keys = document_rows(P.key_bounds, d, P.key_rows);
+          r.prefix = P.prefix ? P.prefix[d] : 0;
+          r.rows = document_rows(P.bounds, d, P.rows);
+          r.units = (r.rows.y - r.rows.x + P.unit_rows - 1) / P.unit_rows;
+        }
+        return r;
+      },
+      [&](const Document& r, int, int index) {
+        Unit u;
+        u.query0 = index * P.unit_rows;
+        u.row0 = r.rows.x + u.query0;
+        u.rows = r.rows.y - u.row0;
+        u.key0 = r.keys.x;
+        u.sight.keys = r.keys.y - r.keys.x;
+        u.sight.ahead = u.sight.keys - (r.rows.y - r.rows.x);
+        u.sight.prefix = r.prefix;
+        u.sight.causal = P.causal != 0;
+        const int seen = u.sight.visible(u.query0 + min(u.rows, P.unit_rows) - 1);
+        const int tiles = (seen + kTile - 1) / kTile;
+        u.kv_begin = static_cast<int>(static_cast<long long>(tiles) * piece / P.splits);
+        u.kv_end = static_cast<int>(static_cast<long long>(tiles) * (piece + 1) / P.splits);
+        S.unit = u;
+      });
 }
 
 template <bool CAP, bool BIAS>

@@ -110,6 +110,28 @@ def test_append(before, new, spread):
     assert all(torch.equal(a, b) for a, b in zip(again, cache.codes))
 
 
+@pytest.mark.parametrize("bits", [0x3C7FFFFF, 0x3D7FFFFF, 0x3D000000, 0x3CFFFFFE, 0x3D2AAAAB])
+def test_append_divides_as_ieee_does(bits):
+    """Codes by scales that are there, one significand of all ones among them, for every bf16 value up to the largest code."""
+    cache = Cache([1 + 63], 1, seed=33)
+    scale = torch.tensor([bits], dtype=torch.int32, device="cuda").view(torch.float32)
+    block = cache.table[0, 0].long()
+    top = float(scale) * 127
+    x = torch.arange(0x7F80, dtype=torch.int32, device="cuda").to(torch.int16).view(torch.bfloat16)
+    x = x[x.float() <= top]
+    for part in x.split(63 * 128):
+        rows = torch.zeros(63 * 128, dtype=torch.bfloat16, device="cuda")
+        rows[: len(part)] = part * torch.where(torch.arange(len(part), device="cuda") % 2 == 0, 1, -1).bfloat16()
+        rows = rows.view(63, 1, 128)
+        for which in range(2):
+            cache.scales[which][block] = scale
+        run_op(append_op(cache, rows, rows, ints([0, 63])))
+        want = torch.round(rows.float() / scale).to(torch.int8)[:, 0]
+        for which in range(2):
+            assert torch.equal(cache.scales[which][block], scale)
+            assert torch.equal(cache.codes[which][block, 0, 1:], want)
+
+
 def test_append_token_by_token_stays_near_the_values():
     """64 tokens appended one at a time: every raise of the scale rounds what is there once more, by half a step at most."""
     cache = Cache([64], 2, seed=4)
