@@ -159,12 +159,14 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
   const int steps = (sight.visible((min(items, item0 + kColumns) - 1) / P.group) + kStep - 1) / kStep;
   const int begin = static_cast<int>(static_cast<long long>(steps) * piece / P.splits);
   const int end = static_cast<int>(static_cast<long long>(steps) * (piece + 1) / P.splits);
-  const int first_step = begin + warp, mine = (end - first_step + kWarps - 1) / kWarps;  // first_step, + kWarps, ...
+  const int first_step = begin + warp, mine = (end - first_step + kWarps - 1) / kWarps;
+  // first_step, + kWarps, ...; under a distance bias from the last, and so nearest and largest, one backwards
+  auto step_at = [&](int i) { return first_step + (BIAS ? mine - 1 - i : i) * kWarps; };
 
   // ---- the table two steps ahead of the loads, the scales one step ahead of their use
   const int* table = P.table + static_cast<size_t>(sequence) * P.max_blocks;
   auto entry = [&](int i) {
-    int block = i < mine ? table[(first_step + i * kWarps) / 2] : 0;
+    int block = i < mine ? table[step_at(i) / 2] : 0;
     if (block < 0 || block >= P.num_blocks) {
       if (lane == 0) atomicOr(P.status, kBadIndex);
       block = -1;
@@ -179,7 +181,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
       mbar_expect_tx(&full[n % kStages], kStepBytes);
       // a block that is not there: any block, whose scores are masked
       tma_load_3d(ring[n % kStages], which ? &map_v : &map_k, &full[n % kStages], 0,
-                  (max(block, 0) * P.kv_heads + key_head) * kBlock + ((first_step + i * kWarps) & 1) * kStep, 0);
+                  (max(block, 0) * P.kv_heads + key_head) * kBlock + (step_at(i) & 1) * kStep, 0);
     }
   };
   int e0 = entry(0), e1 = entry(1), e2 = entry(2);
@@ -281,7 +283,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     __syncwarp();  // all lanes have read K
     load(i + 1, 1, e1);
 
-    const int key0 = (first_step + i * kWarps) * kStep;
+    const int key0 = step_at(i) * kStep;
     const bool whole = e0 >= 0 && fewest >= key0 + kStep;
     uint32_t p[kStep / 16][NT][2];
     float mx[NT][2];

@@ -185,6 +185,8 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
   const int items = S.unit.items;  // 0: no unit
   const int kv_begin = S.unit.kv_begin, n_kv = S.unit.kv_end - kv_begin;
   const int* table = P.table + static_cast<size_t>(S.unit.sequence) * P.max_blocks;
+  // the order of the key tiles: under a distance bias from the last, and so nearest and largest, one backwards
+  auto tile_at = [&](int j) { return BIAS ? n_kv - 1 - j : j; };
   auto spin = [&](uint64_t* bar, uint32_t parity, uint32_t bit) { return warp_poll(bar, parity, abort_flag, status, bit); };
   auto rest = [&](uint64_t* bar, uint32_t parity, uint32_t bit) { return warp_rest(bar, parity, abort_flag, status, bit); };
 
@@ -205,7 +207,7 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
       auto blocks_from = [&](int i) {
         Blocks r = {-1, 0.f, kNotThere};
         if (i + lane < 2 * n_kv) {
-          const int at = 2 * kv_begin + i + lane;
+          const int at = 2 * (kv_begin + tile_at((i + lane) >> 1)) + ((i + lane) & 1);
           r.number = block_of(P, table, at);
           if (r.number < 0 && at * kBlock < S.unit.sight.keys) atomicOr(status, kBadIndex);
           if (v && r.number >= 0) {
@@ -399,16 +401,16 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         const volatile float* kept = &S.scales[block % kScaleSlots].x;
         const float key_scale = kept[0] * row_scale, value_scale = kept[1];
         const bool there = value_scale != kNotThere;
-        const int valid = visible - j * kTile;
+        const int valid = visible - tile_at(j) * kTile;
         // from a raw score to log2 units; a capped or biased one is turned into them at once
         const float unit = CAP || BIAS ? 1.f : key_scale * P.to_log2;
         if constexpr (CAP) cap_scores(s, key_scale, P.to_log2);
         if constexpr (BIAS) {
-          const float from = static_cast<float>(position - j * kTile), f = CAP ? 1.f : key_scale * P.to_log2;
+          const float from = static_cast<float>(position - tile_at(j) * kTile), f = CAP ? 1.f : key_scale * P.to_log2;
 #pragma unroll
           for (int i = 0; i < 64; ++i) s[i] = __float_as_uint(fmaf(__uint_as_float(s[i]), f, -slope * fabsf(from - static_cast<float>(i))));
         }
-        if (j >= partly || !there) {
+        if (tile_at(j) >= partly || !there) {
 #pragma unroll
           for (int i = 0; i < 64; ++i)
             if (i >= valid || !there) s[i] = 0xff800000u;  // -inf

@@ -170,6 +170,11 @@ fa_fwd_masked_bf16_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
   const int n_kv = S.unit.kv_end - S.unit.kv_begin;
   const int kv_begin = S.unit.kv_begin;
   const bool two = unit_rows > kTile;
+  // The order of the key tiles: a distance bias makes the nearest ones the largest, so they come first, from the last row's own
+  // backwards, then the ones ahead.  (From the first key on, steep slopes raised the maximum with every tile: 15104 causal rows x
+  // 14 heads 1065 us.)
+  const int nearest = BIAS ? clamped((S.unit.sight.ahead + S.unit.query0 + unit_rows - 1) / kTile - kv_begin, 0, n_kv - 1) : -1;
+  auto tile_at = [&](int j) { return j <= nearest ? nearest - j : j; };
   // key tiles from this one on (of this CTA's) are not seen whole by the unit's first row
   const int partly = max(0, S.unit.sight.visible(S.unit.query0) / kTile - kv_begin);
 
@@ -199,7 +204,7 @@ fa_fwd_masked_bf16_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
           }
           mbar_expect_tx(&S.kv_full[st], kTileBytes);
           const CUtensorMap* map = (i & 1) ? &map_v : &map_k;
-          const int token = key0 + (kv_begin + (i >> 1)) * kTile;
+          const int token = key0 + (kv_begin + tile_at(i >> 1)) * kTile;
           tma_load_3d(S.kv[st], map, &S.kv_full[st], 0, key_head, token);
           tma_load_3d(S.kv[st] + kHalfBytes, map, &S.kv_full[st], 64, key_head, token);
           issued = i + 1;
@@ -220,10 +225,10 @@ fa_fwd_masked_bf16_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
       for (int j = 0; j < n_kv; ++j) {
         const int st = (2 * j + 1) % kStages, which = j & 1;
         if (!warp_rest(&S.kv_full[st], ((2 * j + 1) / kStages) & 1, abort_flag, status, kWaitTimeoutLoad)) break;
-        const int left = S.unit.sight.keys - (kv_begin + j) * kTile;  // rows of the tile that belong to the document
+        const int tile = tile_at(j), left = S.unit.sight.keys - (kv_begin + tile) * kTile;  // rows of the tile that belong to the document
         bool wrote = false;
 #pragma unroll 1
-        for (int k = 0; k < 4 && j >= partly; ++k) {
+        for (int k = 0; k < 4 && tile >= partly; ++k) {
           const int row = 32 * k + lane;
           uint8_t* at[2] = {S.kv[st] + row * 128, S.kv[st] + kHalfBytes + row * 128};
           // x * 0 is NaN for a value that is not finite, else 0
@@ -380,7 +385,7 @@ fa_fwd_masked_bf16_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
         if (lane == 0) mbar_arrive(&S.s_taken[t]);
         if constexpr (CAP) cap_scores(s, P.scale, P.to_log2);
         if constexpr (BIAS) {
-          const int key = j * kTile;
+          const int key = tile_at(j) * kTile;
           const int first = __shfl_sync(0xffffffffu, position, 0);  // of the warp's rows
           const bool below = key + kTile - 1 <= first, above = key >= first + 31;
           if (below || above) {
@@ -403,8 +408,8 @@ fa_fwd_masked_bf16_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
             }
           }
         }
-        if (j >= partly && __any_sync(0xffffffffu, visible < (j + 1) * kTile)) {
-          const int valid = visible - j * kTile;
+        if (tile_at(j) >= partly && __any_sync(0xffffffffu, visible < (tile_at(j) + 1) * kTile)) {
+          const int valid = visible - tile_at(j) * kTile;
 #pragma unroll
           for (int i = 0; i < 128; ++i)
             if (i >= valid) s[i] = 0xff800000u;  // -inf
@@ -438,11 +443,11 @@ fa_fwd_masked_bf16_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
           tmem_scale_rows(o_addr, alpha);
           m_used = m_new;
         }
-        if (j >= partly) {
+        if (tile_at(j) >= partly) {
           // which of the tile's rows of V were not finite; before the probabilities go, as the note is overwritten after them
           ok = poll(&S.v_clean[j & 1], (j >> 1) & 1, kWaitTimeoutLoad);
           if (!ok) break;
-          const int valid = visible - j * kTile;
+          const int valid = visible - tile_at(j) * kTile;
           uint32_t bad = 0;
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
