@@ -52,7 +52,7 @@ struct __align__(1024) Shared {
   float top[kWarps][16], sum[kWarps][16];
   float share_top[16], share_sum[16];  // of the CTA, for the other CTAs of its cluster
   Unit unit;
-  int units[kWarps];
+  FindScratch<kThreads> find;
   uint32_t abort;
 };
 
@@ -122,20 +122,20 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     mbar_fence_init();
   }
   __syncthreads();
-  const int piece = static_cast<int>(blockIdx.x) % P.splits;
-  const int slot = static_cast<int>(blockIdx.x) / P.splits % P.slots;
-  const int key_head = static_cast<int>(blockIdx.x) / P.splits / P.slots;
+  // all key heads of a unit are neighbours in the grid, the longest sequences' units first
+  const int piece = static_cast<int>(blockIdx.x) % P.splits, place = static_cast<int>(blockIdx.x) / P.splits;
+  const int key_head = place % P.kv_heads, slot = place / P.kv_heads;
   pdl_wait();
   struct Sequence {
     int2 rows;
-    int length, prefix, units;
+    int length, prefix, units, weight;
   };
   find_unit<kThreads, true>(
-      P.sequences, slot, S.units,
+      P.sequences, slot, S.find,
       [&](int d, bool live) {
         Sequence r = {};
         if (live) {
-          r.length = P.lengths[d];
+          r.length = r.weight = P.lengths[d];
           r.prefix = P.prefix ? P.prefix[d] : 0;
           r.rows = document_rows(P.bounds, d, P.rows);
           r.units = ((r.rows.y - r.rows.x) * P.group + kColumns - 1) / kColumns;

@@ -66,7 +66,7 @@ struct __align__(1024) Shared {
   float top[2][kTile], sum[2][kTile];
   float factor[kTile];  // of a row's f16 form
   Unit unit;
-  int units[kThreads / 32];
+  FindScratch<kThreads> find;
   uint32_t tmem_base;
   uint32_t abort;
   uint32_t qk_issued;
@@ -77,14 +77,14 @@ static_assert(sizeof(Shared) + 1024 <= 227 * 1024, "shared memory of an SM");
 __device__ __forceinline__ void find_own_unit(const CacheParams& P, Shared& S, int slot, int piece) {
   struct Sequence {
     int2 rows;
-    int length, prefix, units;
+    int length, prefix, units, weight;
   };
   find_unit<kThreads, true>(
-      P.sequences, slot, S.units,
+      P.sequences, slot, S.find,
       [&](int d, bool live) {
         Sequence r = {};
         if (live) {
-          r.length = P.lengths[d];
+          r.length = r.weight = P.lengths[d];
           r.prefix = P.prefix ? P.prefix[d] : 0;
           r.rows = document_rows(P.bounds, d, P.rows);
           r.units = ((r.rows.y - r.rows.x) * P.group + kTile - 1) / kTile;

@@ -6,6 +6,8 @@
 // outside is touched.
 #pragma once
 
+#include <climits>
+
 #include "common.cuh"
 
 namespace nob200 {
@@ -27,33 +29,68 @@ __device__ __forceinline__ int2 document_rows(const int* bounds, int d, int rows
 }
 
 // Finds the `slot`-th unit of `count` documents with all THREADS threads of a CTA, a document each, so that what is to be known of
-// THREADS documents is one load's latency away: load(d) brings a document's record to its thread and returns its units, and
-// the thread of the document that the unit is in is told (record, document, unit in it) before the barrier.  `totals` is shared
-// memory of THREADS / 32 words.  BACKWARDS: documents, and the units of each, are counted from the last one on - of documents
-// of one length the longest key ranges of a causal mask come first, and the short ones are left for the end of the launch.
-template <int THREADS, bool BACKWARDS, typename Load, typename Found>
-__device__ __forceinline__ void find_unit(int count, int slot, int* totals, const Load& load, const Found& found) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+// THREADS documents is one load's latency away: load(d, live) brings a document's record to its thread, with its `units` and
+// their `weight`, and found(record, document, unit) is called by the thread of the document that the unit is in, before the last
+// barrier.
+// LONGEST_FIRST: up to THREADS documents are taken by falling weight (the longest key ranges), and a document's units from its
+// last one backwards (under a causal mask the longest again), so that short ones are left for the end of a launch; else, and
+// among more documents, they come in order.
+template <int THREADS>
+struct FindScratch {
+  int totals[THREADS / 32];
+  __align__(16) int weight[THREADS];
+  int order[THREADS], units[THREADS], hit[2];
+};
+template <int THREADS, bool LONGEST_FIRST, typename Load, typename Found>
+__device__ __forceinline__ void find_unit(int count, int slot, FindScratch<THREADS>& S, const Load& load, const Found& found) {
+  const int thread = static_cast<int>(threadIdx.x), warp = thread >> 5, lane = thread & 31;
+  const bool sorted = LONGEST_FIRST && count > 1 && count <= THREADS;
   for (int base = 0; base < count; base += THREADS) {
-    const int at = base + static_cast<int>(threadIdx.x), d = BACKWARDS ? count - 1 - at : at;
-    const auto record = load(d, at < count);
-    const int units = record.units;
+    const int d = base + thread;
+    const auto record = load(d, d < count);
+    int units = record.units, document = d;
+    if (sorted) {
+      S.weight[thread] = d < count ? record.weight : INT_MIN;
+      __syncthreads();
+      if (d < count) {
+        int rank = 0;
+        for (int e = 0; e < count; e += 4) {  // what lies behind the last document weighs less than any
+          const int4 four = *reinterpret_cast<const int4*>(&S.weight[e]);
+          const int w[4] = {four.x, four.y, four.z, four.w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) rank += w[i] > record.weight || (w[i] == record.weight && e + i < d);
+        }
+        S.order[rank] = d, S.units[rank] = units;
+      }
+      __syncthreads();
+      units = d < count ? S.units[thread] : 0, document = d < count ? S.order[thread] : 0;
+    }
     int through = units;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int other = __shfl_up_sync(0xffffffffu, through, o);
       if (lane >= o) through += other;
     }
-    if (lane == 31) totals[warp] = through;
+    if (lane == 31) S.totals[warp] = through;
     __syncthreads();
     int total = 0;
 #pragma unroll
     for (int w = 0; w < THREADS / 32; ++w) {
       if (w == warp) through += total;
-      total += totals[w];
+      total += S.totals[w];
     }
-    if (slot < through && slot >= through - units) found(record, d, BACKWARDS ? through - 1 - slot : slot - (through - units));
+    if (slot < through && slot >= through - units) {
+      const int index = LONGEST_FIRST ? through - 1 - slot : slot - (through - units);
+      if (sorted)
+        S.hit[0] = document, S.hit[1] = index;
+      else
+        found(record, d, index);
+    }
     __syncthreads();
+    if (sorted && slot < total) {
+      if (thread == S.hit[0]) found(record, d, S.hit[1]);
+      __syncthreads();
+    }
     if (slot < total) return;
     slot -= total;
   }

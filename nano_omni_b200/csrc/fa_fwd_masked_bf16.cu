@@ -61,7 +61,7 @@ struct __align__(1024) Shared {
   uint64_t v_clean[2];  // the V tile in stage 1 / 3 has been looked through
   uint32_t bad[2][4];   // and these of its rows were not finite
   Unit unit;
-  int units[kThreads / 32];
+  FindScratch<kThreads> find;
   __align__(16) uint8_t staging[8][32 * 64];  // of the softmax warps: 64 bytes of each of their rows
   uint32_t tmem_base;
   uint32_t abort;
@@ -87,10 +87,10 @@ struct MaskedParams {
 __device__ __forceinline__ void find_own_unit(const MaskedParams& P, Shared& S, int slot, int piece) {
   struct Document {
     int2 rows, keys;
-    int prefix, units;
+    int prefix, units, weight;
   };
   find_unit<kThreads, true>(
-      P.documents, slot, S.units,
+      P.documents, slot, S.find,
       [&](int d, bool live) {
         Document r = {};
         if (live) {
@@ -98,6 +98,7 @@ __device__ __forceinline__ void find_own_unit(const MaskedParams& P, Shared& S, 
           r.prefix = P.prefix ? P.prefix[d] : 0;
           r.rows = document_rows(P.bounds, d, P.rows);
           r.units = (r.rows.y - r.rows.x + P.unit_rows - 1) / P.unit_rows;
+          r.weight = r.keys.y - r.keys.x;
         }
         return r;
       },

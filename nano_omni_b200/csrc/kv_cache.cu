@@ -77,11 +77,11 @@ __device__ __forceinline__ int code_at(uint32_t word, int i) { return static_cas
 __global__ void __launch_bounds__(kAppendThreads)
 cache_append_kernel(const AppendParams P) {
   struct Sequence {
-    int first, before, end, units;  // first new row; tokens held before; with the new ones
+    int first, before, end, units, weight;  // first new row; tokens held before; with the new ones
   };
   __shared__ Sequence own;
   __shared__ int own_index[2];  // sequence, which of the blocks that it touches
-  __shared__ int totals[kAppendThreads / 32];
+  __shared__ FindScratch<kAppendThreads> scratch;
   __shared__ float most[2][kAppendThreads / 32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int slot = static_cast<int>(blockIdx.x) % P.slots, which = static_cast<int>(blockIdx.x) / P.slots;
@@ -91,7 +91,7 @@ cache_append_kernel(const AppendParams P) {
   pdl_wait();
   pdl_release();
   find_unit<kAppendThreads, false>(
-      P.sequences, slot, totals,
+      P.sequences, slot, scratch,
       [&](int d, bool live) {
         Sequence r = {};
         if (live) {

@@ -215,9 +215,10 @@ def plan_cache_units(num_rows: int, sequences: int, cached_tokens: int, heads: i
     Up to sixteen rows of a sequence and key head are columns of the small kernel, eight where they do; more take the kernel
     of 128-row tiles (24 rows against 30000 keys x 8 key heads 34 us, 39 in two groups of columns; 16 rows against 8192 x 4
     x 16 sequences 62, 41 as columns).  Shares: as many as have room at once - four CTAs of eight columns an SM, two of sixteen,
-    one of tiles - and where less than two have, eight rounds' worth, with 128 or 512 keys each at least.  Clusters where
-    eight shares do: 1021 keys x 14 heads 9.2 us, 11.5 with the second launch; not in rounds, as a cluster's CTAs wait for
-    room together (64 contexts x 8 key heads 181 us, 200 in clusters of eight)."""
+    one of tiles - with 128 keys each at least; where less than two have, two and a half rounds' worth with 512 keys each
+    (ragged contexts x 8 key heads: 64 of up to 16384 keys 160 us in 3 shares, 166 in 2, 169 in 4, 276 undivided; 96 of 8192
+    111 in 2, 120 in 3, 142 undivided; 64 of 2048 35 in 2, 41 in 3, 44 undivided).  Clusters where eight shares do: 1021 keys
+    x 14 heads 8.9 us, 11.3 with the second launch; not in rounds, as a cluster's CTAs wait for room together."""
     each = -(-num_rows * (heads // kv_heads) // sequences)
     columns = 8 if each <= 8 else 16 if each <= 16 else 128
     units = -(-each // columns) * sequences * kv_heads
@@ -238,7 +239,7 @@ def plan_cache_units(num_rows: int, sequences: int, cached_tokens: int, heads: i
         shares = max(1, min(64, tokens // 128, room // units))
         clusters = 1 < shares < 12 and units * min(shares, MAX_CLUSTER) <= room
         return CacheUnits(columns, min(shares, MAX_CLUSTER) if clusters else shares, clusters)
-    return CacheUnits(columns, max(1, min(64, tokens // 512, -(-8 * room // units))), False)
+    return CacheUnits(columns, max(1, min(64, tokens // 512, (5 * room + units) // (2 * units))), False)
 
 
 class CacheAttentionConfig(Config):

@@ -374,3 +374,136 @@ def test_append_then_attend_then_read():
             # read back, K and V are rounded to bf16: a score by HALF of sum |q k| / sqrt(128), a value by HALF of itself
             near = HALF * (q[rows].double().abs().sum(-1).amax() * cache.rows(0, s).abs().amax() * 128**-0.5)
             assert ((again[rows].double() - want).abs() <= (2 * near + 3 * HALF) * size + HALF * want.abs()).all()
+
+
+def run_attention_kernel(cache, q, bounds, columns, splits, causal=True, prefix=None, cap=0.0, slopes=None):
+    """The kernel at a chosen division of the work, whatever the operator would choose."""
+    from nano_omni_b200.core import DType
+    from nano_omni_b200.kernels.cache import CacheAttentionArguments, CacheAttentionConfig, CacheAttentionKernel
+    from nano_omni_b200.kernels.masked import share_workspace_bytes
+    from tests.gpu_util import desc, run
+
+    c, out, b = cache.desc(), torch.full_like(q, float("nan")), ints(bounds)
+    need = share_workspace_bytes(len(q), q.shape[1], splits)
+    workspace = desc(torch.empty(need, dtype=torch.uint8, device="cuda"), DType.U8) if need else None
+    p = ints(prefix) if prefix else None
+    arguments = CacheAttentionArguments(
+        desc(q), c.key, c.value, c.key_scales, c.value_scales, c.table, c.lengths, desc(b), None if p is None else desc(p),
+        None if slopes is None else desc(slopes), desc(out), 0, causal, cap=cap, workspace=workspace,
+    )  # fmt: skip
+    run(CacheAttentionKernel(arguments, CacheAttentionConfig(columns=columns, kv_splits=splits)))
+    return out
+
+
+def check(cache, out, q, bounds, extra=0.0, prefix=None, **options):
+    """As in ``compare``; key shares are joined in fp32 and rounded once."""
+    from tests.attention64 import attend
+
+    for s in range(len(bounds) - 1):
+        rows = slice(bounds[s], bounds[s + 1])
+        if rows.start == rows.stop:
+            continue
+        k, v = cache.rows(0, s), cache.rows(1, s)
+        want, size = attend(q[rows], k, v, prefix=prefix[s] if prefix else 0, **options)
+        allowed = HALF * (0.3 * size + want.abs()) + 2 * extra * size + len(k) * 2.0**-25 * (v.abs().amax() if len(v) else 0) + 1e-30
+        assert ((out[rows].double() - want).abs() <= allowed).all(), f"sequence {s}"
+    assert out[bounds[-1] :].isnan().all()
+
+
+@pytest.mark.parametrize("columns,sequences", [(8, 128), (8, 129), (16, 300), (128, 640), (128, 641)])
+def test_many_sequences(columns, sequences):
+    """As many sequences as a CTA orders by their lengths, and more, which it takes as they come."""
+    g = torch.Generator().manual_seed(sequences)
+    new = torch.randint(0, 3, (sequences,), generator=g)
+    new[sequences // 2], new[-1] = 40, 0
+    held = new + torch.randint(0, 90, (sequences,), generator=g)
+    held[1], held[2] = 700, 0
+    cache = Cache(held.tolist(), 2, seed=40)
+    q, bounds = random_rows(41, int(new.sum()) + 2, 4), ends(new.tolist())
+    for splits in (1, 3):
+        check(cache, run_attention_kernel(cache, q, bounds, columns, splits), q, bounds, causal=True)
+
+
+@pytest.mark.parametrize("splits", [1, 2, 5])
+@pytest.mark.parametrize("cap,prefix", [(0.0, None), (20.0, None), (0.0, [650, 0, 3]), (20.0, [650, 0, 3])])
+def test_bias_and_cap_over_shares_of_tiles(splits, cap, prefix):
+    """Several units of rows to a sequence, nearest tiles first, shares that a unit's rows do not reach."""
+    cache = Cache([900, 290, 40], 2, seed=42)
+    q, bounds = random_rows(43, 401, 4), [0, 120, 390, 400]
+    slopes = torch.tensor([0.3, 0.01, 0.0, -0.002], device="cuda")
+    options = {"causal": True, "prefix": prefix, "cap": cap, "slopes": slopes}
+    for columns in (8, 128):
+        check(cache, run_attention_kernel(cache, q, bounds, columns, splits, **options), q, bounds, extra=1e-4, **options)
+
+
+@pytest.mark.parametrize("new", [1, 30])
+def test_head_slice_and_scale(new):
+    from tests.gpu_util import desc
+
+    cache = Cache([400, 90], 1, seed=44)
+    q, bounds = random_rows(45, 2 * new, 3), [0, new, 2 * new]
+    out = torch.full((2 * new, 8, 128), float("nan"), dtype=torch.bfloat16, device="cuda")
+    run_op(attention_op(cache, q, ints(bounds), total_heads=8, head_offset=4, scale=0.05).to(desc(out)))
+    assert out[:, :4].isnan().all() and out[:, 7:].isnan().all()
+    check(cache, out[:, 4:7], q, bounds, causal=True, scale=0.05)
+
+
+@pytest.mark.parametrize("sequences", [256, 257, 600])
+def test_append_and_read_of_many_sequences(sequences):
+    from nano_omni_b200 import ops
+    from tests.attention64 import append
+    from tests.gpu_util import desc
+
+    g = torch.Generator().manual_seed(sequences)
+    new = torch.randint(0, 3, (sequences,), generator=g)
+    new[5] = 100
+    before = torch.randint(0, 70, (sequences,), generator=g)
+    cache = Cache((before + new).tolist(), 1, seed=46)
+    total, bounds = int(new.sum()), ends(new.tolist())
+    k, v = random_rows(47, total, 1), random_rows(48, total, 1)
+    want = [[x.clone() for x in part] for part in (cache.codes, cache.scales)]
+    for s in range(sequences):
+        for which, x in enumerate((k, v)):
+            append(want[0][which], want[1][which], x[bounds[s] : bounds[s + 1]].float(), cache.table[s], int(before[s]))
+    run_op(append_op(cache, k, v, ints(bounds)))
+    for which in range(2):
+        assert torch.equal(cache.scales[which], want[1][which]) and torch.equal(cache.codes[which], want[0][which])
+    held = int((before + new).sum())
+    out = [torch.full((held, 128), float("nan"), dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    found = torch.full((sequences + 1,), -1, dtype=torch.int32, device="cuda")
+    run_op(ops.CacheRead(cache.desc(), held).to(desc(out[0]), desc(out[1]), desc(found)))
+    assert found.tolist() == ends((before + new).tolist())
+    for which in range(2):
+        rows = torch.cat([cache.rows(which, s) for s in range(sequences)]).view(held, 128)
+        assert torch.equal(out[which], rows.float().bfloat16())
+
+
+@pytest.mark.parametrize("new", [1, 20])
+def test_a_cache_past_32_bits(new):
+    """Blocks whose codes lie further than 2^32 bytes behind the first; what lies between is never touched."""
+    from nano_omni_b200 import ops
+    from tests.attention64 import append
+    from tests.gpu_util import desc
+
+    cache, blocks = Cache([200], 8, seed=49), 66000  # x 8 heads x 8192 bytes = 4.3e9
+    used = cache.table[0].long()
+    far = torch.arange(blocks - len(used), blocks, device="cuda")
+    for part, shape, kind in ((cache.codes, (blocks, 8, 64, 128), torch.int8), (cache.scales, (blocks, 8), torch.float32)):
+        for which in range(2):
+            whole = torch.empty(shape, dtype=kind, device="cuda")
+            whole[far] = part[which][used]
+            part[which] = whole
+    cache.table[0] = far.int()
+    k, v, q = random_rows(50, new, 8), random_rows(51, new, 8), random_rows(52, new, 16)
+    want = [[part[which][far].clone() for which in range(2)] for part in (cache.codes, cache.scales)]
+    local = torch.arange(len(far), device="cuda")
+    for which, x in enumerate((k, v)):
+        append(want[0][which], want[1][which], x.float(), local, 200 - new)
+    run_op(append_op(cache, k, v, ints([0, new])))
+    for which in range(2):
+        assert torch.equal(cache.codes[which][far], want[0][which]) and torch.equal(cache.scales[which][far], want[1][which])
+    compare(cache, q, [0, new])
+    out = [torch.empty(200, 1024, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    run_op(ops.CacheRead(cache.desc(), 200).to(desc(out[0]), desc(out[1]), desc(ints([0, 0]))))
+    for which in range(2):
+        assert torch.equal(out[which], cache.rows(which, 0).view(200, 1024).float().bfloat16())

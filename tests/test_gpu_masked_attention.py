@@ -243,3 +243,15 @@ def test_runs_again_with_other_bounds_streams_and_graphs():
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(out, second)
+
+
+@pytest.mark.parametrize("documents", [2, 31, 384, 385, 900])  # a CTA orders up to 384 documents by their keys, more it does not
+@pytest.mark.parametrize("causal", [False, True])
+def test_many_documents(documents, causal):
+    g = torch.Generator().manual_seed(documents)
+    queries = torch.randint(0, 4, (documents,), generator=g)
+    queries[documents // 2], queries[-1] = 300, 140
+    keys = queries + torch.randint(0, 30, (documents,), generator=g)
+    keys[0], keys[1] = 500, 0
+    q, k, v = rows(34, int(queries.sum()) + 1, 2), rows(35, int(keys.sum()), 1), rows(36, int(keys.sum()), 1)
+    compare(q, k, v, ends(queries.tolist()), ends(keys.tolist()), causal=causal)
