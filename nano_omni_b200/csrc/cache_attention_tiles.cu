@@ -1,25 +1,33 @@
 // Attention over the 8-bit cache of kv_cache.cu for many rows per sequence and key head: a chunk of new tokens, or a few drafted
 // ones whose query heads share a key head.  head_dim 128, sm_100a; the definition is cache_attention.cu's.
 //
-// A unit is 128 rows - (new token, head of the group) pairs of a sequence and key head - against 128 keys, two blocks, at a
+// A unit is up to 128 rows - (new token, head of the group) pairs of a sequence and key head - against 128 keys, two blocks, at a
 // time.  The scores and values are tcgen05 products of f16 operands, which hold an 8-bit code exactly (and take five instructions
 // for four codes, bf16 eight); queries are scaled by a power of two to a row maximum in [1, 2) (exact down to 2^-24 of it).  The
 // scales of K multiply the scores as they leave TMEM, those of V the probabilities before these are rounded to f16, so
-// nothing of K and V is rounded.  (Sixteen columns at a time by mma.sync widen every code once per sixteen rows: 1200 warp instructions per 32 keys,
-// 28 rows against 4000 keys x 8 heads x 16 sequences 102 us.)
+// nothing of K and V is rounded.  (Sixteen columns at a time by mma.sync widen every code once per sixteen rows: 1200 warp
+// instructions per 32 keys, 28 rows against 4000 keys x 8 heads x 16 sequences 102 us, here 60.)
 //   warps 16, 19  TMA producers: the blocks of K and of V as they are, 8 bits, into a ring of five blocks each (one producer for both,
 //                 whose K waited for V's places, held the kernel at 1.8 us a tile)
 //   warps 8-11    widen the blocks of K to f16 in the 128-byte-swizzled layout of the MMAs, warps 12-15 those of V, into a ring of
 //                 four 32 KiB tiles; first of all warps 12-15 bring the queries, a row per thread, into TMEM
 //   warps 17, 18  issue the score and the value MMAs
 //   warps 0-3     softmax of the even blocks, a thread per row; warps 4-7 of the odd ones.  Each half has a running maximum, sum
-//                 and accumulator of its own, so that they need not meet before the end, where they join through shared
-//                 memory and put out half of the channels each.  (One warp per 32 rows for both halves had its scheduler to
-//                 itself and waited for its own instructions: 3500 cycles a tile, so .... )
+//                 and accumulator of its own, so that they need not meet before the end, where they join through shared memory.
+//                 The two warps of a scheduler take turns at the exponentials, whose unit one of them keeps busy (1560 rows
+//                 against 31560 keys x 14 heads 511 us, 527 at once).
+// Up to 64 (32) rows stand twice (four times) in the 128 of the MMAs, and each copy's warps take their half (quarter) of the keys of a
+// block; the probabilities of the others' are zero, and the copies join like the halves.  A warp reaches only its own 32 lanes of
+// TMEM, so without copies one scheduler of four did all of the softmax (60 drafted tokens of 16 sequences x 56 heads 78 us, 60).
+// What bounds it: a softmax warp's chain of waits, loads, maximum, exponentials (512 cycles of the MUFU a tile for each of two warps)
+// and store, 2700 cycles a tile of 128 full rows; the widening (1300) and the MMAs (1024) run beside it and with half of the
+// exponentials left out the time falls by 13 %, without the widening not at all.
 // TMEM columns: S 0-127, P 128-191 (f16, two keys per column), O of the even blocks 192-319, of the odd ones 320-447,
 // Q 448-511 (f16, two channels per column).
 #include <cuda.h>
 #include <cuda_fp16.h>
+
+#include <type_traits>
 
 #include "cache_attention.cuh"
 #include "common.cuh"
@@ -61,8 +69,10 @@ struct __align__(1024) Shared {
   uint64_t raw_full[2][kRawStages], raw_empty[2][kRawStages];
   uint64_t kv_full[kStages], kv_empty[kStages];
   uint64_t s_full, s_taken, p_full[2], pv_done[2];
+  uint64_t values_done;  // after the last value MMA
   uint64_t scales_full[kScaleSlots];  // a block's scales are there
-  uint64_t joined[8];               // a softmax warp has left what its partner needs
+  uint64_t turn[2][4];                // a half's warp of a quarter of the rows is through with a tile's exponentials
+  uint64_t joined;                    // the softmax warps have left their rows
   float top[2][kTile], sum[2][kTile];
   float factor[kTile];  // of a row's f16 form
   Unit unit;
@@ -156,11 +166,13 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
     }
     mbar_init(&S.s_full, 1);
     mbar_init(&S.s_taken, 8);
+    mbar_init(&S.values_done, 1);
+    mbar_init(&S.joined, 8);
+    for (int q = 0; q < 8; ++q) mbar_init(&S.turn[q >> 2][q & 3], 1);
     for (int h = 0; h < 2; ++h) {
       mbar_init(&S.p_full[h], 4);
       mbar_init(&S.pv_done[h], 1);
     }
-    for (int w = 0; w < 8; ++w) mbar_init(&S.joined[w], 1);
     for (int i = 0; i < kScaleSlots; ++i) mbar_init(&S.scales_full[i], 1);
     S.unit = Unit{};
     S.abort = 0;
@@ -183,6 +195,8 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
   pdl_release();
 
   const int items = S.unit.items;  // 0: no unit
+  // Few rows stand four or two times in the MMAs' 128, and the warps of either copy take their own part of the keys.
+  const int unit_rows = items <= 32 ? 32 : items <= 64 ? 64 : kTile;
   const int kv_begin = S.unit.kv_begin, n_kv = S.unit.kv_end - kv_begin;
   const int* table = P.table + static_cast<size_t>(S.unit.sequence) * P.max_blocks;
   // the order of the key tiles: under a distance bias from the last, and so nearest and largest, one backwards
@@ -198,24 +212,22 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
       const int v = warp == kValueWarp;
       const CUtensorMap* map = v ? &map_v : &map_k;
       if (lane == 0) tma_prefetch_desc(map);
-      // A lane holds the number and scales of one block in 32, those of the next 32 on their way: one after the other they
-      // would take two loads' latency each.
+      // A lane holds the number and scales of one block in 32; those of the next 32 are asked for eight blocks earlier: one after
+      // the other they would take two loads' latency each.
       struct Blocks {
         int number;
-        float key, value_log2;
+        float key, value;
       };
       auto blocks_from = [&](int i) {
-        Blocks r = {-1, 0.f, kNotThere};
+        Blocks r = {-1, 0.f, 0.f};
         if (i + lane < 2 * n_kv) {
           const int at = 2 * (kv_begin + tile_at((i + lane) >> 1)) + ((i + lane) & 1);
           r.number = block_of(P, table, at);
           if (r.number < 0 && at * kBlock < S.unit.sight.keys) atomicOr(status, kBadIndex);
           if (v && r.number >= 0) {
             const size_t place = static_cast<size_t>(r.number) * P.kv_heads + key_head;
-            const float value = P.value_scales[place];
+            r.value = P.value_scales[place];
             r.key = P.key_scales[place];
-            // a summand of the exponent; of a block whose scale is 0 (or less) next to nothing is taken
-            r.value_log2 = log2f(value > 0.f ? value : value != value ? value : 1e-30f);
           }
         }
         return r;
@@ -224,20 +236,25 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
       Blocks some = {}, next = blocks_from(0);
       for (int i = 0; ok && i < 2 * n_kv; ++i) {
         const int st = i % kRawStages;
-        if (i % 32 == 0) some = next, next = blocks_from(i + 32);
+        if (i % 32 == 0) some = next;
         const int block = __shfl_sync(0xffffffffu, some.number, i % 32);
         if (i >= kRawStages) ok = rest(&S.raw_empty[v][st], ((i / kRawStages) - 1) & 1, kWaitTimeoutRing);
         if (!ok) break;
-        if (v) {
-          const float key = __shfl_sync(0xffffffffu, some.key, i % 32), value_log2 = __shfl_sync(0xffffffffu, some.value_log2, i % 32);
-          if (lane == 0) S.scales[i % kScaleSlots] = make_float2(key, value_log2);
-        }
         if (lane == 0) {
           mbar_expect_tx(&S.raw_full[v][st], kRawBytes);
           // a block that is not there: any block, whose scores are masked
           tma_load_3d(S.raw[v][st], map, &S.raw_full[v][st], 0, (max(block, 0) * P.kv_heads + key_head) * kBlock, 0);
-          if (v) mbar_arrive(&S.scales_full[i % kScaleSlots]);
         }
+        if (v) {
+          const float key = __shfl_sync(0xffffffffu, some.key, i % 32), value = __shfl_sync(0xffffffffu, some.value, i % 32);
+          // V's is a summand of the exponent; of a block whose scale is 0 (or less) next to nothing is taken
+          const float value_log2 = block < 0 ? kNotThere : log2f(value > 0.f ? value : value != value ? value : 1e-30f);
+          if (lane == 0) {
+            S.scales[i % kScaleSlots] = make_float2(key, value_log2);
+            mbar_arrive(&S.scales_full[i % kScaleSlots]);
+          }
+        }
+        if (i % 32 == 24) next = blocks_from(i + 8);
         __syncwarp();
       }
     } else if (warp == kMmaWarp) {
@@ -248,7 +265,7 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
       for (int j = 0; ok && j < n_kv; ++j) {
         const int ik = 2 * j, sk = ik % kStages;
         const uint64_t b0 = kv_k_desc + sk * (kTileBytes >> 4);
-        ok = rest(&S.kv_full[sk], (ik / kStages) & 1, kWaitTimeoutLoad) && (j == 0 || spin(&S.s_taken, (j - 1) & 1, kWaitTimeoutSoftmax));
+        ok = rest(&S.kv_full[sk], (ik / kStages) & 1, kWaitTimeoutLoad) && (j == 0 || rest(&S.s_taken, (j - 1) & 1, kWaitTimeoutSoftmax));
         if (!ok) break;
         tc_fence_after();
         if (elect_one()) {
@@ -270,7 +287,7 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
       for (int j = 0; ok && j < n_kv; ++j) {
         const int iv = 2 * j + 1, sv = iv % kStages;
         for (int half = 0; ok && half < 2; ++half) {
-          ok = (half > 0 || rest(&S.kv_full[sv], (iv / kStages) & 1, kWaitTimeoutLoad)) && spin(&S.p_full[half], j & 1, kWaitTimeoutSoftmax) &&
+          ok = (half > 0 || rest(&S.kv_full[sv], (iv / kStages) & 1, kWaitTimeoutLoad)) && rest(&S.p_full[half], j & 1, kWaitTimeoutSoftmax) &&
                warp_wait_counter(&S.qk_issued, min(j + 2, n_kv), abort_flag, status, kWaitTimeoutMma);
           if (!ok) break;
           tc_fence_after();
@@ -282,20 +299,21 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
               umma_ts<0>(tmem + kColO + half * kDim, tmem + kColP + half * 32 + 8 * k, b0 + k * (2048 >> 4), idesc_pv, j > 0 || k > 0);
             tc_commit(&S.pv_done[half]);
             if (half == 1) tc_commit(&S.kv_empty[sv]);
+            if (half == 1 && j == n_kv - 1) tc_commit(&S.values_done);
           }
           __syncwarp();
         }
       }
     }
   } else if (warp >= kWidenWarp) {
-    // ------------------------------------------------- queries, then codes to bf16 tiles
+    // ------------------------------------------------- queries, then codes to f16 tiles
     reg_dealloc<kWidenRegs>();
     const int v = warp >= kWidenWarp + 4, quarter = warp & 3;  // of K or V; which 32 rows of a tile
     if (v && n_kv > 0) {
-      // row `thread` of the unit
-      const int thread = threadIdx.x - 32 * (kWidenWarp + 4);
-      const bool live = thread < items;
-      const int item = S.unit.item0 + (live ? thread : 0), token = item / P.group, head = key_head * P.group + item - token * P.group;
+      // a thread per row of the MMAs
+      const int thread = threadIdx.x - 32 * (kWidenWarp + 4), in_unit = thread & (unit_rows - 1);
+      const bool live = in_unit < items;
+      const int item = S.unit.item0 + (live ? in_unit : 0), token = item / P.group, head = key_head * P.group + item - token * P.group;
       const uint4* src = reinterpret_cast<const uint4*>(P.query + (static_cast<size_t>(S.unit.row0 + token) * P.heads + head) * kDim);
       float top = 0.f;
 #pragma unroll
@@ -325,8 +343,10 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
       __syncwarp();
       if (lane == 0) mbar_arrive(&S.q_full);
     }
-    // a lane's 16 bytes of a row become two pieces of one half; which of the two goes first keeps the eight lanes of a row apart
-    const int piece16 = lane & 7, swap = piece16 >> 2, first = 2 * (piece16 & 3);
+    // A lane's 16 bytes become two pieces of 16; eight lanes take as many rows, whose swizzles keep loads and stores apart.
+    const int row = quarter * 16 + (lane & 7), piece = lane >> 3;  // and row + 8; piece and piece + 4
+    const int from[2] = {row * kDim + ((piece ^ (lane & 7)) << 4), row * kDim + (((piece + 4) ^ (lane & 7)) << 4)};
+    const int to[2] = {row * 128 + (((2 * piece) ^ (lane & 7)) << 4), row * 128 + (((2 * piece + 1) ^ (lane & 7)) << 4)};
     bool ok = true;
     for (int j = 0; ok && j < n_kv; ++j) {  // a tile of K is in ring stage 0 or 2, of V in 1 or 3
       const int st = (2 * j + v) % kStages;
@@ -336,20 +356,18 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         const int i = 2 * j + half, raw = i % kRawStages;
         ok = ok && rest(&S.raw_full[v][raw], (i / kRawStages) & 1, kWaitTimeoutLoad);
         if (!ok) break;
-        const uint8_t* from = S.raw[v][raw] + quarter * 16 * kDim + lane * 16;
-        uint4 x[4];  // rows 4 k + lane / 8 of the warp's 16
+        uint4 x[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) x[k] = *reinterpret_cast<const uint4*>(from + k * 512);
+        for (int k = 0; k < 4; ++k) x[k] = *reinterpret_cast<const uint4*>(S.raw[v][raw] + from[k >> 1] + (k & 1) * 8 * kDim);
         __syncwarp();
         if (lane == 0) mbar_arrive(&S.raw_empty[v][raw]);
-        uint8_t* to = S.kv[st] + swap * kHalfBytes + (half * kBlock + quarter * 16 + (lane >> 3)) * 128;
+        uint8_t* tile = S.kv[st] + half * kBlock * 128;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const uint2 a = widen(x[k].x), b = widen(x[k].y), c = widen(x[k].z), d = widen(x[k].w);
-          const uint4 low = make_uint4(a.x, a.y, b.x, b.y), high = make_uint4(c.x, c.y, d.x, d.y);
-          const int row = 4 * k + (lane >> 3);
-          *reinterpret_cast<uint4*>(to + k * 512 + (((first + swap) ^ (row & 7)) << 4)) = swap ? high : low;
-          *reinterpret_cast<uint4*>(to + k * 512 + (((first + 1 - swap) ^ (row & 7)) << 4)) = swap ? low : high;
+          uint8_t* at = tile + (k >> 1) * kHalfBytes + (k & 1) * 8 * 128;
+          *reinterpret_cast<uint4*>(at + to[0]) = make_uint4(a.x, a.y, b.x, b.y);
+          *reinterpret_cast<uint4*>(at + to[1]) = make_uint4(c.x, c.y, d.x, d.y);
         }
       }
       if (!ok) break;
@@ -360,25 +378,34 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
   } else {
     // ------------------------------------------------- softmax + epilogue warps
     reg_alloc<kSoftmaxRegs>();
-    if (items > 0) {
-      const int half = warp >> 2, in_unit = static_cast<int>(threadIdx.x & 127);
-      const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
-      const uint32_t s_addr = tmem + lane_base + kColS + 64 * half, p_addr = tmem + lane_base + kColP + 32 * half;
+    auto softmax = [&](auto copies_constant) {
+      constexpr int kCopies = decltype(copies_constant)::value, kRows = kTile / kCopies, kKeys = kBlock / kCopies;
+      const int half = warp >> 2, quarter = warp & 3, in_unit = static_cast<int>(threadIdx.x) & (kRows - 1);
+      const int part = quarter / (4 / kCopies) * kKeys;  // the first of this warp's keys in a block
+      const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
+      const uint32_t s_addr = tmem + lane_base + kColS + kBlock * half + part, p_addr = tmem + lane_base + kColP + 32 * half;
       const uint32_t o_addr = tmem + lane_base + kColO + kDim * half;
       const bool live = in_unit < items;
       const int item = S.unit.item0 + (live ? in_unit : 0), token = item / P.group, head = key_head * P.group + item - token * P.group;
-      const int visible = S.unit.sight.visible(token) - kv_begin * kTile - 64 * half;  // keys from this half's first block on
+      const int first_key = kv_begin * kTile + kBlock * half + part;
+      const int visible = S.unit.sight.visible(token) - first_key;
       const int partly = max(0, S.unit.sight.visible(S.unit.item0 / P.group) / kTile - kv_begin);
-      const float slope = BIAS ? P.slopes[head] * 1.4426950408889634f : 0.f;
-      // relative to this half's first key
-      const int position = BIAS ? S.unit.sight.ahead + token - kv_begin * kTile - 64 * half : 0;
+      [[maybe_unused]] const float slope = BIAS ? P.slopes[head] * 1.4426950408889634f : 0.f;
+      [[maybe_unused]] const int position = BIAS ? S.unit.sight.ahead + token - first_key : 0;
       // a warp without live rows only keeps the others' pace: what its rows of P and O hold goes nowhere
-      const bool idle = (warp & 3) * 32 >= items;
+      const bool idle = (quarter * 32 & (kRows - 1)) >= items;
       // The maximum is that of the probabilities times V's scale, which are what is rounded; the sum is relative to it too.
       float m_used = kLowestMaximum, sum = 0.f, row_scale = 0.f;
       bool ok = true;
+      if constexpr (kCopies > 1) {  // the other copies' keys weigh nothing in this one
+        uint32_t none[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) none[i] = 0;
+        if (n_kv > 0) tmem_st32(p_addr, none), tc_wait_st();
+      }
       for (int j = 0; j < n_kv; ++j) {
-        ok = rest(&S.s_full, j & 1, kWaitTimeoutMma);
+        const int block = 2 * j + half;
+        ok = spin(&S.scales_full[block % kScaleSlots], (block / kScaleSlots) & 1, kWaitTimeoutLoad) && rest(&S.s_full, j & 1, kWaitTimeoutMma);
         if (!ok) break;
         tc_fence_after();
         if (idle) {
@@ -387,17 +414,18 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
           if (lane == 0) mbar_arrive(&S.s_taken), mbar_arrive(&S.p_full[half]);
           continue;
         }
-        uint32_t s[64];
+        uint32_t s[kKeys];
+        if constexpr (kKeys == 16) {
+          tmem_ld16(s_addr, s);
+        } else {
 #pragma unroll
-        for (int c = 0; c < 2; ++c) tmem_ld32(s_addr + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&s[32 * c]));
+          for (int c = 0; c < kKeys / 32; ++c) tmem_ld32(s_addr + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&s[32 * c]));
+        }
         tc_wait_ld();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&S.s_taken);
-        if (j == 0) row_scale = *const_cast<const volatile float*>(&S.factor[in_unit]) * P.scale;
-        const int block = 2 * j + half;
-        ok = rest(&S.scales_full[block % kScaleSlots], (block / kScaleSlots) & 1, kWaitTimeoutLoad);
-        if (!ok) break;
+        if (j == 0) row_scale = *const_cast<const volatile float*>(&S.factor[threadIdx.x & 127]) * P.scale;
         const volatile float* kept = &S.scales[block % kScaleSlots].x;
         const float key_scale = kept[0] * row_scale, value_scale = kept[1];
         const bool there = value_scale != kNotThere;
@@ -408,22 +436,23 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         if constexpr (BIAS) {
           const float from = static_cast<float>(position - tile_at(j) * kTile), f = CAP ? 1.f : key_scale * P.to_log2;
 #pragma unroll
-          for (int i = 0; i < 64; ++i) s[i] = __float_as_uint(fmaf(__uint_as_float(s[i]), f, -slope * fabsf(from - static_cast<float>(i))));
+          for (int i = 0; i < kKeys; ++i) s[i] = __float_as_uint(fmaf(__uint_as_float(s[i]), f, -slope * fabsf(from - static_cast<float>(i))));
         }
         if (tile_at(j) >= partly || !there) {
 #pragma unroll
-          for (int i = 0; i < 64; ++i)
+          for (int i = 0; i < kKeys; ++i)
             if (i >= valid || !there) s[i] = 0xff800000u;  // -inf
         }
         float a = __uint_as_float(s[0]), b = __uint_as_float(s[1]);
 #pragma unroll
-        for (int i = 2; i < 62; i += 4) {
+        for (int i = 2; i < kKeys - 2; i += 4) {
           a = max3(a, __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
           b = max3(b, __uint_as_float(s[i + 2]), __uint_as_float(s[i + 3]));
         }
-        const bool sees = there && valid > 0;  // a row that sees nothing of the block takes nothing of it, whatever its scales are
+        const bool sees = there && valid > 0;  // a row that sees nothing of the keys takes nothing of them, whatever their scales are
         const float value_log2 = sees ? value_scale : 0.f;
-        const float mx = sees ? fmaf(max3(a, b, fmaxf(__uint_as_float(s[62]), __uint_as_float(s[63]))), unit, value_log2) : kLowestMaximum;
+        const float mx =
+            sees ? fmaf(max3(a, b, fmaxf(__uint_as_float(s[kKeys - 2]), __uint_as_float(s[kKeys - 1]))), unit, value_log2) : kLowestMaximum;
         if (__any_sync(0xffffffffu, mx > m_used + kRescaleThreshold)) {
           const float m_new = fmaxf(m_used, mx);
           const float alpha = ex2(m_used - m_new);
@@ -436,14 +465,15 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
             tmem_scale_rows(o_addr, alpha);
           }
         }
+        if (kCopies == 1 && j >= 1 - half && !(ok = rest(&S.turn[1 - half][quarter], (j - 1 + half) & 1, kWaitTimeoutSoftmax))) break;
         // Probabilities times V's scale at once: 2^(x + log2 scale - m), rounded to f16 for the value MMAs; the row sum is taken
         // before, and divided by the scale.
         const float offset = value_log2 - m_used, f = sees ? unit : 1.f;
         const uint64_t unit2 = pack2(f, f), offset2 = pack2(offset, offset);
         uint64_t la = 0ull, lb = 0ull;
-        uint32_t p[32];
+        uint32_t p[kKeys / 2];
 #pragma unroll
-        for (int i = 0; i < 64; i += 4) {
+        for (int i = 0; i < kKeys; i += 4) {
           float x0, x1, x2, x3;
           unpack2(fma2(pack2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), unit2, offset2), x0, x1);
           unpack2(fma2(pack2(__uint_as_float(s[i + 2]), __uint_as_float(s[i + 3])), unit2, offset2), x2, x3);
@@ -453,6 +483,7 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
           p[i / 2] = pack_f16(c, d);
           p[i / 2 + 1] = pack_f16(e, g);
         }
+        if (kCopies == 1 && lane == 0) mbar_arrive(&S.turn[half][quarter]);
         float l0, l1, l2, l3;
         unpack2(la, l0, l1);
         unpack2(lb, l2, l3);
@@ -462,101 +493,75 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
           if (!ok) break;
           tc_fence_after();
         }
-        tmem_st32(p_addr, p);
+        if constexpr (kKeys == 64)
+          tmem_st32(p_addr, p);
+        else if constexpr (kKeys == 32)
+          tmem_st16(p_addr + part / 2, p);
+        else
+          tmem_st8(p_addr + part / 2, p);
         tc_wait_st();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&S.p_full[half]);
       }
-      if (ok && n_kv > 0) ok = spin(&S.pv_done[half], (n_kv - 1) & 1, kWaitTimeoutMma);
-      if (ok) {
-        // ---- join of the halves: each leaves the 64 channels that the other puts out in a K tile (whose last reader is done)
+      if (ok && n_kv > 0) ok = spin(&S.values_done, 0, kWaitTimeoutMma);
+      if (!ok) return;
+      // ---- join of the 2 kCopies parts of a row: every warp leaves its rows in the place of the tiles, whose last reader is done,
+      // a row in 32 pieces of four channels, and puts out every eighth row of the unit
+      if (n_kv > 0 && !idle) {
         tc_fence_after();
-        float4* leave = reinterpret_cast<float4*>(S.kv[2 * half]) + in_unit;  // [16 pieces of 4 channels][128 rows]
-        const float4* take = reinterpret_cast<const float4*>(S.kv[2 - 2 * half]) + in_unit;
+        float4* leave = reinterpret_cast<float4*>(S.kv[0]) + (warp * 32 + lane) * 32;
 #pragma unroll 1
-        for (int c = 0; c < 2; ++c) {
+        for (int c = 0; c < 4; ++c) {
           uint32_t o[32];
-          if (n_kv > 0) {
-            tmem_ld32(o_addr + 64 * (1 - half) + 32 * c, o);
-            tc_wait_ld();
-          } else {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = 0;
-          }
+          tmem_ld32(o_addr + 32 * c, o);
+          tc_wait_ld();
 #pragma unroll
           for (int g = 0; g < 8; ++g)
-            leave[(8 * c + g) * kTile] = make_float4(__uint_as_float(o[4 * g]), __uint_as_float(o[4 * g + 1]), __uint_as_float(o[4 * g + 2]),
-                                                     __uint_as_float(o[4 * g + 3]));
+            leave[8 * c + (g ^ (lane & 7))] = make_float4(__uint_as_float(o[4 * g]), __uint_as_float(o[4 * g + 1]),
+                                                          __uint_as_float(o[4 * g + 2]), __uint_as_float(o[4 * g + 3]));
         }
-        S.top[half][in_unit] = m_used, S.sum[half][in_unit] = sum;
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&S.joined[warp]);
-        ok = spin(&S.joined[warp ^ 4], 0, kWaitTimeoutSoftmax);
-        if (ok) {
-          const float other_top = S.top[1 - half][in_unit], other_sum = S.sum[1 - half][in_unit], top = fmaxf(m_used, other_top);
-          const float mine_weight = ex2(m_used - top), other_weight = ex2(other_top - top);
-          const float l = fmaf(sum, mine_weight, other_sum * other_weight);
-          const float inv = l == 0.f ? 0.f : 1.0f / l, mine_inv = mine_weight * inv, other_inv = other_weight * inv;
-          const int row = S.unit.row0 + token;
-          const bool store = NOB_CHECK(!live || (row >= 0 && row < P.rows && head + P.head_offset < P.total_heads), status) && live;
-          const size_t share = static_cast<size_t>(piece) * P.heads * P.rows;  // of divided keys
-          if (P.splits > 1 && store && half == 0) P.lse[share + static_cast<size_t>(head) * P.rows + row] = top + log2f(l);
-          // rows leave through shared memory, 64 bytes of each at a time, so that four lanes write one row's piece
-          const int to = P.splits > 1 ? head * P.rows + row : row * P.total_heads + head + P.head_offset;  // the host checks the range
-          uint8_t* mine = S.raw[0][0] + warp * 2048;  // all blocks have been widened
-          const uint32_t rows_live = __ballot_sync(0xffffffffu, store);
-          uint4 part[4];
-          auto flush = [&](int byte) {  // `part`, the bytes from `byte` on of every lane's row
-            __syncwarp();
+        S.top[half][threadIdx.x & 127] = m_used, S.sum[half][threadIdx.x & 127] = sum;
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&S.joined);
+      if (!spin(&S.joined, 0, kWaitTimeoutSoftmax)) return;
+      const size_t share = static_cast<size_t>(piece) * P.heads * P.rows;  // of divided keys
+#pragma unroll 2
+      for (int r = warp; r < min(items, kRows); r += 8) {
+        float top = kLowestMaximum, l = 0.f;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (n_kv > 0) {
 #pragma unroll
-            for (int g = 0; g < 4; ++g) *reinterpret_cast<uint4*>(mine + lane * 64 + ((g ^ ((lane >> 1) & 3)) << 4)) = part[g];
-            __syncwarp();
+          for (int i = 0; i < 2 * kCopies; ++i) top = fmaxf(top, S.top[i & 1][r + (i >> 1) * kRows]);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int r = 8 * i + (lane >> 2);
-              const size_t at = __shfl_sync(0xffffffffu, to, r);
-              if (!(rows_live >> r & 1)) continue;
-              const uint4 x = *reinterpret_cast<const uint4*>(mine + r * 64 + (((lane & 3) ^ ((r >> 1) & 3)) << 4));
-              char* dst = P.splits > 1 ? reinterpret_cast<char*>(P.partial) + (share + at) * 512 : reinterpret_cast<char*>(P.output) + at * 256;
-              *reinterpret_cast<uint4*>(dst + byte + 16 * (lane & 3)) = x;
-            }
-          };
-#pragma unroll 1
-          for (int c = 0; c < 2; ++c) {
-            uint32_t o[32];
-            if (n_kv > 0) {
-              tmem_ld32(o_addr + 64 * half + 32 * c, o);
-              tc_wait_ld();
-            } else {
-#pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] = 0;
-            }
-#pragma unroll
-            for (int g = 0; g < 8; ++g) {
-              const float4 x = take[(8 * c + g) * kTile];
-              const float other[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                o[4 * g + i] = __float_as_uint(fmaf(__uint_as_float(o[4 * g + i]), mine_inv, other[i] * other_inv));
-            }
-            if (P.splits > 1) {
-#pragma unroll
-              for (int k = 0; k < 2; ++k) {
-#pragma unroll
-                for (int g = 0; g < 4; ++g) part[g] = make_uint4(o[16 * k + 4 * g], o[16 * k + 4 * g + 1], o[16 * k + 4 * g + 2], o[16 * k + 4 * g + 3]);
-                flush(256 * half + 128 * c + 64 * k);
-              }
-            } else {
-              auto two = [&](int i) { return pack_bf16(__uint_as_float(o[i]), __uint_as_float(o[i + 1])); };
-#pragma unroll
-              for (int g = 0; g < 4; ++g) part[g] = make_uint4(two(8 * g), two(8 * g + 2), two(8 * g + 4), two(8 * g + 6));
-              flush(128 * half + 64 * c);
-            }
+          for (int i = 0; i < 2 * kCopies; ++i) {
+            const int from = r + (i >> 1) * kRows;
+            const float weight = ex2(S.top[i & 1][from] - top);
+            const float4 x = (reinterpret_cast<const float4*>(S.kv[0]) + ((i & 1) * kTile + from) * 32)[lane ^ (r & 7)];
+            l = fmaf(S.sum[i & 1][from], weight, l);
+            o.x = fmaf(x.x, weight, o.x), o.y = fmaf(x.y, weight, o.y), o.z = fmaf(x.z, weight, o.z), o.w = fmaf(x.w, weight, o.w);
           }
         }
+        const float inv = l == 0.f ? 0.f : 1.0f / l;
+        const int at = S.unit.item0 + r, of = at / P.group, row = S.unit.row0 + of, own_head = key_head * P.group + at - of * P.group;
+        if (!NOB_CHECK(row >= 0 && row < P.rows && own_head + P.head_offset < P.total_heads, status)) continue;
+        if (P.splits > 1) {
+          const size_t to = share + static_cast<size_t>(own_head) * P.rows + row;
+          reinterpret_cast<float4*>(P.partial + to * kDim)[lane] = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+          if (lane == 0) P.lse[to] = top + log2f(l);
+        } else {
+          const size_t to = static_cast<size_t>(row) * P.total_heads + own_head + P.head_offset;
+          reinterpret_cast<uint2*>(P.output + to * kDim)[lane] = make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
+        }
       }
-    }
+    };
+    if (items > 64)
+      softmax(std::integral_constant<int, 1>());
+    else if (items > 32)
+      softmax(std::integral_constant<int, 2>());
+    else if (items > 0)
+      softmax(std::integral_constant<int, 4>());
   }
 
   if (*abort_flag) {  // gave up: let the copies in flight land before the CTA exits (a microsecond; one millisecond)
@@ -577,7 +582,7 @@ int launch_cache_tiles(const CacheParams& params, const void* key, const void* v
   const uint64_t lines = static_cast<uint64_t>(params.num_blocks) * params.kv_heads * kBlock;
   for (int i = 0; i < 2; ++i)
     if ((rc = make_tensor_map_3d(i ? &mv : &mk, CU_TENSOR_MAP_DATA_TYPE_UINT8, i ? value : key, kDim, lines, 1, kDim, kDim * lines, kDim,
-                                 kBlock, 1, CU_TENSOR_MAP_SWIZZLE_NONE)))
+                                 kBlock, 1, CU_TENSOR_MAP_SWIZZLE_128B)))
       return rc;
   auto kernel = capped ? (params.slopes ? cache_tiles_kernel<true, true> : cache_tiles_kernel<true, false>)
                        : (params.slopes ? cache_tiles_kernel<false, true> : cache_tiles_kernel<false, false>);
