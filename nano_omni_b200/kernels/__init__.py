@@ -3,12 +3,12 @@ counterpart there (masked attention, the 8-bit cache)."""
 
 from __future__ import annotations
 
-from functools import cache
+import functools
 
 from nano_omni_b200.core import Kernel
 
 
-@cache
+@functools.cache
 def classes() -> dict[str, type[Kernel]]:
     from nano_omni_b200.kernels import (
         cache,

@@ -201,3 +201,10 @@ def test_workspace_sizes_are_the_planned_ones(lib):
         fn.restype = ctypes.c_size_t
         for rows, heads, splits in ((1, 1, 1), (1, 14, 21), (32768, 28, 8), (100, 8, 9), (4096, 56, 64)):
             assert fn(rows, heads, splits) == share_workspace_bytes(rows, heads, splits)
+
+
+def test_the_kernels_are_in_the_registry():
+    from nano_omni_b200 import kernels
+
+    names = {"masked_bf16_attention_d128", "int8_cache_append_d128", "int8_cache_read_d128", "int8_cache_attention_d128"}
+    assert names <= set(kernels.classes())
