@@ -402,10 +402,10 @@ int nob200_int8_cache_read_d128(int capacity, int sequences, int max_blocks, int
  * Attention of the queries bounds[s] .. bounds[s + 1] over the cached tokens of sequence s, with positions, masks, cap and
  * slopes as nob200_masked_bf16_attention_d128 (a sequence is a document, lengths[s] its keys).  query bf16
  * [num_rows, heads, 128], key / value codes int8 [num_blocks, kv_heads, 64, 128], output bf16 [num_rows, total_heads, 128]
- * at head_offset.  For a few rows per sequence and key head (new tokens x query heads of a key head): `columns`, 8 or 16, of
- * them are a CTA's.  kv_splits > 1 divides each sequence's keys over so many CTAs, whose
- * fp32 results a second kernel joins (workspace of ..._workspace_bytes()); without workspace up to eight are a cluster that
- * joins them itself.
+ * at head_offset.  Of the rows of a sequence and key head (new tokens x query heads of a key head) `columns` are a CTA's: 8 or
+ * 16 for few, 128 for more, which take tcgen05 tiles.  kv_splits > 1 divides each sequence's keys over so many CTAs, whose
+ * fp32 results a second kernel joins (workspace of ..._workspace_bytes()); of 8 and 16 columns up to eight shares without
+ * workspace are a cluster that joins them itself.
  */
 size_t nob200_int8_cache_attention_d128_workspace_bytes(int num_rows, int heads, int kv_splits);
 int nob200_int8_cache_attention_d128(int num_rows, int sequences, int max_blocks, int num_blocks, int head_offset,

@@ -13,7 +13,8 @@
 // A CTA's four warps take steps of 32 keys in turn from its share of the sequence, each with a running maximum, sum and
 // accumulator of its own, joined at the end.  A warp feeds itself: its lane 0 issues TMA loads of K and V (32 x 128 bytes,
 // 128-byte swizzle) into a ring of three, two of which are in flight while one is worked on; sixteen warps per SM make
-// 128 KiB in flight, well over the 45 KiB that latency x bandwidth asks for.
+// 128 KiB in flight, well over the 45 KiB that latency x bandwidth asks for.  One token against 131072 x 14 heads 84-88 us (5.3-5.6
+// TB/s), 64 ragged contexts x 8 key heads 5.5 TB/s, of the 6.55 of a copy; the schedulers issue in 59 % of the cycles.
 //  * scores: A = codes, which f16 holds exactly (byte -> f16 by a permute onto 1024 + (code + 128) and a subtraction); B = the
 //    queries as f16, scaled by a power of two to a row maximum in [1, 2) (exact down to 2^-24 of it).  The channels of an
 //    instruction's k index are chosen so that a lane reads 32 consecutive bytes of a key.
