@@ -364,6 +364,7 @@ int nob200_hadamard128_heads(int tokens, int head_offset, const void* input, voi
  * bounds[d] .. bounds[d + 1] attend to key rows key_bounds[d] .. key_bounds[d + 1]; rows outside all documents are left as
  * they are.  Query i of n stands at position p = i + m - n among its document's m keys.
  *   score = scale * q.k;  cap > 0: cap * tanh(score / cap);  slopes f32 [heads] not NULL: minus slopes[h] * |p - j|
+ *   (without a cap they take a scale of 1e-12 or more)
  *   causal != 0: key j is seen if j <= p or j < prefix[d] (int32 [documents], NULL: 0); else all keys of the document are.
  * A row that sees no key gets zeros.  Keys and values that a row does not see may hold anything (infinities, NaN); where a
  * document's value row is not finite, whole rows that see it under a partial mask become NaN.

@@ -18,7 +18,7 @@
 //    by 1 - 2 / (1 + e^2x) on the MUFU (cap_scores).
 // Bound by the softmax warps like the dense kernel, 3500 cycles per 256 rows x 128 keys of which the MMAs and the MUFU have 2048
 // each, and under long loads by the power cap: 32768 causal rows x 14 heads 3.24-3.52 ms (1.09-1.18 PFLOP/s), 15104 with a distance
-// bias 821-915 us, 9461 rows of nine documents 126 us (0.69), 4096 capped rows of three, 32 heads over 4, 133 us (104 without the
+// bias 761 us, 9461 rows of nine documents 126 us (0.69), 4096 capped rows of three, 32 heads over 4, 133 us (104 without the
 // cap).  Short documents pay a CTA's start and end, about two tiles' time.
 #include <cuda.h>
 
@@ -177,7 +177,7 @@ fa_fwd_masked_bf16_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
   const bool two = unit_rows > kTile;
   // The order of the key tiles: a distance bias makes the nearest ones the largest, so they come first, from the last row's own
   // backwards, then the ones ahead.  (From the first key on, steep slopes raised the maximum with every tile: 15104 causal rows x
-  // 14 heads 1065 us.)
+  // 14 heads 1065 us, so 821.)
   const int nearest = BIAS ? clamped((S.unit.sight.ahead + S.unit.query0 + unit_rows - 1) / kTile - kv_begin, 0, n_kv - 1) : -1;
   auto tile_at = [&](int j) { return j <= nearest ? nearest - j : j; };
   // key tiles from this one on (of this CTA's) are not seen whole by the unit's first row
@@ -370,9 +370,8 @@ fa_fwd_masked_bf16_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
       const uint32_t o_addr = tmem + lane_base + kColO + t * kTile;
       const int query = S.unit.query0 + t * kTile + (warp & 3) * 32 + lane;
       const int visible = S.unit.sight.visible(query) - kv_begin * kTile;  // keys of this CTA's that the row sees
-      // from a raw score to log2 units; capped and biased ones are turned into them at once
-      const float sc = CAP ? 1.f : P.to_log2, unit_log2 = CAP || BIAS ? 1.f : P.to_log2;
-      const float slope = BIAS ? P.slopes[head] * 1.4426950408889634f : 0.f;
+      const float unit_log2 = CAP ? 1.f : P.to_log2;  // from a raw score to log2 units; capped ones are turned into them at once
+      const float slope = !BIAS ? 0.f : CAP ? P.slopes[head] * 1.4426950408889634f : P.slopes[head] / P.scale;  // in units of a score
       const int position = BIAS ? S.unit.sight.ahead + query - kv_begin * kTile : 0;  // relative to this CTA's first key
       float m_used = 0.f;
       uint64_t la = 0ull, lb = 0ull;  // four partial row sums as two fp32 pairs
@@ -389,29 +388,25 @@ fa_fwd_masked_bf16_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
         __syncwarp();
         if (lane == 0) mbar_arrive(&S.s_taken[t]);
         if constexpr (CAP) cap_scores(s, P.scale, P.to_log2);
+        [[maybe_unused]] float row_base = 0.f;
         if constexpr (BIAS) {
           const int key = tile_at(j) * kTile;
           const int first = __shfl_sync(0xffffffffu, position, 0);  // of the warp's rows
           const bool below = key + kTile - 1 <= first, above = key >= first + 31;
           if (below || above) {
-            // all keys on one side of all rows: the distance is linear in the key
-            const float a = below ? slope : -slope;
-            const float base = a * static_cast<float>(key - position);
-            const uint64_t a2 = pack2(a, a), base2 = pack2(base, base), sc2 = pack2(sc, sc);
+            // All keys on one side of all rows: the distance is linear in the key, and the same for all rows but for a summand,
+            // which joins the maximum; the slope is in units of a raw score, so that a key costs one fma with its number as an
+            // immediate (821 us of the 15104 rows above with packed pairs of keys, so 761).
+            const float step = below ? slope : -slope;
+            row_base = step * static_cast<float>(key - position);
 #pragma unroll
-            for (int i = 0; i < 128; i += 2) {
-              float x, y;
-              unpack2(fma2(pack2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), sc2, fma2(pack2(i, i + 1), a2, base2)), x, y);
-              s[i] = __float_as_uint(x), s[i + 1] = __float_as_uint(y);
-            }
+            for (int i = 0; i < 128; ++i) s[i] = __float_as_uint(fmaf(step, static_cast<float>(i), __uint_as_float(s[i])));
           } else {
             const float from = static_cast<float>(position - key);
 #pragma unroll
-            for (int i = 0; i < 128; ++i) {
-              const float distance = fabsf(from - static_cast<float>(i));
-              s[i] = __float_as_uint(fmaf(__uint_as_float(s[i]), sc, -slope * distance));
-            }
+            for (int i = 0; i < 128; ++i) s[i] = __float_as_uint(fmaf(-slope, fabsf(from - static_cast<float>(i)), __uint_as_float(s[i])));
           }
+          row_base *= unit_log2;
         }
         if (tile_at(j) >= partly && __any_sync(0xffffffffu, visible < (tile_at(j) + 1) * kTile)) {
           const int valid = visible - tile_at(j) * kTile;
@@ -430,7 +425,7 @@ fa_fwd_masked_bf16_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
         }
         mx0 = max3(mx0, __uint_as_float(s[124]), __uint_as_float(s[125]));
         mx1 = max3(mx1, __uint_as_float(s[126]), __uint_as_float(s[127]));
-        const float mx = fmaxf(max3(mx0, mx1, mx2), mx3) * unit_log2;
+        const float mx = BIAS ? fmaf(fmaxf(max3(mx0, mx1, mx2), mx3), unit_log2, row_base) : fmaxf(max3(mx0, mx1, mx2), mx3) * unit_log2;
         bool pv_waited = j == 0;  // P_t and O_t are untouched by the tensor core before the first PV
         if (j == 0) {
           m_used = fmaxf(mx, kLowestMaximum);
@@ -462,7 +457,8 @@ fa_fwd_masked_bf16_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
           if (bad) la = ~0ull;  // the row sees one: its sum, and with it the row, is not a number
         }
         const uint64_t scale2 = pack2(unit_log2, unit_log2);
-        const uint64_t neg_m2 = pack2(-m_used, -m_used);
+        const float neg_m = BIAS ? row_base - m_used : -m_used;
+        const uint64_t neg_m2 = pack2(neg_m, neg_m);
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           uint32_t p[32];
@@ -661,6 +657,7 @@ extern "C" int nob200_masked_bf16_attention_d128(int num_rows, int num_key_rows,
   NOB_REQUIRE(reinterpret_cast<uintptr_t>(output) % 16 == 0, "%s: output %p is not 16-byte aligned", name, output);
   NOB_REQUIRE(scale > 0.f && scale <= 1e30f, "%s: scale %g must be positive and finite", name, scale);
   NOB_REQUIRE(cap >= 0.f && cap <= 1e30f, "%s: cap %g must be finite, 0 for none", name, cap);
+  NOB_REQUIRE(!slopes || cap > 0.f || scale >= 1e-12f, "%s: slopes, which are divided by it, need a scale of 1e-12 or more (got %g)", name, scale);
   NOB_REQUIRE(unit_rows == kTile || unit_rows == 2 * kTile, "%s: unit_rows must be 128 or 256 (got %d)", name, unit_rows);
   NOB_REQUIRE(kv_splits >= 1 && kv_splits <= 64, "%s: kv_splits %d outside [1, 64]", name, kv_splits);
   const long long slots = most_units(num_rows, documents, unit_rows);

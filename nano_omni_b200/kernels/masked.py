@@ -154,6 +154,7 @@ class MaskedBf16AttentionKernel(
         documents = a.bounds.shape[0] - 1
         check_masks(a, documents, heads)
         require_tensor(a.key_bounds, DType.I32, (documents + 1,), "key_bounds")
+        assert a.slopes is None or a.cap > 0 or not a.scale < 1e-12, f"slopes need a scale of 1e-12 or more, not {a.scale}"
         return MaskedBf16AttentionWorkload(
             num_rows=num_rows, num_key_rows=num_key_rows, documents=documents, heads=heads, kv_heads=kv_heads,
             total_heads=total_heads, causal=a.causal, use_prefix=a.prefix is not None, use_slopes=a.slopes is not None,

@@ -67,6 +67,14 @@ def test_masked_attention_refuses(options):
         masked(**options).to(at(DType.BF16, 300, 6, 128)).prepare()
 
 
+def test_masked_attention_refuses_slopes_with_next_to_no_scale():
+    slopes, out = at(DType.F32, 4), at(DType.BF16, 300, 6, 128)
+    with pytest.raises(AssertionError):
+        masked(slopes=slopes, scale=1e-13).to(out).prepare()
+    masked(slopes=slopes, scale=1e-13, cap=1.0).to(out).prepare()
+    masked(scale=1e-13).to(out).prepare()
+
+
 @pytest.mark.parametrize("options", [{"cap": -1.0}, {"cap": float("inf")}, {"scale": 0.0}, {"scale": float("nan")}], ids=str)
 def test_masked_attention_refuses_numbers(options):
     with pytest.raises(ValueError):
@@ -153,8 +161,8 @@ def test_c_entries_refuse_before_any_launch(lib):
         assert function(*arguments) == -1 and text in lib.nob200_last_error(), lib.nob200_last_error()
 
     def attention(rows=9, heads=4, kv_heads=2, offset=0, query=p, output=p, scale=0.1, cap=0.0, unit=256, splits=1, workspace=null,
-                  size=z):  # fmt: skip
-        return (rows, 70, 3, offset, query, p, p, p, p, null, null, output, heads, kv_heads, 4, 1, f(scale), f(cap), unit, splits,
+                  size=z, slopes=null):  # fmt: skip
+        return (rows, 70, 3, offset, query, p, p, p, p, null, slopes, output, heads, kv_heads, 4, 1, f(scale), f(cap), unit, splits,
                 workspace, size, null)  # fmt: skip
 
     fn = lib.nob200_masked_bf16_attention_d128
@@ -166,6 +174,7 @@ def test_c_entries_refuse_before_any_launch(lib):
     refused(fn, attention(scale=float("nan")), b"scale")
     refused(fn, attention(cap=-1.0), b"cap")
     refused(fn, attention(unit=192), b"unit_rows")
+    refused(fn, attention(scale=1e-13, slopes=p), b"slopes")
     refused(fn, attention(splits=65), b"kv_splits")
     refused(fn, attention(splits=2), b"workspace required")
     refused(fn, attention(rows=0x7FFFFFFF, heads=4, splits=64, workspace=p, size=ctypes.c_size_t(1 << 62)), b"grid limit")
