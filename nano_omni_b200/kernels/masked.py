@@ -75,14 +75,15 @@ def plan_masked_units(num_rows: int, num_key_rows: int, documents: int, heads: i
     """Units of a launch whose documents are taken to be of one length (the device alone knows their bounds).
 
     Times are counted in key tiles of a 256-row unit (1.9 us); a 128-row unit takes 0.72 of one per key tile, a CTA 2 beside
-    its tiles, the join of shares 2.5 and 0.025 per 256-row share.  Units of one length run in whole rounds of the SMs, others
-    fill the last round to about a half.  One unit of 256 rows stays unless the estimate falls by 2 %: 1024 rows x 14 heads
-    18.9 us in 128-row units, 21.9 in 256; 1560 rows against 31560 keys x 14 heads 364 us in three shares, 510 whole; 8192 rows
-    x 14 heads 475 us whole, 505 in two shares."""
+    its tiles, the join of shares 2.5 and 0.025 per 256-row share.  Units of one length (or within a quarter of it: a chunk
+    behind a long causal context) run in whole rounds of the SMs, others fill the last round to about a half.  One unit of 256
+    rows stays unless the estimate falls by 2 %: 1024 rows x 14 heads 18.9 us in 128-row units, 21.9 in 256; 1560 causal rows
+    against 30000 keys x 14 heads 331 us in three shares, 441 in six, 420 whole; 8192 rows x 14 heads 475 us whole, 505 in two
+    shares."""
     rows, keys = -(-num_rows // documents), -(-num_key_rows // documents)
     seen = keys - min(rows, keys) / 2 if causal else keys
     tiles = max(1.0, seen / 128)
-    alike = documents == 1 and not causal
+    alike = documents == 1 and (not causal or 4 * rows <= keys)
     best, plan = None, MaskedUnits(256, 1)
     for unit_rows, step in ((256, 1.0), (128, 0.72)):
         units = -(-rows // unit_rows) * documents * heads

@@ -217,3 +217,10 @@ def test_the_kernels_are_in_the_registry():
 
     names = {"masked_bf16_attention_d128", "int8_cache_append_d128", "int8_cache_read_d128", "int8_cache_attention_d128"}
     assert names <= set(kernels.classes())
+
+
+def test_a_chunk_behind_a_long_context_runs_in_whole_rounds():
+    from nano_omni_b200.kernels.masked import plan_masked_units
+
+    for causal in (False, True):  # 7 units x 14 heads x 3 shares: 294 of the 296 places of two rounds
+        assert plan_masked_units(1560, 30000, 1, 14, causal) == (256, 3)
