@@ -556,8 +556,6 @@ extern "C" int nob200_int8_cache_attention_d128(int num_rows, int sequences, int
 
   int rc;
   if (columns == 128) {
-    NOB_REQUIRE(static_cast<long long>(num_rows) * total_heads <= 0x7fffffffll, "%s: %d rows x %d heads exceed the limit of 2^31", name,
-                num_rows, total_heads);
     rc = launch_cache_tiles(P, key, value, cap > 0.f, stream);
     if (rc || !need) return rc;
     return launch_join_shares({P.bounds, P.partial, P.lse, P.output, sequences, num_rows, heads, total_heads, head_offset, kv_splits}, stream);

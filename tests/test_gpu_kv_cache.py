@@ -507,3 +507,53 @@ def test_a_cache_past_32_bits(new):
     run_op(ops.CacheRead(cache.desc(), 200).to(desc(out[0]), desc(out[1]), desc(ints([0, 0]))))
     for which in range(2):
         assert torch.equal(out[which], cache.rows(which, 0).view(200, 1024).float().bfloat16())
+
+
+@pytest.mark.parametrize("new", [[1, 3], [40, 25]])
+def test_rows_in_front_of_the_first_sequence(new):
+    from tests.attention64 import append
+
+    cache = Cache([300, 90], 2, seed=53)
+    bounds = [5, 5 + new[0], 5 + sum(new)]
+    k, v, q = (random_rows(seed, bounds[-1] + 3, heads) for seed, heads in ((54, 2), (55, 2), (56, 8)))
+    want = [[x.clone() for x in part] for part in (cache.codes, cache.scales)]
+    for s, n in enumerate(new):
+        for which, x in enumerate((k, v)):
+            append(want[0][which], want[1][which], x[bounds[s] : bounds[s + 1]].float(), cache.table[s], cache.plain[s] - n)
+    run_op(append_op(cache, k, v, ints(bounds)))
+    for which in range(2):
+        assert torch.equal(cache.scales[which], want[1][which]) and torch.equal(cache.codes[which], want[0][which])
+    compare(cache, q, bounds)
+
+
+@pytest.mark.parametrize("new", [1, 20])
+def test_sequences_that_share_blocks(new):
+    """The blocks of a common beginning stand in several rows of the table."""
+    cache = Cache([200, 150, 128], 2, seed=57)
+    cache.table[1, :2] = cache.table[0, :2]
+    cache.table[2, :2] = cache.table[0, :2]
+    compare(cache, random_rows(58, 3 * new, 4), [0, new, 2 * new, 3 * new])
+
+
+def test_attention_on_two_streams_at_once():
+    from nano_omni_b200 import _lib
+    from tests.gpu_util import desc
+
+    cache = Cache([5000, 40, 3000], 2, seed=59)
+    for new in (1, 30):
+        q, bounds = random_rows(60, 3 * new, 8), ints([0, new, 2 * new, 3 * new])
+        want = torch.zeros_like(q)
+        run_op(attention_op(cache, q, bounds).to(desc(want)))
+        runs = []
+        for _ in range(2):
+            out = torch.zeros_like(q)
+            op = attention_op(cache, q, bounds).to(desc(out))
+            scratch = torch.empty(op.prepare()[1] + 256, dtype=torch.uint8, device="cuda")
+            runs.append((op, out, scratch[(-scratch.data_ptr()) % 256 :], torch.cuda.Stream()))
+        torch.cuda.synchronize()
+        for _ in range(5):
+            for op, _, scratch, stream in runs:
+                op.run(scratch, stream.cuda_stream)
+        torch.cuda.synchronize()
+        assert _lib.read_status() == 0
+        assert all(torch.equal(out, want) for _, out, _, _ in runs)

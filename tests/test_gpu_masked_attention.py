@@ -255,3 +255,33 @@ def test_many_documents(documents, causal):
     keys[0], keys[1] = 500, 0
     q, k, v = rows(34, int(queries.sum()) + 1, 2), rows(35, int(keys.sum()), 1), rows(36, int(keys.sum()), 1)
     compare(q, k, v, ends(queries.tolist()), ends(keys.tolist()), causal=causal)
+
+
+@pytest.mark.parametrize("causal", [False, True])
+def test_rows_in_front_of_the_first_document(causal):
+    """Neither Q's nor K's documents need begin at row 0; several key shares write and join only what lies inside."""
+    q, k, v = rows(37, 340, 2), rows(38, 3000, 2), rows(39, 3000, 2)
+    compare(q, k, v, [7, 200, 333], [500, 700, 2990], causal=causal)
+    compare(q, k, v, [339, 340], [11, 2999], causal=causal)
+
+
+def test_two_calls_at_once():
+    """The same operator twice, on two streams with scratch of their own, beside each other."""
+    from nano_omni_b200 import _lib
+    from tests.gpu_util import desc
+
+    q, k, v = rows(40, 600, 4), rows(41, 20000, 2), rows(42, 20000, 2)
+    want = attend(q, k, v, [0, 100, 600], [0, 9000, 20000], causal=True)
+    outs, ops_, streams, scratches = [], [], [torch.cuda.Stream() for _ in range(2)], []
+    for _ in streams:
+        outs.append(torch.zeros_like(q))
+        ops_.append(op_of(q, k, v, [0, 100, 600], [0, 9000, 20000], causal=True).to(desc(outs[-1])))
+        scratch = torch.empty(ops_[-1].prepare()[1] + 256, dtype=torch.uint8, device="cuda")
+        scratches.append(scratch[(-scratch.data_ptr()) % 256 :])
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for op, stream, scratch in zip(ops_, streams, scratches):
+            op.run(scratch, stream.cuda_stream)
+    torch.cuda.synchronize()
+    assert _lib.read_status() == 0
+    assert all(torch.equal(out, want) for out in outs)
