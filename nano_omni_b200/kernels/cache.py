@@ -209,44 +209,64 @@ class CacheUnits(NamedTuple):
     clusters: bool
 
 
+def _tile_shares(units: int, sequences: int, tokens: int, sm_count: int) -> int:
+    """In key tiles of 128: a CTA takes 8 tiles' time beside its own, the join 3.  One sequence's CTAs run in whole rounds; of
+    several, the longest is taken to hold twice the average and to begin first, and the last CTAs to end unevenly (drafted
+    tokens of 16 sequences up to 8192 keys long x 8 key heads: 119 us undivided, 60 in two shares, 67 in three)."""
+    tiles = max(1, tokens // 128)
+
+    def cost(n: int) -> float:
+        several = max(units * (tiles + 8 * n) / sm_count, 2 * tiles / n + 8) + tiles / (2 * n)
+        whole = -(-units * n // sm_count) * (tiles / n + 8)
+        return (whole if sequences == 1 else several) + 3 * (n > 1)
+
+    return min(range(1, max(1, min(64, tiles // 4)) + 1), key=cost)
+
+
+def _column_shares(units: int, sequences: int, tokens: int, room: int) -> tuple[int, bool]:
+    """As many as have room at once, with 128 keys each at least.  Several sequences are taken to be of unequal lengths, the
+    longest of which begin first: up to eight shares 2.25 rounds' worth, more 1.25, with 512 keys each at least (ragged
+    contexts x 8 key heads: 64 of up to 16384 keys 160 us in 3 shares, 166 in 2, 169 in 4, 276 undivided; 24 of 8192 43 in 6,
+    45 in 4, 46 in 8, 58 in 2; 8 of 8192 23.5 in 12, 25.0 in 8, 25.7 in 16).  Clusters where eight shares do: 1021 keys x 14
+    heads 8.9 us, 11.3 with the second launch; of several sequences where 128 keys each are the bound (16 of 1024 keys 12.8
+    us, 13.6), as a cluster's CTAs wait for room and for one another (8 of 8192 30 us in clusters of eight, 25)."""
+    shares = max(1, min(64, tokens // 128, room // units))
+    if sequences > 1:
+        rounds = (9 * room + 2 * units) // (4 * units)
+        rounds = min(tokens // 512, rounds if rounds <= 8 else max(8, 5 * room // (4 * units)))
+        shares = min(64, max(shares, rounds))
+    in_clusters = 1 < shares < 12 and units * min(shares, MAX_CLUSTER) <= room and (sequences == 1 or shares == tokens // 128)
+    return (min(shares, MAX_CLUSTER) if in_clusters else shares), in_clusters
+
+
 def plan_cache_units(num_rows: int, sequences: int, cached_tokens: int, heads: int, kv_heads: int, sm_count: int = 148) -> CacheUnits:
     """Units of a launch whose sequences are taken to be of one length (the device alone knows).
 
-    Up to sixteen rows of a sequence and key head are columns of the small kernel, eight where they do; more take the kernel
-    of 128-row tiles (24 rows against 30000 keys x 8 key heads 34 us, 39 in two groups of columns; 16 rows against 8192 x 4
-    x 16 sequences 37, 34 as columns).  Shares: as many as have room at once - four CTAs of eight columns an SM, two of
-    sixteen - with 128 keys each at least.  Several sequences are taken to be of unequal lengths, the longest of which begin
-    first: up to eight shares 2.25 rounds' worth, more 1.25, with 512 keys each at least (ragged contexts x 8 key heads: 64 of
-    up to 16384 keys 160 us in 3 shares, 166 in 2, 169 in 4, 276 undivided; 24 of 8192 43 in 6, 45 in 4, 46 in 8, 58 in 2; 8
-    of 8192 23.5 in 12, 25.0 in 8, 25.7 in 16).  Clusters where eight shares do: 1021 keys x 14 heads 8.9 us, 11.3 with the
-    second launch; of several sequences where 128 keys each are the bound (16 of 1024 keys 12.8 us, 13.6), as a cluster's
-    CTAs wait for room and for one another (8 of 8192 30 us in clusters of eight, 25)."""
+    Up to sixteen rows of a sequence and key head are columns of the small kernel, eight where they do, of which an SM has room
+    for four CTAs, of sixteen for two (16 rows against 8192 x 4 x 16 sequences 34 us as columns, 37 in tiles).  More are eights
+    of columns or take the kernel of 128-row tiles, whichever is estimated to be faster: a CTA of eight columns 7.6 us and
+    0.018 a key, of tiles 11.5 and 0.0081, a second launch 3 (64 sequences x 14 key heads, 30 rows: 100 keys 53 us in eights, 75
+    in tiles, 276 72 and 84, 1005 154 and 121; 24 rows of one sequence x 8 key heads: 1524 keys 11 and 16, 30000 39 and 34)."""
     each = -(-num_rows * (heads // kv_heads) // sequences)
-    columns = 8 if each <= 8 else 16 if each <= 16 else 128
-    units = max(1, -(-each // columns) * sequences * kv_heads)
     tokens = -(-cached_tokens // sequences)
-    if columns == 128:
-        # in key tiles of 128: a CTA takes 8 tiles' time beside its own, the join 3.  One sequence's CTAs run in whole rounds;
-        # of several, the longest is taken to hold twice the average and to begin first, and the last CTAs to end unevenly
-        # (drafted tokens of 16 sequences up to 8192 keys long x 8 key heads: 119 us undivided, 60 in two shares, 67 in three).
-        tiles = max(1, tokens // 128)
 
-        def cost(n: int) -> float:
-            several = max(units * (tiles + 8 * n) / sm_count, 2 * tiles / n + 8) + tiles / (2 * n)
-            whole = -(-units * n // sm_count) * (tiles / n + 8)
-            return (whole if sequences == 1 else several) + 3 * (n > 1)
+    def in_columns(columns: int) -> CacheUnits:
+        units = max(1, -(-each // columns) * sequences * kv_heads)
+        return CacheUnits(columns, *_column_shares(units, sequences, tokens, 32 // columns * sm_count))
 
-        return CacheUnits(columns, min(range(1, max(1, min(64, tiles // 4)) + 1), key=cost), False)
-    room = (4 if columns == 8 else 2) * sm_count
-    at_once = max(1, min(tokens // 128, room // units))
-    if sequences == 1:
-        shares = min(64, at_once)
-    else:
-        rounds = (9 * room + 2 * units) // (4 * units)
-        rounds = min(tokens // 512, rounds if rounds <= 8 else max(8, 5 * room // (4 * units)))
-        shares = min(64, max(at_once, rounds))
-    in_clusters = 1 < shares < 12 and units * min(shares, MAX_CLUSTER) <= room and (sequences == 1 or shares == tokens // 128)
-    return CacheUnits(columns, min(shares, MAX_CLUSTER) if in_clusters else shares, in_clusters)
+    if each <= 16:
+        return in_columns(8 if each <= 8 else 16)
+    groups = sequences * kv_heads
+    tiles = -(-each // 128) * groups
+    shares = _tile_shares(tiles, sequences, tokens, sm_count)
+    if each <= 64:
+        few = in_columns(8)
+        rounds = max(1.0, -(-each // 8) * groups * few.kv_splits / (4 * sm_count))
+        of_columns = rounds * (7.6 + 0.018 * tokens / few.kv_splits) + (0 if few.kv_splits == 1 or few.clusters else 3)
+        of_tiles = max(1.0, tiles * shares / sm_count) * (11.5 + 0.0081 * tokens / shares) + (0 if shares == 1 else 3)
+        if of_columns < of_tiles:
+            return few
+    return CacheUnits(128, shares, False)
 
 
 class CacheAttentionConfig(Config):

@@ -478,7 +478,7 @@ def test_append_and_read_of_many_sequences(sequences):
         assert torch.equal(out[which], rows.float().bfloat16())
 
 
-@pytest.mark.parametrize("new", [1, 20])
+@pytest.mark.parametrize("new", [1, 20, 70])
 def test_a_cache_past_32_bits(new):
     """Blocks whose codes lie further than 2^32 bytes behind the first; what lies between is never touched."""
     from nano_omni_b200 import ops
@@ -526,7 +526,7 @@ def test_rows_in_front_of_the_first_sequence(new):
     compare(cache, q, bounds)
 
 
-@pytest.mark.parametrize("new", [1, 20])
+@pytest.mark.parametrize("new", [1, 20, 64])
 def test_sequences_that_share_blocks(new):
     """The blocks of a common beginning stand in several rows of the table."""
     cache = Cache([200, 150, 128], 2, seed=57)
