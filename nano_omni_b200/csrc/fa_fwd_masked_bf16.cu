@@ -18,9 +18,11 @@
 //    by 1 - 2 / (1 + e^2x) on the MUFU (cap_scores).
 // Bound by the softmax warps like the dense kernel, 3500 cycles per 256 rows x 128 keys of which the MMAs and the MUFU have 2048
 // each, and under long loads by the power cap: 32768 causal rows x 14 heads 3.24-3.52 ms (1.09-1.18 PFLOP/s), 15104 with a distance
-// bias 761 us, 9461 rows of nine documents 126 us (0.69), 4096 capped rows of three, 32 heads over 4, 133 us (104 without the
-// cap).  Short documents pay a CTA's start and end, about two tiles' time.
+// bias 761 us, 9461 rows of nine documents 119-126 us (0.69), 4096 capped rows of three, 32 heads over 4, 134-138 us (104
+// without the cap).  Short documents pay a CTA's start and end, two to three tiles' time.
 #include <cuda.h>
+
+#include <type_traits>
 
 #include "common.cuh"
 #include "documents.cuh"
@@ -34,16 +36,22 @@ namespace {
 constexpr int kTile = 128;
 constexpr int kHalfBytes = kTile * 64 * 2;
 constexpr int kTileBytes = 2 * kHalfBytes;
-constexpr int kStages = 4;
-constexpr int kThreads = 384;
-constexpr int kProducerWarp = 8, kMmaWarp = 9, kCleanWarp = 11;  // warp 10 issues the value MMAs
-constexpr uint32_t kTmemCols = 512;
 constexpr float kRescaleThreshold = 8.0f;  // log2 units
 constexpr float kLowestMaximum = -1e38f;   // relative to it a key of score -inf weighs 0
-constexpr int kServiceRegs = 88;
-constexpr int kSoftmaxRegs = (384 * 168 - 128 * kServiceRegs) / 256 / 8 * 8;
-static_assert(256 * kSoftmaxRegs + 128 * kServiceRegs <= 384 * 168, "setmaxnreg split exceeds the registers the CTA owns");
-constexpr uint32_t kColS = 0, kColP = 128, kColO = 256;  // TMEM columns; P_t at kColP + 64 t, O_t at kColO + 128 t
+// SMALL: a CTA of one query tile, half of an SM's shared memory, TMEM and registers: two of them overlap one's start and end with
+// the other's tiles (148 documents of 100 rows x 4 heads 44 us, one CTA to an SM 57; 592 of 4 rows 23, 38), which long key ranges
+// pay for with 15 to 25 % (8192 rows x 14 heads 582 us, 491).  Its probabilities take the place of its scores, so a tile's scores wait
+// for the value MMAs of the one before (those of the 64 keys whose columns are free issued at once: 2 % more, not less).
+template <bool SMALL>
+struct Form {
+  static constexpr int kSoftmaxWarps = SMALL ? 4 : 8, kThreads = 32 * (kSoftmaxWarps + 4), kStages = SMALL ? 2 : 4;
+  static constexpr int kProducerWarp = kSoftmaxWarps, kMmaWarp = kSoftmaxWarps + 1, kCleanWarp = kSoftmaxWarps + 3;  // between: value MMAs
+  static constexpr int kLaunchRegs = SMALL ? 128 : 168, kServiceRegs = SMALL ? 56 : 88;
+  static constexpr int kSoftmaxRegs = (kThreads * kLaunchRegs - 128 * kServiceRegs) / (32 * kSoftmaxWarps) / 8 * 8;
+  static_assert(32 * kSoftmaxWarps * kSoftmaxRegs + 128 * kServiceRegs <= kThreads * kLaunchRegs, "setmaxnreg split exceeds the registers the CTA owns");
+  static constexpr uint32_t kTmemCols = SMALL ? 256 : 512;
+  static constexpr uint32_t kColS = 0, kColP = SMALL ? 0 : 128, kColO = SMALL ? 128 : 256;  // P_t at kColP + 64 t, O_t at kColO + 128 t
+};
 
 struct Unit {
   int row0, rows;        // first row, rows of the document from there on (0: no unit)
@@ -52,21 +60,23 @@ struct Unit {
   Sight sight;
 };
 
+template <bool SMALL>
 struct __align__(1024) Shared {
-  uint8_t q[2][kTileBytes];
-  uint8_t kv[kStages][kTileBytes];
+  using F = Form<SMALL>;
+  uint8_t q[SMALL ? 1 : 2][kTileBytes];
+  uint8_t kv[F::kStages][kTileBytes];
   uint64_t q_full;
-  uint64_t kv_full[kStages];
-  uint64_t kv_empty[kStages];
+  uint64_t kv_full[F::kStages];
+  uint64_t kv_empty[F::kStages];
   uint64_t s_full[2];
   uint64_t s_taken[2];
   uint64_t p_full[2][2];
   uint64_t pv_done[2];
-  uint64_t v_clean[2];  // the V tile in stage 1 / 3 has been looked through
+  uint64_t v_clean[2];  // an even / odd V tile has been looked through
   uint32_t bad[2][4];   // and these of its rows were not finite
   Unit unit;
-  FindScratch<kThreads> find;
-  __align__(16) uint8_t staging[8][32 * 64];  // of the softmax warps: 64 bytes of each of their rows
+  FindScratch<F::kThreads> find;
+  __align__(16) uint8_t staging[F::kSoftmaxWarps][32 * 64];  // of the softmax warps: 64 bytes of each of their rows
   uint32_t tmem_base;
   uint32_t abort;
   uint32_t qk_issued;
@@ -88,12 +98,13 @@ struct MaskedParams {
 };
 
 // The unit of this CTA, into shared memory.
-__device__ __forceinline__ void find_own_unit(const MaskedParams& P, Shared& S, int slot, int piece) {
+template <bool SMALL>
+__device__ __forceinline__ void find_own_unit(const MaskedParams& P, Shared<SMALL>& S, int slot, int piece) {
   struct Document {
     int2 rows, keys;
     int prefix, units, weight;
   };
-  find_unit<kThreads, true>(
+  find_unit<Form<SMALL>::kThreads, true>(
       P.documents, slot, S.find,
       [&](int d, bool live) {
         Document r = {};
@@ -124,12 +135,15 @@ __device__ __forceinline__ void find_own_unit(const MaskedParams& P, Shared& S, 
       });
 }
 
-template <bool CAP, bool BIAS>
-__global__ void __launch_bounds__(kThreads, 1)
+template <bool CAP, bool BIAS, bool SMALL>
+__global__ void __launch_bounds__(Form<SMALL>::kThreads, SMALL ? 2 : 1)
 fa_fwd_masked_bf16_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                           const __grid_constant__ CUtensorMap map_v, const MaskedParams P) {
   extern __shared__ uint8_t smem_raw[];
-  Shared& S = *reinterpret_cast<Shared*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  using F = Form<SMALL>;
+  constexpr int kStages = F::kStages, kProducerWarp = F::kProducerWarp, kMmaWarp = F::kMmaWarp, kCleanWarp = F::kCleanWarp;
+  constexpr uint32_t kColS = F::kColS, kColP = F::kColP, kColO = F::kColO;
+  Shared<SMALL>& S = *reinterpret_cast<Shared<SMALL>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -156,7 +170,7 @@ fa_fwd_masked_bf16_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
     mbar_fence_init();
   }
   if (warp == kProducerWarp) {
-    tmem_alloc(&S.tmem_base, kTmemCols);
+    tmem_alloc(&S.tmem_base, F::kTmemCols);
     tmem_relinquish();
   }
   tc_fence_before();
@@ -174,7 +188,7 @@ fa_fwd_masked_bf16_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
   const int unit_rows = min(S.unit.rows, P.unit_rows);  // 0: no unit
   const int n_kv = S.unit.kv_end - S.unit.kv_begin;
   const int kv_begin = S.unit.kv_begin;
-  const bool two = unit_rows > kTile;
+  const bool two = !SMALL && unit_rows > kTile;
   // The order of the key tiles: a distance bias makes the nearest ones the largest, so they come first, from the last row's own
   // backwards, then the ones ahead.  (From the first key on, steep slopes raised the maximum with every tile: 15104 causal rows x
   // 14 heads 1065 us, so 821.)
@@ -183,8 +197,8 @@ fa_fwd_masked_bf16_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
   // key tiles from this one on (of this CTA's) are not seen whole by the unit's first row
   const int partly = max(0, S.unit.sight.visible(S.unit.query0) / kTile - kv_begin);
 
-  if (warp >= 8) {
-    reg_dealloc<kServiceRegs>();
+  if (warp >= F::kSoftmaxWarps) {
+    reg_dealloc<F::kServiceRegs>();
     if (n_kv == 0) {
     } else if (warp == kProducerWarp) {
       // ------------------------------------------------------------ TMA producer
@@ -197,8 +211,8 @@ fa_fwd_masked_bf16_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
         tma_load_3d(S.q[0], &map_q, &S.q_full, 0, head, row0);
         tma_load_3d(S.q[0] + kHalfBytes, &map_q, &S.q_full, 64, head, row0);
         if (two) {
-          tma_load_3d(S.q[1], &map_q, &S.q_full, 0, head, row0 + kTile);
-          tma_load_3d(S.q[1] + kHalfBytes, &map_q, &S.q_full, 64, head, row0 + kTile);
+          tma_load_3d(S.q[SMALL ? 0 : 1], &map_q, &S.q_full, 0, head, row0 + kTile);
+          tma_load_3d(S.q[SMALL ? 0 : 1] + kHalfBytes, &map_q, &S.q_full, 64, head, row0 + kTile);
         }
         const int loads = 2 * n_kv;  // K_j at 2j, V_j at 2j+1
         int issued = 0;
@@ -273,7 +287,7 @@ fa_fwd_masked_bf16_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
       auto rest = [&](uint64_t* bar, uint32_t parity, uint32_t bit) { return warp_rest(bar, parity, abort_flag, status, bit); };
       if (warp == kMmaWarp) {
         const uint64_t desc_k_major = umma_smem_desc(0, 16, 1024, kSwizzle128B);
-        const uint64_t q_desc[2] = {desc_k_major + (smem_u32(S.q[0]) >> 4), desc_k_major + (smem_u32(S.q[1]) >> 4)};
+        const uint64_t q_desc[2] = {desc_k_major + (smem_u32(S.q[0]) >> 4), desc_k_major + (smem_u32(S.q[SMALL ? 0 : 1]) >> 4)};
         const uint64_t kv_k_desc = desc_k_major + (smem_u32(S.kv[0]) >> 4);
         const uint32_t d = tmem + kColS;
         uint32_t issued = 0;
@@ -310,7 +324,7 @@ fa_fwd_masked_bf16_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
         bool ok = rest(&S.q_full, 0, kWaitTimeoutLoad) && qk(0, 0, nullptr, 0);
         for (int j = 0; ok && j < n_kv; ++j) {
           if (two && !(ok = qk(1, j, &S.s_taken[0], j & 1))) break;
-          if (j + 1 < n_kv && !(ok = qk(0, j + 1, &S.s_taken[two ? 1 : 0], j & 1))) break;
+          if (j + 1 < n_kv && !(ok = qk(0, j + 1, SMALL ? &S.pv_done[0] : &S.s_taken[two ? 1 : 0], j & 1))) break;
         }
       } else {
         const uint64_t desc_n_major = umma_smem_desc(0, kHalfBytes, 1024, kSwizzle128B);
@@ -354,13 +368,13 @@ fa_fwd_masked_bf16_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
                  pv_half(1, j, 1, 2 * j + 5);
           }
         } else {
-          for (int j = 0; ok && j < n_kv; ++j) ok = pv_half(0, j, 0, j + 2) && pv_half(0, j, 1, j + 2);
+          for (int j = 0; ok && j < n_kv; ++j) ok = pv_half(0, j, 0, SMALL ? 0 : j + 2) && pv_half(0, j, 1, SMALL ? 0 : j + 2);
         }
       }
     }
   } else {
     // ------------------------------------------------- softmax + epilogue warps
-    reg_alloc<kSoftmaxRegs>();
+    reg_alloc<F::kSoftmaxRegs>();
     auto poll = [&](uint64_t* bar, uint32_t parity, uint32_t bit) { return warp_poll(bar, parity, abort_flag, status, bit); };
     const int t = warp >> 2;
     if (unit_rows > 0 && (t == 0 || two)) {
@@ -561,7 +575,7 @@ fa_fwd_masked_bf16_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
 
   tc_fence_before();
   __syncthreads();
-  if (warp == kProducerWarp) tmem_dealloc(tmem, kTmemCols);
+  if (warp == kProducerWarp) tmem_dealloc(tmem, F::kTmemCols);
 }
 
 // o = sum_z 2^(lse_z - max) o_z / sum_z 2^(lse_z - max).  A thread owns eight channels of a row and every LANES-th share of it, so
@@ -694,13 +708,19 @@ extern "C" int nob200_masked_bf16_attention_d128(int num_rows, int num_key_rows,
   if ((rc = make_tensor_map_3d(&mv, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, value, 128, kv_heads, num_key_rows, 256, key_pitch, 64, 1, kTile)))
     return rc;
 
-  auto kernel = cap > 0.f ? (slopes ? fa_fwd_masked_bf16_kernel<true, true> : fa_fwd_masked_bf16_kernel<true, false>)
-                          : (slopes ? fa_fwd_masked_bf16_kernel<false, true> : fa_fwd_masked_bf16_kernel<false, false>);
-  const size_t smem = sizeof(Shared) + 1024;
-  cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  if (err != cudaSuccess)
-    return fail(kCudaError, "%s: cannot reserve %zu B of shared memory: %s", name, smem, cudaGetErrorString(err));
-  if ((rc = launch_pdl(name, kernel, static_cast<unsigned>(blocks), kThreads, smem, stream, mq, mk, mv, P))) return rc;
+  // CTAs of one query tile share an SM once there are more of them than SMs; alone on it a tile's scores need not wait
+  const bool small = unit_rows == kTile && blocks > 148;
+  auto launch = [&](auto small_form) -> int {
+    constexpr bool kSmall = decltype(small_form)::value;
+    auto kernel = cap > 0.f ? (slopes ? fa_fwd_masked_bf16_kernel<true, true, kSmall> : fa_fwd_masked_bf16_kernel<true, false, kSmall>)
+                            : (slopes ? fa_fwd_masked_bf16_kernel<false, true, kSmall> : fa_fwd_masked_bf16_kernel<false, false, kSmall>);
+    const size_t smem = sizeof(Shared<kSmall>) + 1024;
+    cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (err != cudaSuccess)
+      return fail(kCudaError, "%s: cannot reserve %zu B of shared memory: %s", name, smem, cudaGetErrorString(err));
+    return launch_pdl(name, kernel, static_cast<unsigned>(blocks), Form<kSmall>::kThreads, smem, stream, mq, mk, mv, P);
+  };
+  if ((rc = small ? launch(std::true_type()) : launch(std::false_type()))) return rc;
   if (kv_splits == 1) return kOk;
   return launch_join_shares({P.bounds, P.partial, P.lse, P.output, documents, num_rows, heads, total_heads, head_offset, kv_splits}, stream);
 }

@@ -71,28 +71,36 @@ class MaskedUnits(NamedTuple):
     kv_splits: int
 
 
-def plan_masked_units(num_rows: int, num_key_rows: int, documents: int, heads: int, causal: bool, sm_count: int = 148) -> MaskedUnits:
+def plan_masked_units(
+    num_rows: int, num_key_rows: int, documents: int, heads: int, causal: bool, capped: bool = False, sm_count: int = 148
+) -> MaskedUnits:
     """Units of a launch whose documents are taken to be of one length (the device alone knows their bounds).
 
-    Times are counted in key tiles of a 256-row unit (1.9 us); a 128-row unit takes 0.72 of one per key tile, a CTA 2 beside
-    its tiles, the join of shares 2.5 and 0.025 per 256-row share.  Units of one length (or within a quarter of it: a chunk
-    behind a long causal context) run in whole rounds of the SMs, others fill the last round to about a half.  One unit of 256
-    rows stays unless the estimate falls by 2 %: 1024 rows x 14 heads 18.9 us in 128-row units, 21.9 in 256; 1560 causal rows
-    against 30000 keys x 14 heads 331 us in three shares, 441 in six, 420 whole; 8192 rows x 14 heads 475 us whole, 505 in two
-    shares."""
+    Times are counted in key tiles of a 256-row unit (1.9 us); 128 rows alone on an SM take 0.72 of one per key tile, a CTA 2
+    beside its tiles, capped scores 1.28 times as long; units of 128 rows that share SMs, as they do where there are more
+    than SMs, 0.88 (capped 0.7) and 0.3 (592 documents of 4 rows 23 us, 38 one to an SM; 148 of 100 rows x 4 heads 44, 57; five
+    capped documents, 2100 x 28 63 and 75; nine of 9461 x 14 134, 119 in 256-row units); the join of shares 2.5 and 0.025 per
+    256-row share.  Units of one length (or within a quarter of it: a chunk behind a long causal context) run in whole rounds
+    of the SMs, others fill the last round to about a half.  One unit of 256 rows stays unless the estimate falls by 2 %: 1024
+    rows x 14 heads 18.9 us in 128-row units, 21.9 in 256; 1560 causal rows against 30000 keys x 14 heads 331 us in three
+    shares, 441 in six, 420 whole; 8192 rows x 14 heads 475 us whole, 505 in two shares."""
     rows, keys = -(-num_rows // documents), -(-num_key_rows // documents)
     seen = keys - min(rows, keys) / 2 if causal else keys
     tiles = max(1.0, seen / 128)
     alike = documents == 1 and (not causal or 4 * rows <= keys)
     best, plan = None, MaskedUnits(256, 1)
-    for unit_rows, step in ((256, 1.0), (128, 0.72)):
+    for unit_rows in (256, 128):
         units = -(-rows // unit_rows) * documents * heads
         for splits in range(1, 65):
             if splits > 1 and tiles / splits < 2:
                 break
             pieces = units * splits
             rounds = -(-pieces // sm_count) if alike or pieces <= sm_count else pieces / sm_count + 0.5
-            cost = rounds * (tiles / splits * step + 2)
+            if unit_rows == 128 and pieces > sm_count:
+                step, beside = 0.7 if capped else 0.88, 0.3
+            else:  # a document's 256 rows, or fewer alone; of ragged documents on few SMs some have more
+                step, beside = (1.0 if unit_rows == 256 and (rows > 128 or pieces <= sm_count) else 0.72) * (1.28 if capped else 1.0), 2
+            cost = rounds * (tiles / splits * step + beside)
             if splits > 1:
                 cost += 2.5 + 0.025 * pieces * unit_rows / 256
             if best is None:

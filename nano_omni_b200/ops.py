@@ -846,7 +846,7 @@ class MaskedBf16Attention(Op):
         self.documents = bounds.shape[0] - 1
         self.causal, self.cap, self.scale = causal, cap, DEFAULT_SCALE if scale is None else scale
         self.key_bounds, self.prefix, self.slopes, self.rotation = key_bounds, prefix, slopes, rotation
-        self.units = plan_masked_units(self.rows, self.key_rows, self.documents, self.heads, causal)
+        self.units = plan_masked_units(self.rows, self.key_rows, self.documents, self.heads, causal, cap > 0)
         super().__init__(query, key, value, bounds, outputs=((DType.BF16, (self.rows, total_heads, 128)),))
 
     def kernels(self, scratch: ScratchLayout) -> list[Kernel]:

@@ -285,3 +285,32 @@ def test_two_calls_at_once():
     torch.cuda.synchronize()
     assert _lib.read_status() == 0
     assert all(torch.equal(out, want) for out in outs)
+
+
+@pytest.mark.parametrize("causal,prefix", [(False, None), (True, None), (True, [300, 0, 40, 10])])
+@pytest.mark.parametrize("cap,biased", [(0.0, False), (30.0, False), (0.0, True), (30.0, True)])
+@pytest.mark.parametrize("spoiled", [False, True])
+def test_units_that_share_an_sm(causal, prefix, cap, biased, spoiled):
+    """More units of 128 rows than SMs, from no key tile to eight; what lies behind a document's keys may be anything."""
+    from nano_omni_b200.core import DType
+    from nano_omni_b200.kernels.masked import MaskedBf16AttentionArguments, MaskedBf16AttentionConfig, MaskedBf16AttentionKernel
+    from tests.attention64 import attend_documents
+    from tests.gpu_util import desc, run
+
+    bounds, key_bounds = [0, 3, 600, 601, 1111], [0, 130, 1130, 1130, 1200]
+    q, k, v = rows(43, 1130, 16), rows(44, 1250, 4), rows(45, 1250, 4)
+    slopes = torch.linspace(0.0, 0.4, 16, device="cuda") if biased else None
+    want, size = attend_documents(q, k, v, bounds, key_bounds, causal=causal, prefix=prefix, cap=cap, slopes=slopes)
+    if spoiled:
+        k[1200:], v[1200:], q[1111:] = float("nan"), float("inf"), float("nan")
+    b, kb = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in (bounds, key_bounds))
+    p = torch.tensor(prefix, dtype=torch.int32, device="cuda") if prefix else None
+    out = torch.full_like(q, float("nan"))
+    arguments = MaskedBf16AttentionArguments(
+        desc(q), desc(k), desc(v), desc(b), desc(kb), None if p is None else desc(p), None if slopes is None else desc(slopes),
+        desc(out), 0, causal, 128**-0.5, cap, None,
+    )  # fmt: skip
+    run(MaskedBf16AttentionKernel(arguments, MaskedBf16AttentionConfig(unit_rows=128)))
+    off = (out.double() - want).abs()[:1111]
+    assert (off <= tolerance(want, size, 1e-4)[:1111]).all()
+    assert out[1111:].isnan().all()
