@@ -12,7 +12,7 @@
 // masks add:
 //  * tiles that some row of the unit does not see whole are masked in registers, a compare and a select per score;
 //  * rows of V behind the document's end (another document's, or anything at all) and rows of it that are not finite would
-//    spoil rows that do not see them: 0 x NaN.  Warp 11 walks the V tiles that are not seen whole before their value
+//    spoil rows that do not see them: 0 x NaN.  A warp walks the V tiles that are not seen whole before their value
 //    MMAs start, zeroes such rows and notes the non-finite ones; a query row that does see one of those becomes NaN.
 //  * capped scores: tanh by odd polynomials while all of a warp's rows stay within a third of the cap, or within the cap, else
 //    by 1 - 2 / (1 + e^2x) on the MUFU (cap_scores).
