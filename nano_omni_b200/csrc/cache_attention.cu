@@ -115,6 +115,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int quad = lane >> 2, part = lane & 3;  // of a fragment: row of A, column of B; and which pair of the other index
   volatile uint32_t* abort_flag = &S.abort;
+  if (threadIdx.x >= 32 && threadIdx.x < 34) tma_prefetch_desc(threadIdx.x == 32 ? &map_k : &map_v);
   if (threadIdx.x == 0) {
     for (int w = 0; w < kWarps; ++w)
       for (int s = 0; s < kStages; ++s) mbar_init(&S.full[w][s], 1);

@@ -180,6 +180,8 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
     mbar_fence_init();
   }
   if (warp == kKeyWarp) {
+    if (lane < 2) tma_prefetch_desc(lane ? &map_v : &map_k);
+    __syncwarp();
     tmem_alloc(&S.tmem_base, kTmemCols);
     tmem_relinquish();
   }
@@ -211,7 +213,6 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
       // ------------------------------------------------------------ TMA producers, a block at a time
       const int v = warp == kValueWarp;
       const CUtensorMap* map = v ? &map_v : &map_k;
-      if (lane == 0) tma_prefetch_desc(map);
       // A lane holds the number and scales of one block in 32; those of the next 32 are asked for eight blocks earlier: one after
       // the other they would take two loads' latency each.
       struct Blocks {
