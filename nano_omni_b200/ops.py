@@ -844,6 +844,7 @@ class MaskedBf16Attention(Op):
         assert 0 <= head_offset <= total_heads - self.heads
         self.total_heads, self.head_offset = total_heads, head_offset
         self.documents = bounds.shape[0] - 1
+        assert self.rows > 0 and self.documents > 0, "no rows, or bounds of no document"
         self.causal, self.cap, self.scale = causal, cap, DEFAULT_SCALE if scale is None else scale
         self.key_bounds, self.prefix, self.slopes, self.rotation = key_bounds, prefix, slopes, rotation
         self.units = plan_masked_units(self.rows, self.key_rows, self.documents, self.heads, causal, cap > 0)
@@ -977,7 +978,7 @@ class CacheAttention(Op):
         self.total_heads, self.head_offset = total_heads, head_offset
         self.cache = cache
         self.cached_tokens = cache.capacity if cached_tokens is None else min(cached_tokens, cache.capacity)
-        assert self.cached_tokens > 0
+        assert self.rows > 0 and self.cached_tokens > 0, "no rows, or no cached tokens to plan for"
         self.causal, self.cap, self.scale = causal, cap, DEFAULT_SCALE if scale is None else scale
         self.prefix, self.slopes = prefix, slopes
         super().__init__(query, bounds, outputs=((DType.BF16, (self.rows, total_heads, 128)),))

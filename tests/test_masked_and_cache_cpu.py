@@ -224,3 +224,13 @@ def test_a_chunk_behind_a_long_context_runs_in_whole_rounds():
 
     for causal in (False, True):  # 7 units x 14 heads x 3 shares: 294 of the 296 places of two rounds
         assert plan_masked_units(1560, 30000, 1, 14, causal) == (256, 3)
+
+
+def test_calls_without_rows_documents_or_tokens_are_refused():
+    with pytest.raises(AssertionError):
+        masked(documents=0)
+    with pytest.raises(AssertionError):
+        masked(rows=0, key_rows=0)
+    for rows, tokens in ((0, None), (3, 0)):
+        with pytest.raises(AssertionError):
+            ops.CacheAttention(at(DType.BF16, rows, 512), at(DType.I32, 4), cache(), total_heads=4, cached_tokens=tokens)
