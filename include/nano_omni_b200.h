@@ -382,12 +382,14 @@ int nob200_masked_bf16_attention_d128(int num_rows, int num_key_rows, int docume
  * A cache of keys and values in 8 bits (no counterpart in the reference): blocks of 64 tokens, codes int8
  * [num_blocks, heads, 64, 128], scales f32 [num_blocks, heads] for each of K and V; value = code * scale.
  * table int32 [sequences, max_blocks]: the block of tokens 64 b .. 64 b + 63 of a sequence; lengths int32 [sequences].
- * What a block number, length or bound points to outside these tensors is skipped and bit 6 of the status word set.
+ * What a block number, length or bound points to outside these tensors is skipped and bit 6 of the status word set; read
+ * gives zeros for a block that is not there.
  *
  * append: rows bounds[s] .. bounds[s + 1] (int32 [sequences + 1]) of key / value bf16 [num_rows, heads, 128] become the last
  * tokens of sequence s, whose `lengths` count them already.  A block's scale is max(largest magnitude / 127, 1e-10); a token
  * that raises it has the tokens already in the block rounded again on the new grid.  Two sequences must not append to one
- * block in the same call.
+ * block in the same call.  A sequence whose bounds leave the rows or descend, or whose length counts fewer tokens than they
+ * or more than the table has room for, is left as it is, and bit 6 set.
  * read: the sequences' tokens as bf16 rows [capacity, heads, 128], one sequence behind the other, and where each begins
  * (bounds int32 [sequences + 1]); rows behind the last are left as they are, tokens past the capacity are not written.
  */

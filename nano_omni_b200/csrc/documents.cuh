@@ -28,10 +28,15 @@ __device__ __forceinline__ int2 document_rows(const int* bounds, int d, int rows
   return make_int2(begin, clamped(bounds[d + 1], begin, rows));
 }
 
+// Whether document `d` begins and ends inside [0, rows], in this order.
+__device__ __forceinline__ bool bounds_fit(const int* bounds, int d, int rows) {
+  return bounds[d] >= 0 && bounds[d] <= bounds[d + 1] && bounds[d + 1] <= rows;
+}
+
 // Finds the `slot`-th unit of `count` documents with all THREADS threads of a CTA, a document each, so that what is to be known of
 // THREADS documents is one load's latency away: load(d, live) brings a document's record to its thread, with its `units` and
 // their `weight`, and found(record, document, unit) is called by the thread of the document that the unit is in, before the last
-// barrier.
+// barrier.  load may note documents that cannot be right: between them the CTAs load every one.
 // LONGEST_FIRST: up to THREADS documents are taken by falling weight (the longest key ranges), and a document's units from its
 // last one backwards (under a causal mask the longest again), so that short ones are left for the end of a launch; else, and
 // among more documents, they come in order.
@@ -91,7 +96,11 @@ __device__ __forceinline__ void find_unit(int count, int slot, FindScratch<THREA
       if (thread == S.hit[0]) found(record, d, S.hit[1]);
       __syncthreads();
     }
-    if (slot < total) return;
+    if (slot < total) {
+      if (blockIdx.x == 0)  // behind the last unit's documents nobody looks for one
+        for (base += THREADS; base < count; base += THREADS) load(base + thread, base + thread < count);
+      return;
+    }
     slot -= total;
   }
 }

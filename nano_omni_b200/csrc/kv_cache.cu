@@ -97,13 +97,12 @@ cache_append_kernel(const AppendParams P) {
         Sequence r = {};
         if (live) {
           r.end = P.lengths[d];
-          const int2 rows = document_rows(P.bounds, d, P.rows);
-          const int fresh = rows.y - rows.x;
-          r.first = rows.x, r.before = r.end - fresh;
-          if (fresh > 0 && (r.before < 0 || r.end > P.max_blocks * kBlock))
-            atomicOr(P.status, kBadIndex);  // a length that cannot be right
+          const bool fit = bounds_fit(P.bounds, d, P.rows);
+          const int fresh = fit ? P.bounds[d + 1] - P.bounds[d] : 0;
+          if (!fit || (fresh > 0 && (r.end < fresh || r.end > P.max_blocks * kBlock)))
+            atomicOr(P.status, kBadIndex);  // bounds or a length that cannot be right: no rows of it are appended
           else if (fresh > 0)
-            r.units = (r.end + kBlock - 1) / kBlock - r.before / kBlock;
+            r.first = P.bounds[d], r.before = r.end - fresh, r.units = (r.end + kBlock - 1) / kBlock - r.before / kBlock;
         }
         return r;
       },
