@@ -43,7 +43,8 @@ constexpr float kLowestMaximum = -1e38f;  // relative to it a key of score -inf 
 
 struct Unit {
   int sequence, index;   // -1: none; which group of columns of it
-  int row0, tokens;      // its new tokens
+  int row0, tokens;      // its new tokens that are there
+  int behind;            // new tokens whose rows would lie past the last one
   int length, prefix;
 };
 
@@ -130,7 +131,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
   pdl_wait();
   struct Sequence {
     int2 rows;
-    int length, prefix, units, weight;
+    int behind, length, prefix, units, weight;
   };
   find_unit<kThreads, true>(
       P.sequences, slot, S.find,
@@ -139,12 +140,13 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         if (live) {
           r.length = r.weight = P.lengths[d];
           r.prefix = P.prefix ? P.prefix[d] : 0;
-          r.rows = document_rows(P.bounds, d, P.rows);
+          r.rows = document_rows(P.bounds, d, P.rows, &r.behind);
+          if (!bounds_fit(P.bounds, d, P.rows)) atomicOr(P.status, kBadIndex);
           r.units = ((r.rows.y - r.rows.x) * P.group + kColumns - 1) / kColumns;
         }
         return r;
       },
-      [&](const Sequence& r, int d, int index) { S.unit = {d, index, r.rows.x, r.rows.y - r.rows.x, r.length, r.prefix}; });
+      [&](const Sequence& r, int d, int index) { S.unit = {d, index, r.rows.x, r.rows.y - r.rows.x, r.behind, r.length, r.prefix}; });
   pdl_release();
   const Unit unit = S.unit;
   const int sequence = unit.sequence;
@@ -153,7 +155,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
   Sight sight;
   sight.keys = clamped(unit.length, 0, P.max_blocks * kBlock);
   if (unit.length != sight.keys && threadIdx.x == 0) atomicOr(P.status, kBadIndex);
-  sight.ahead = sight.keys - unit.tokens;
+  sight.ahead = sight.keys - unit.tokens - unit.behind;
   sight.prefix = unit.prefix;
   sight.causal = P.causal != 0;
   const int items = unit.tokens * P.group;  // (token, head of the group) pairs

@@ -87,7 +87,7 @@ static_assert(sizeof(Shared) + 1024 <= 227 * 1024, "shared memory of an SM");
 __device__ __forceinline__ void find_own_unit(const CacheParams& P, Shared& S, int slot, int piece) {
   struct Sequence {
     int2 rows;
-    int length, prefix, units, weight;
+    int behind, length, prefix, units, weight;
   };
   find_unit<kThreads, true>(
       P.sequences, slot, S.find,
@@ -96,7 +96,8 @@ __device__ __forceinline__ void find_own_unit(const CacheParams& P, Shared& S, i
         if (live) {
           r.length = r.weight = P.lengths[d];
           r.prefix = P.prefix ? P.prefix[d] : 0;
-          r.rows = document_rows(P.bounds, d, P.rows);
+          r.rows = document_rows(P.bounds, d, P.rows, &r.behind);
+          if (!bounds_fit(P.bounds, d, P.rows)) atomicOr(P.status, kBadIndex);
           r.units = ((r.rows.y - r.rows.x) * P.group + kTile - 1) / kTile;
         }
         return r;
@@ -110,7 +111,7 @@ __device__ __forceinline__ void find_own_unit(const CacheParams& P, Shared& S, i
         u.row0 = r.rows.x;
         u.sight.keys = clamped(r.length, 0, P.max_blocks * kBlock);
         if (u.sight.keys != r.length) atomicOr(P.status, kBadIndex);
-        u.sight.ahead = u.sight.keys - tokens;
+        u.sight.ahead = u.sight.keys - tokens - r.behind;
         u.sight.prefix = r.prefix;
         u.sight.causal = P.causal != 0;
         const int seen = u.sight.visible((u.item0 + min(u.items, kTile) - 1) / P.group);

@@ -22,10 +22,11 @@ inline long long most_units(long long rows, long long documents, int unit) {
 
 __device__ __forceinline__ int clamped(int x, int low, int high) { return min(max(x, low), high); }
 
-// Rows [begin, end) of document `d`, inside [0, rows].
-__device__ __forceinline__ int2 document_rows(const int* bounds, int d, int rows) {
-  const int begin = clamped(bounds[d], 0, rows);
-  return make_int2(begin, clamped(bounds[d + 1], begin, rows));
+// Rows [begin, end) of document `d`, inside [0, rows].  `behind` of them, if given, are rows that it claims past the last one.
+__device__ __forceinline__ int2 document_rows(const int* bounds, int d, int rows, int* behind = nullptr) {
+  const int begin = clamped(bounds[d], 0, rows), end = clamped(bounds[d + 1], begin, rows);
+  if (behind) *behind = max(bounds[d + 1], end) - end;
+  return make_int2(begin, end);
 }
 
 // Whether document `d` begins and ends inside [0, rows], in this order.

@@ -4,12 +4,39 @@ the largest."""
 import pytest
 import torch
 
-from tests.test_gpu_kv_cache import Cache, append_op, ints, random_rows, run_op
+from tests.test_gpu_kv_cache import HALF, Cache, append_op, ints, random_rows, run_op
 
 pytestmark = pytest.mark.gpu
 
 MOST, LEAST = 2**31 - 1, -(2**31)
 BAD = 64  # bit 6 of the status word
+
+
+def cached(cache, q, bounds, columns, splits=1, status=0, total_heads=None, causal=True, cap=0.0, scale=128**-0.5):
+    """The cache attention at a chosen division of the work; rows that it does not write stay NaN."""
+    from nano_omni_b200 import _lib
+    from nano_omni_b200.core import DType
+    from nano_omni_b200.kernels.cache import CacheAttentionArguments, CacheAttentionConfig, CacheAttentionKernel
+    from nano_omni_b200.kernels.masked import share_workspace_bytes
+    from tests.gpu_util import desc
+
+    c, out, b = cache.desc(), torch.full_like(q, float("nan")), ints(bounds)
+    need = share_workspace_bytes(len(q), q.shape[1], splits)
+    workspace = desc(torch.full((need,), 255, dtype=torch.uint8, device="cuda"), DType.U8) if need else None
+    arguments = CacheAttentionArguments(
+        desc(q), c.key, c.value, c.key_scales, c.value_scales, c.table, c.lengths, desc(b), None, None, desc(out), 0, causal, scale, cap,
+        workspace,
+    )  # fmt: skip
+    CacheAttentionKernel(arguments, CacheAttentionConfig(columns=columns, kv_splits=splits)).submit()
+    got = _lib.read_status()
+    assert got == status, f"{got:#x}"
+    return out
+
+
+def allowed_of(want, size, keys, most, extra=0.0):
+    """Of the cached attention: the result rounded to bf16, probabilities to f16 (2^-11 = HALF / 8, and HALF / 5 for what fp32
+    leaves out), those below 2^-21 of the row's largest by 2^-32 of it; ``extra``: of the scores, absolute."""
+    return HALF * (0.4 * size + want.abs()) + 2 * extra * size + keys * 2.0**-32 * most + 1e-30
 
 
 # ------------------------------------------------------------------ append
@@ -68,3 +95,53 @@ def test_append_notes_bounds_behind_the_last_rows(bounds):
     run_op(append_op(cache, k, v, ints([*range(129), *[128] * 170, *bounds])), status=BAD)
     for which in range(2):
         assert torch.equal(cache.scales[which], want[1][which]) and torch.equal(cache.codes[which], want[0][which])
+
+
+# ------------------------------------------------------------------ bounds of the attentions
+@pytest.mark.parametrize("columns,splits", [(8, 1), (8, 3), (16, 1), (128, 1), (128, 2)])
+@pytest.mark.parametrize("bounds", [[0, 30, 50], [-7, 20, 40], [0, 30, MOST], [LEAST, 25, 40], [0, 40, 41]], ids=str)
+def test_cached_rows_keep_their_positions_under_bounds_outside_the_rows(columns, splits, bounds):
+    """Rows that are there stand where the bounds put them, and the status word says that some are not there."""
+    from tests.attention64 import attend
+
+    cache = Cache([300, 170], 2, seed=7)
+    q = random_rows(8, 40, 4)
+    out = cached(cache, q, bounds, columns, splits, status=BAD)
+    for s in range(2):
+        k, v = cache.rows(0, s), cache.rows(1, s)
+        for row in range(max(bounds[s], 0), min(bounds[s + 1], 40)):
+            seen = min(len(k), max(0, len(k) - (bounds[s + 1] - row) + 1))
+            want, size = attend(q[row : row + 1], k[:seen], v[:seen])
+            off = (out[row : row + 1].double() - want).abs()
+            assert (off <= allowed_of(want, size, seen, v.abs().amax())).all(), (s, row)
+
+
+@pytest.mark.parametrize("columns,splits", [(8, 1), (16, 2), (128, 1), (128, 2)])
+def test_cached_bounds_that_descend_show(columns, splits):
+    """A sequence that ends before it begins has no rows; the others' are right where no two claim a row."""
+    from tests.attention64 import attend
+
+    cache = Cache([300, 170, 90], 2, seed=9)
+    q, bounds = random_rows(10, 40, 4), [0, 20, 12, 40]
+    out = cached(cache, q, bounds, columns, splits, status=BAD)
+    for s, rows in ((0, slice(0, 12)), (2, slice(20, 40))):
+        k, v = cache.rows(0, s), cache.rows(1, s)
+        want, size = attend(q[bounds[s] : bounds[s + 1]], k, v, causal=True)
+        here = slice(rows.start - bounds[s], rows.stop - bounds[s])
+        off = (out[rows].double() - want[here]).abs()
+        assert (off <= allowed_of(want, size, len(k), v.abs().amax())[here]).all(), s
+
+
+@pytest.mark.parametrize("columns,first", [(8, 128), (128, 640)])
+@pytest.mark.parametrize("last", [9999, 100])
+def test_cached_bounds_behind_the_last_rows_show(columns, first, last):
+    """More sequences than a CTA looks up at once; those behind the first have no rows, and no CTA to look for any."""
+    from tests.attention64 import attend
+
+    cache = Cache([70] * (2 * first + 20), 1, seed=31)
+    q = random_rows(32, first, 1)
+    out = cached(cache, q, [*range(first + 1), *[first] * (first + 19), last], columns, status=BAD)
+    for s in (0, 1, first - 1):
+        k, v = cache.rows(0, s), cache.rows(1, s)
+        want, size = attend(q[s : s + 1], k, v)
+        assert ((out[s : s + 1].double() - want).abs() <= allowed_of(want, size, 70, v.abs().amax())).all()
