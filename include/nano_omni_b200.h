@@ -362,7 +362,9 @@ int nob200_hadamard128_heads(int tokens, int head_offset, const void* input, voi
  * [num_key_rows, kv_heads, 128] (heads a multiple of kv_heads; head h reads key head h / (heads / kv_heads)), output bf16
  * [num_rows, total_heads, 128] at head_offset.  bounds / key_bounds int32 [documents + 1], ascending: rows
  * bounds[d] .. bounds[d + 1] attend to key rows key_bounds[d] .. key_bounds[d + 1]; rows outside all documents are left as
- * they are.  Query i of n stands at position p = i + m - n among its document's m keys.
+ * they are.  Bounds count as clamped to [0, num_rows] and [0, num_key_rows]; a document that ends before it begins has no
+ * rows, or no keys, and sets bit 6 of the status word.  Query i of n stands at position p = i + m - n among its document's
+ * m keys.
  *   score = scale * q.k;  cap > 0: cap * tanh(score / cap);  slopes f32 [heads] not NULL: minus slopes[h] * |p - j|
  *   (without a cap they take a scale of 1e-12 or more)
  *   causal != 0: key j is seen if j <= p or j < prefix[d] (int32 [documents], NULL: 0); else all keys of the document are.

@@ -145,3 +145,54 @@ def test_cached_bounds_behind_the_last_rows_show(columns, first, last):
         k, v = cache.rows(0, s), cache.rows(1, s)
         want, size = attend(q[s : s + 1], k, v)
         assert ((out[s : s + 1].double() - want).abs() <= allowed_of(want, size, 70, v.abs().amax())).all()
+
+
+@pytest.mark.parametrize("unit_rows,splits", [(256, 1), (128, 1), (128, 2)])
+@pytest.mark.parametrize("which", ["rows", "keys"])
+def test_masked_bounds_that_descend_show(unit_rows, splits, which):
+    from nano_omni_b200 import _lib
+    from nano_omni_b200.core import DType
+    from nano_omni_b200.kernels.masked import (
+        MaskedBf16AttentionArguments,
+        MaskedBf16AttentionConfig,
+        MaskedBf16AttentionKernel,
+        share_workspace_bytes,
+    )
+    from tests.attention64 import attend
+    from tests.gpu_util import desc
+    from tests.test_gpu_masked_attention import tolerance
+
+    q, k, v = (random_rows(seed, 300, 2) for seed in (11, 12, 13))
+    bounds = [0, 120, 90, 300] if which == "rows" else [0, 120, 200, 300]
+    key_bounds = [0, 120, 90, 300] if which == "keys" else bounds
+    out = torch.full_like(q, float("nan"))
+    need = share_workspace_bytes(300, 2, splits)
+    workspace = desc(torch.empty(need, dtype=torch.uint8, device="cuda"), DType.U8) if need else None
+    b, kb = ints(bounds), ints(key_bounds)
+    arguments = MaskedBf16AttentionArguments(desc(q), desc(k), desc(v), desc(b), desc(kb), None, None, desc(out), 0, False, workspace=workspace)
+    MaskedBf16AttentionKernel(arguments, MaskedBf16AttentionConfig(unit_rows=unit_rows, kv_splits=splits)).submit()
+    got = _lib.read_status()
+    assert got == BAD, f"{got:#x}"
+    want, size = attend(q[:120], k[:120], v[:120])
+    assert ((out[:90].double() - want[:90]).abs() <= tolerance(want, size)[:90]).all()
+    if which == "keys":
+        assert (out[120:200] == 0).all()  # no keys
+    want, size = attend(q[200:300], k[90:300], v[90:300])
+    assert ((out[200:300].double() - want).abs() <= tolerance(want, size)).all()
+
+
+@pytest.mark.parametrize("heads,last", [(1, 100), (4, 100), (4, 9999)])
+def test_masked_bounds_behind_the_last_rows(heads, last):
+    """More documents than a CTA looks up at once; those behind the first have no rows, and no CTA to look for any."""
+    from nano_omni_b200 import _lib
+    from tests.gpu_util import desc
+    from tests.test_gpu_masked_attention import op_of
+
+    q, k, v = (random_rows(seed, 384, heads) for seed in (33, 34, 35))
+    out = torch.zeros_like(q)
+    op = op_of(q, k, v, [*range(385), *[384] * 600, last]).to(desc(out))
+    scratch = torch.empty(op.prepare()[1] + 256, dtype=torch.uint8, device="cuda")
+    op.run(scratch[(-scratch.data_ptr()) % 256 :])
+    got = _lib.read_status()
+    assert got == (BAD if last < 384 else 0), f"{got:#x}"
+    assert torch.equal(out, v)  # every document is a row that sees itself
