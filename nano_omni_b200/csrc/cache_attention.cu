@@ -300,13 +300,35 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
 #pragma unroll
         for (int m = 0; m < kStep / 16; ++m)
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            float x = s[m][n][2 * h + c] * f;
-            if constexpr (CAP) x = tanh_any(x) * P.to_log2;
-            if constexpr (BIAS) x -= slope[n][c] * static_cast<float>(abs(position[n][c] - (key0 + quad + 16 * m + 8 * h)));
-            s[m][n][2 * h + c] = x;
-          }
+          for (int h = 0; h < 2; ++h) s[m][n][2 * h + c] *= f;
       }
+    if constexpr (CAP) {
+      float most = 0.f;
+      auto each = [&](auto function) {
+#pragma unroll
+        for (int m = 0; m < kStep / 16; ++m)
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) function(s[m][n][c]);
+      };
+      each([&](float& x) { most = fmaxf(most, fabsf(x)); });
+      if (__all_sync(0xffffffffu, most <= 0.3f))
+        each([&](float& x) { x = tanh_near(x) * P.to_log2; });
+      else
+        each([&](float& x) { x = tanh_any(x) * P.to_log2; });
+    }
+    if constexpr (BIAS) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int m = 0; m < kStep / 16; ++m)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              s[m][n][2 * h + c] -= slope[n][c] * static_cast<float>(abs(position[n][c] - (key0 + quad + 16 * m + 8 * h)));
+    }
     if (!whole) {
 #pragma unroll
       for (int n = 0; n < NT; ++n)

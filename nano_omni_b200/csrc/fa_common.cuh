@@ -99,13 +99,21 @@ __device__ __forceinline__ float rcp(float x) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// tanh(x) for |x| <= 0.3 by the polynomial of three terms in cap_scores; relative error 4e-6.
+__device__ __forceinline__ float tanh_near(float x) {
+  const float u = x * x;
+  return x * fmaf(fmaf(0.1252259100369678f, u, -0.3329747970785575f), u, 0.9999960103875557f);
+}
 // any x: 1 - 2 / (1 + 2^(2 log2(e) x)); absolute error some 2^-22
-__device__ __forceinline__ float tanh_any(float x) { return fmaf(-2.f, rcp(1.f + ex2(x * 2.885390081777927f)), 1.f); }
+__device__ __forceinline__ float tanh_far(float x) { return fmaf(-2.f, rcp(1.f + ex2(x * 2.885390081777927f)), 1.f); }
+// any x: relative error 4e-6.  2^-22 of the cap is too much for a score far below a large one.
+__device__ __forceinline__ float tanh_any(float x) { return fabsf(x) <= 0.3f ? tanh_near(x) : tanh_far(x); }
 
 // s = f tanh(c s) for the scores of a row, by as short a way as the warp's largest allows.  c s up to 0.3 in magnitude: an odd
 // polynomial of three terms (1.7e-7 absolute) with c and f in its coefficients, four packed operations a pair; up to 1: of six
-// terms, nine operations; else the exponential, two MUFU operations a score.  (4096 capped rows of three documents x 32 heads:
-// 153 us with six terms for all up to 1.)
+// terms, nine operations; else the exponential, two MUFU operations a score, beside it the short polynomial where the cap is so
+// large that an error of 2^-22 of it counts (5e-5 at 180; for every cap it took the 1560 rows against 31560 keys, scores past
+// the cap, from 952 to 1089 us).  (4096 capped rows of three documents x 32 heads: 153 us with six terms for all up to 1.)
 template <int N>
 __device__ __forceinline__ void cap_scores(uint32_t (&s)[N], float c, float f) {
   float most[4] = {0.f, 0.f, 0.f, 0.f};
@@ -131,6 +139,9 @@ __device__ __forceinline__ void cap_scores(uint32_t (&s)[N], float c, float f) {
     const uint64_t c2 = pack2(c, c), f2 = pack2(f, f);
 #pragma unroll
     for (int i = 0; i < N; i += 2) put(i, mul2(tanh_small2(mul2(pair(i), c2)), f2));
+  } else if (f <= 256.f) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) s[i] = __float_as_uint(tanh_far(__uint_as_float(s[i]) * c) * f);
   } else {
 #pragma unroll
     for (int i = 0; i < N; ++i) s[i] = __float_as_uint(tanh_any(__uint_as_float(s[i]) * c) * f);

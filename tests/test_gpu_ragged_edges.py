@@ -196,3 +196,33 @@ def test_masked_bounds_behind_the_last_rows(heads, last):
     got = _lib.read_status()
     assert got == (BAD if last < 384 else 0), f"{got:#x}"
     assert torch.equal(out, v)  # every document is a row that sees itself
+
+
+# ------------------------------------------------------------------ caps
+@pytest.mark.parametrize("columns", [8, 16, 128])
+@pytest.mark.parametrize("cap", [1e3, 1e5, 1e6, 1e9, 1e30])
+def test_cached_scores_far_below_the_cap(columns, cap):
+    """Scores of up to some 10 under caps that are next to none: the tanh's polynomial is off by 4e-6 of a score."""
+    from tests.attention64 import attend
+
+    cache = Cache([900], 1, seed=14)
+    q = random_rows(15, 9, 3)
+    out = cached(cache, q, [0, 9], columns, cap=cap)
+    k, v = cache.rows(0, 0), cache.rows(1, 0)
+    want, size = attend(q, k, v, causal=True, cap=cap)
+    most = (torch.einsum("nhd,md->nhm", q.double(), k[:, 0]) * 128**-0.5).abs().amax().item()
+    assert ((out.double() - want).abs() <= allowed_of(want, size, 900, v.abs().amax(), extra=4e-6 * most)).all()
+
+
+@pytest.mark.parametrize("columns", [8, 16, 128])
+def test_small_scores_beside_capped_ones(columns):
+    """Rows of one call whose scores differ by orders of magnitude: a large cap is as exact for the small ones."""
+    from tests.attention64 import attend
+
+    cache = Cache([700], 1, seed=16)
+    q = random_rows(17, 8, 1)
+    q[::2] *= 2.0**20
+    out = cached(cache, q, [0, 8], columns, cap=1e6)[1::2]
+    k, v = cache.rows(0, 0), cache.rows(1, 0)
+    want, size = (x[1::2] for x in attend(q, k, v, causal=True, cap=1e6))
+    assert ((out.double() - want).abs() <= allowed_of(want, size, 700, v.abs().amax(), extra=6e-5)).all()
