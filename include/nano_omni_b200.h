@@ -366,7 +366,7 @@ int nob200_hadamard128_heads(int tokens, int head_offset, const void* input, voi
  * rows, or no keys, and sets bit 6 of the status word.  Query i of n stands at position p = i + m - n among its document's
  * m keys.
  *   score = scale * q.k;  cap > 0: cap * tanh(score / cap);  slopes f32 [heads] not NULL: minus slopes[h] * |p - j|
- *   (without a cap they take a scale of 1e-12 or more)
+ *   (without a cap they take a scale of 1e-12 or more; scale / cap lies between 1e-35 and 1e35)
  *   causal != 0: key j is seen if j <= p or j < prefix[d] (int32 [documents], NULL: 0); else all keys of the document are.
  * A row that sees no key gets zeros.  Keys and values that a row does not see may hold anything (infinities, NaN); where a
  * document's value row is not finite, whole rows that see it under a partial mask become NaN.

@@ -229,6 +229,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     for (int c = 0; c < 2; ++c) {
       const int from = 4 * (2 * part + c);  // a lane that read the column
       factor[n][c] = __shfl_sync(0xffffffffu, __uint_as_float(exponent << 23) * P.scale, from);
+      if (CAP) factor[n][c] = fminf(factor[n][c], 1e30f);  // past the cap at any scale of K, and a score of 0 is not 0 x inf
       visible[n][c] = __shfl_sync(0xffffffffu, live ? sight.visible(token) : 0, from);
       position[n][c] = BIAS ? __shfl_sync(0xffffffffu, sight.ahead + token, from) : 0;
       slope[n][c] = BIAS ? __shfl_sync(0xffffffffu, P.slopes[head] * 1.4426950408889634f, from) : 0.f;
@@ -547,6 +548,7 @@ extern "C" int nob200_int8_cache_attention_d128(int num_rows, int sequences, int
               "%s: a tensor is not 16-byte aligned", name);
   NOB_REQUIRE(scale > 0.f && scale <= 1e30f, "%s: scale %g must be positive and finite", name, scale);
   NOB_REQUIRE(cap >= 0.f && cap <= 1e30f, "%s: cap %g must be finite, 0 for none", name, cap);
+  NOB_REQUIRE(cap_fits(scale, cap), "%s: scale / cap must lie between 1e-35 and 1e35 (got %g / %g)", name, scale, cap);
   NOB_REQUIRE(columns == 8 || columns == 16 || columns == 128, "%s: columns must be 8, 16 or 128 (got %d)", name, columns);
   NOB_REQUIRE(kv_splits >= 1 && kv_splits <= 64, "%s: kv_splits %d outside [1, 64]", name, kv_splits);
   const int group = heads / kv_heads;

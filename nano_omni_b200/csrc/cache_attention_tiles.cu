@@ -427,7 +427,10 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&S.s_taken);
-        if (j == 0) row_scale = *const_cast<const volatile float*>(&S.factor[threadIdx.x & 127]) * P.scale;
+        if (j == 0) {
+          row_scale = *const_cast<const volatile float*>(&S.factor[threadIdx.x & 127]) * P.scale;
+          if (CAP) row_scale = fminf(row_scale, 1e30f);  // past the cap at any scale of K, and a score of 0 is not 0 x inf
+        }
         const volatile float* kept = &S.scales[block % kScaleSlots].x;
         const float key_scale = kept[0] * row_scale, value_scale = kept[1];
         const bool there = value_scale != kNotThere;

@@ -18,6 +18,9 @@ inline long long most_units(long long rows, long long documents, int unit) {
   return most < rows ? most : rows;
 }
 
+// Scores are multiplied by scale / cap, which fp32 has to hold with all of its bits.
+inline bool cap_fits(float scale, float cap) { return cap == 0.f || (scale / cap >= 1e-35f && scale / cap <= 1e35f); }
+
 #ifdef __CUDACC__
 
 __device__ __forceinline__ int clamped(int x, int low, int high) { return min(max(x, low), high); }

@@ -126,7 +126,8 @@ __device__ __forceinline__ void cap_scores(uint32_t (&s)[N], float c, float f) {
     unpack2(v, a, b);
     s[i] = __float_as_uint(a), s[i + 1] = __float_as_uint(b);
   };
-  if (__all_sync(0xffffffffu, x <= 0.3f && top <= 1e18f)) {  // whose square is finite
+  // The scores' square and c's fifth power stay finite; below 1e-7 the latter may vanish, which leaves the first term of the tanh.
+  if (__all_sync(0xffffffffu, x <= (c >= 1e-7f ? 0.3f : 1e-3f) && top <= 1e18f && c <= 1e5f) && f <= 1e10f) {
     const float cc = c * c, b0 = f * c;
     const float a0 = b0 * 0.9999960103875557f, a1 = b0 * cc * -0.3329747970785575f, a2 = b0 * cc * cc * 0.1252259100369678f;
     const uint64_t p0 = pack2(a0, a0), p1 = pack2(a1, a1), p2 = pack2(a2, a2);

@@ -672,6 +672,7 @@ extern "C" int nob200_masked_bf16_attention_d128(int num_rows, int num_key_rows,
   NOB_REQUIRE(reinterpret_cast<uintptr_t>(output) % 16 == 0, "%s: output %p is not 16-byte aligned", name, output);
   NOB_REQUIRE(scale > 0.f && scale <= 1e30f, "%s: scale %g must be positive and finite", name, scale);
   NOB_REQUIRE(cap >= 0.f && cap <= 1e30f, "%s: cap %g must be finite, 0 for none", name, cap);
+  NOB_REQUIRE(cap_fits(scale, cap), "%s: scale / cap must lie between 1e-35 and 1e35 (got %g / %g)", name, scale, cap);
   NOB_REQUIRE(!slopes || cap > 0.f || scale >= 1e-12f, "%s: slopes, which are divided by it, need a scale of 1e-12 or more (got %g)", name, scale);
   NOB_REQUIRE(unit_rows == kTile || unit_rows == 2 * kTile, "%s: unit_rows must be 128 or 256 (got %d)", name, unit_rows);
   NOB_REQUIRE(kv_splits >= 1 && kv_splits <= 64, "%s: kv_splits %d outside [1, 64]", name, kv_splits);

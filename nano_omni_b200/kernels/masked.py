@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import dataclasses
+import math
 from typing import Literal, NamedTuple
 
 from pydantic import Field
@@ -122,6 +123,9 @@ def check_masks(arguments, documents: int, heads: int) -> None:
         require_tensor(arguments.prefix, DType.I32, (documents,), "prefix")
     if arguments.slopes is not None:
         require_tensor(arguments.slopes, DType.F32, (heads,), "slopes")
+    scale, cap = arguments.scale, arguments.cap
+    if scale > 0 and 0 < cap < math.inf:
+        assert 1e-35 <= scale / cap <= 1e35, f"scale / cap must lie between 1e-35 and 1e35, not {scale} / {cap}"
 
 
 class MaskedBf16AttentionKernel(

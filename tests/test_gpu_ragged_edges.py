@@ -226,3 +226,43 @@ def test_small_scores_beside_capped_ones(columns):
     k, v = cache.rows(0, 0), cache.rows(1, 0)
     want, size = (x[1::2] for x in attend(q, k, v, causal=True, cap=1e6))
     assert ((out.double() - want).abs() <= allowed_of(want, size, 700, v.abs().amax(), extra=6e-5)).all()
+
+
+@pytest.mark.parametrize("cap", [1e-9, 1e-12, 1e-20, 1e-30])
+@pytest.mark.parametrize("zero", [True, False])
+@pytest.mark.parametrize("form", ["masked", 8, 16, 128])
+def test_caps_next_to_nothing(form, zero, cap):
+    """All scores are within the cap of zero, so a row is the plain mean of what it sees."""
+    from tests.attention64 import attend
+    from tests.test_gpu_masked_attention import attend as masked_attend
+    from tests.test_gpu_masked_attention import tolerance
+
+    q = random_rows(18, 200, 2)
+    if zero:
+        q.zero_()
+    if form == "masked":
+        k, v = random_rows(19, 200, 2), random_rows(20, 200, 2)
+        out = masked_attend(q, k, v, [0, 200], causal=True, cap=cap)
+        want, size = attend(q, k, v, causal=True, cap=cap)
+        allowed = tolerance(want, size)
+    else:
+        cache = Cache([300], 2, seed=21)
+        out = cached(cache, q, [0, 200], form, cap=cap)
+        k, v = cache.rows(0, 0), cache.rows(1, 0)
+        want, size = attend(q, k, v, causal=True, cap=cap)
+        allowed = allowed_of(want, size, 300, v.abs().amax())
+    assert ((out.double() - want).abs() <= allowed).all()
+
+
+def test_capped_scores_of_large_products():
+    """Products of 2^50 under a scale that makes ordinary scores of them: the scale over the cap has no square in fp32's range."""
+    from tests.attention64 import attend
+    from tests.test_gpu_masked_attention import attend as masked_attend
+    from tests.test_gpu_masked_attention import tolerance
+
+    q, k, v = random_rows(22, 130, 1), random_rows(23, 130, 1), random_rows(24, 130, 1)
+    scale = 128**-0.5 * 2.0**-50
+    q, k = q * 2.0**25, k * 2.0**25
+    out = masked_attend(q, k, v, [0, 130], cap=15.0, scale=scale)
+    want, size = attend(q, k, v, cap=15.0, scale=scale)
+    assert ((out.double() - want).abs() <= tolerance(want, size, extra=6e-5)).all()

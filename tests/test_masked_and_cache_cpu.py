@@ -234,3 +234,21 @@ def test_calls_without_rows_documents_or_tokens_are_refused():
     for rows, tokens in ((0, None), (3, 0)):
         with pytest.raises(AssertionError):
             ops.CacheAttention(at(DType.BF16, rows, 512), at(DType.I32, 4), cache(), total_heads=4, cached_tokens=tokens)
+
+
+@pytest.mark.parametrize("scale,cap", [(0.1, 1e-37), (1e-12, 1e26), (1e20, 1e-17)])
+def test_a_scale_over_the_cap_outside_fp32_is_refused(lib, scale, cap):
+    with pytest.raises(AssertionError):
+        masked(scale=scale, cap=cap).to(at(DType.BF16, 300, 6, 128)).prepare()
+    op = ops.CacheAttention(at(DType.BF16, 3, 512), at(DType.I32, 4), cache(), total_heads=4, scale=scale, cap=cap)
+    with pytest.raises(AssertionError):
+        op.to(at(DType.BF16, 3, 4, 128)).prepare()
+    p, null, z, f = ctypes.c_void_p(1 << 20), ctypes.c_void_p(0), ctypes.c_size_t(0), ctypes.c_float
+    calls = {
+        "masked_bf16": (9, 70, 3, 0, p, p, p, p, p, null, null, p, 4, 2, 4, 1, f(scale), f(cap), 256, 1, null, z, null),
+        "int8_cache": (3, 3, 5, 11, 0, p, p, p, p, p, p, p, p, null, null, p, 4, 2, 4, 1, f(scale), f(cap), 16, 1, null, z, null),
+    }
+    for name, arguments in calls.items():
+        fn = getattr(lib, f"nob200_{name}_attention_d128")
+        fn.restype = ctypes.c_int
+        assert fn(*arguments) == -1 and b"scale / cap" in lib.nob200_last_error()
