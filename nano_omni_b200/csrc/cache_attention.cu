@@ -383,11 +383,14 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     // ---- values
     ok = warp_rest(&full[nv % kStages], (nv / kStages) & 1, abort_flag, P.status, kWaitTimeoutLoad);
     if (!ok) break;
-    float take[NT][2];  // a column that sees nothing of the step has probabilities of 0 and takes 0 of it, whatever its scale is
+    // a column that sees nothing of the step has probabilities of 0 and takes 0 of it, whatever its scale is; one below 1e-30 is
+    // taken for 0, as in the tiles
+    float take[NT][2];
+    const float taken = fabsf(value_scale) < 1e-30f ? 0.f : value_scale;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int c = 0; c < 2; ++c) take[n][c] = e0 >= 0 && visible[n][c] > key0 ? value_scale : 0.f;
+      for (int c = 0; c < 2; ++c) take[n][c] = e0 >= 0 && visible[n][c] > key0 ? taken : 0.f;
     const uint32_t v_at = smem_u32(ring[nv % kStages]);
     const int v_key = ((lane >> 3) & 1) * 8 + (lane & 7);  // ldmatrix: the row whose address this lane gives
 #pragma unroll

@@ -4,8 +4,8 @@
 // A unit is up to 128 rows - (new token, head of the group) pairs of a sequence and key head - against 128 keys, two blocks, at a
 // time.  The scores and values are tcgen05 products of f16 operands, which hold an 8-bit code exactly (and take five instructions
 // for four codes, bf16 eight); queries are scaled by a power of two to a row maximum in [1, 2) (exact down to 2^-24 of it).  The
-// scales of K multiply the scores as they leave TMEM, those of V the probabilities before these are rounded to f16, so
-// nothing of K and V is rounded.  (Sixteen columns at a time by mma.sync widen every code once per sixteen rows: 1200 warp
+// scales of K multiply the scores as they leave TMEM, those of V the probabilities before these are rounded to f16 (their
+// signs the codes, in the fused multiply-add that widens them), so nothing of K and V is rounded.  (Sixteen columns at a time by mma.sync widen every code once per sixteen rows: 1200 warp
 // instructions per 32 keys, 28 rows against 4000 keys x 8 heads x 16 sequences 102 us, here 60.)
 //   warps 16, 19  TMA producers: the blocks of K and of V as they are, 8 bits, into a ring of five blocks each (one producer for both,
 //                 whose K waited for V's places, held the kernel at 1.8 us a tile)
@@ -64,7 +64,8 @@ struct Unit {
 struct __align__(1024) Shared {
   uint8_t kv[kStages][kTileBytes];
   uint8_t raw[2][kRawStages][kRawBytes];  // of K, of V
-  __align__(16) float2 scales[kScaleSlots];  // (K's, log2 of V's) of a block; NaN, kNotThere for one that is not there
+  __align__(16) float2 scales[kScaleSlots];  // (K's, log2 of V's) magnitude for a block; NaN, kNotThere for one that is not there
+  __half2 sign[2][kRawStages];               // and their signs, for the codes of K and of V; 0 for a V whose scale counts as 0
   uint64_t q_full;
   uint64_t raw_full[2][kRawStages], raw_empty[2][kRawStages];
   uint64_t kv_full[kStages], kv_empty[kStages];
@@ -129,12 +130,12 @@ __device__ __forceinline__ int block_of(const CacheParams& P, const int* table, 
   return block >= 0 && block < P.num_blocks ? block : -1;
 }
 
-// Four signed bytes as f16: offset by 128, a byte u under the exponent of 1024 is 1024 + u.
-__device__ __forceinline__ uint2 widen(uint32_t w) {
+// Four signed bytes times 1, -1 or 0 as f16: offset by 128, a byte u under the exponent of 1024 is 1024 + u; base is -1152 sign.
+__device__ __forceinline__ uint2 widen(uint32_t w, __half2 sign, __half2 base) {
   const uint32_t offset = w ^ 0x80808080u;
   auto two = [&](uint32_t select) {
     const uint32_t a = __byte_perm(offset, 0x64646464u, select);
-    const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&a), __float2half2_rn(1152.f));
+    const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&a), sign, base);
     return *reinterpret_cast<const uint32_t*>(&r);
   };
   return make_uint2(two(0x4140), two(0x4342));
@@ -226,10 +227,10 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
           const int at = 2 * (kv_begin + tile_at((i + lane) >> 1)) + ((i + lane) & 1);
           r.number = block_of(P, table, at);
           if (r.number < 0 && at * kBlock < S.unit.sight.keys) atomicOr(status, kBadIndex);
-          if (v && r.number >= 0) {
+          if (r.number >= 0) {
             const size_t place = static_cast<size_t>(r.number) * P.kv_heads + key_head;
-            r.value = P.value_scales[place];
             r.key = P.key_scales[place];
+            if (v) r.value = P.value_scales[place];
           }
         }
         return r;
@@ -242,17 +243,19 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         const int block = __shfl_sync(0xffffffffu, some.number, i % 32);
         if (i >= kRawStages) ok = rest(&S.raw_empty[v][st], ((i / kRawStages) - 1) & 1, kWaitTimeoutRing);
         if (!ok) break;
+        const float key = __shfl_sync(0xffffffffu, some.key, i % 32), value = __shfl_sync(0xffffffffu, some.value, i % 32);
+        const bool none = v && fabsf(value) < 1e-30f;
         if (lane == 0) {
+          S.sign[v][st] = __float2half2_rn(none ? 0.f : (v ? value : key) < 0.f ? -1.f : 1.f);
           mbar_expect_tx(&S.raw_full[v][st], kRawBytes);
           // a block that is not there: any block, whose scores are masked
           tma_load_3d(S.raw[v][st], map, &S.raw_full[v][st], 0, (max(block, 0) * P.kv_heads + key_head) * kBlock, 0);
         }
         if (v) {
-          const float key = __shfl_sync(0xffffffffu, some.key, i % 32), value = __shfl_sync(0xffffffffu, some.value, i % 32);
-          // V's is a summand of the exponent; of a block whose scale is 0 (or less) next to nothing is taken
-          const float value_log2 = block < 0 ? kNotThere : log2f(value > 0.f ? value : value != value ? value : 1e-30f);
+          // V's is a summand of the exponent; of a block whose scale counts as 0 next to nothing is taken, of zeros
+          const float value_log2 = block < 0 ? kNotThere : log2f(none ? 1e-30f : fabsf(value));
           if (lane == 0) {
-            S.scales[i % kScaleSlots] = make_float2(key, value_log2);
+            S.scales[i % kScaleSlots] = make_float2(fabsf(key), value_log2);
             mbar_arrive(&S.scales_full[i % kScaleSlots]);
           }
         }
@@ -361,12 +364,13 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         uint4 x[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) x[k] = *reinterpret_cast<const uint4*>(S.raw[v][raw] + from[k >> 1] + (k & 1) * 8 * kDim);
+        const __half2 sign = S.sign[v][raw], base = __hmul2(sign, __float2half2_rn(-1152.f));
         __syncwarp();
         if (lane == 0) mbar_arrive(&S.raw_empty[v][raw]);
         uint8_t* tile = S.kv[st] + half * kBlock * 128;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const uint2 a = widen(x[k].x), b = widen(x[k].y), c = widen(x[k].z), d = widen(x[k].w);
+          const uint2 a = widen(x[k].x, sign, base), b = widen(x[k].y, sign, base), c = widen(x[k].z, sign, base), d = widen(x[k].w, sign, base);
           uint8_t* at = tile + (k >> 1) * kHalfBytes + (k & 1) * 8 * 128;
           *reinterpret_cast<uint4*>(at + to[0]) = make_uint4(a.x, a.y, b.x, b.y);
           *reinterpret_cast<uint4*>(at + to[1]) = make_uint4(c.x, c.y, d.x, d.y);

@@ -266,3 +266,41 @@ def test_capped_scores_of_large_products():
     out = masked_attend(q, k, v, [0, 130], cap=15.0, scale=scale)
     want, size = attend(q, k, v, cap=15.0, scale=scale)
     assert ((out.double() - want).abs() <= tolerance(want, size, extra=6e-5)).all()
+
+
+# ------------------------------------------------------------------ scales of any sign
+@pytest.mark.parametrize("columns,rows", [(8, 8), (16, 9), (128, 9), (128, 40), (128, 100)])
+@pytest.mark.parametrize("others", [0.01, 0.0, -0.01, 1e-34])
+def test_value_scales_of_any_sign(columns, rows, others):
+    """Blocks whose values are negated, zero or next to it, beside ordinary ones and alone."""
+    from tests.attention64 import attend
+
+    cache = Cache([500], 1, seed=25)
+    blocks = cache.table[0].long()
+    cache.scales[1][blocks[::2]] = others
+    cache.scales[1][blocks[1]] *= -1
+    cache.scales[1][blocks[3]] = 0.0
+    for alone in (False, True):
+        if alone:
+            cache.scales[1].fill_(others)
+        q = random_rows(26, rows, 1)
+        out = cached(cache, q, [0, rows], columns)
+        k, v = cache.rows(0, 0), cache.rows(1, 0)
+        want, size = attend(q, k, v, causal=True)
+        assert ((out.double() - want).abs() <= allowed_of(want, size, 500, v.abs().amax())).all(), alone
+
+
+@pytest.mark.parametrize("columns,rows", [(8, 8), (16, 9), (128, 9), (128, 40), (128, 100)])
+@pytest.mark.parametrize("cap", [0.0, 2.0])
+def test_key_scales_of_any_sign(columns, rows, cap):
+    """Keys that are negated, with scores large enough that the largest and the lowest are not to be taken for one another."""
+    from tests.attention64 import attend
+
+    cache = Cache([500], 1, seed=36)
+    blocks = cache.table[0].long()
+    cache.scales[0][blocks[1:6]] *= -1
+    q = random_rows(37, rows, 1, 6.0)
+    out = cached(cache, q, [0, rows], columns, cap=cap)
+    k, v = cache.rows(0, 0), cache.rows(1, 0)
+    want, size = attend(q, k, v, causal=True, cap=cap)
+    assert ((out.double() - want).abs() <= allowed_of(want, size, 500, v.abs().amax(), extra=1e-4)).all()
