@@ -20,8 +20,8 @@
 //    instruction's k index are chosen so that a lane reads 32 consecutive bytes of a key.
 //  * values: A = V transposed by ldmatrix.trans, which delivers two channels of two keys per register; a permute puts the even
 //    channels in rows 0-7 and the odd ones in rows 8-15.  B = the probabilities, from the scores' layout by movmatrix,
-//    rounded to f16 (2^-11; their sum is taken before); the block's scale of V multiplies the step's product as it joins
-//    the accumulator.
+//    rounded to f16 (2^-11, and 2^-32 of the largest: kLift; their sum is taken before); the block's scale of V multiplies the
+//    step's product as it joins the accumulator.
 #include <cuda.h>
 #include <cuda_fp16.h>
 
@@ -350,7 +350,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         mx[n][c] = fmaxf(fmaxf(s[0][n][c], s[0][n][2 + c]), fmaxf(s[1][n][c], s[1][n][2 + c]));
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) mx[n][c] = fmaxf(mx[n][c], __shfl_xor_sync(0xffffffffu, mx[n][c], d));
-        grown |= mx[n][c] > top[n][c] + kRescaleThreshold;
+        grown |= mx[n][c] > top[n][c] + (kLift + kRescaleThreshold);
       }
     if (__any_sync(0xffffffffu, grown)) {
 #pragma unroll
@@ -358,7 +358,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         float alpha[2];
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          const float now = fmaxf(top[n][c], mx[n][c]);
+          const float now = fmaxf(top[n][c], mx[n][c] - kLift);
           alpha[c] = ex2(top[n][c] - now);
           top[n][c] = now;
           sum[n][c] *= alpha[c];

@@ -6,6 +6,11 @@
 
 namespace nob200 {
 
+// Probabilities are rounded to f16, whose range they use from above: relative to 2^-kLift of a row's running maximum, which they
+// outgrow by 2^8 at most before it is raised, they stay below 2^15, and a weight counts down to 2^-32 of the largest (2^-25
+// without the lift: 131071 keys of 2^-26 each, 0.2 % together, were lost).
+constexpr float kLift = 7.0f;  // log2 units
+
 struct CacheParams {
   const __nv_bfloat16* query;
   const float* key_scales;

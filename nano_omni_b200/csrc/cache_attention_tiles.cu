@@ -253,7 +253,7 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         }
         if (v) {
           // V's is a summand of the exponent; of a block whose scale counts as 0 next to nothing is taken, of zeros
-          const float value_log2 = block < 0 ? kNotThere : log2f(none ? 1e-30f : fabsf(value));
+          const float value_log2 = block < 0 ? kNotThere : log2f(none ? 1e-24f : fabsf(value));
           if (lane == 0) {
             S.scales[i % kScaleSlots] = make_float2(fabsf(key), value_log2);
             mbar_arrive(&S.scales_full[i % kScaleSlots]);
@@ -462,8 +462,8 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         const float value_log2 = sees ? value_scale : 0.f;
         const float mx =
             sees ? fmaf(max3(a, b, fmaxf(__uint_as_float(s[kKeys - 2]), __uint_as_float(s[kKeys - 1]))), unit, value_log2) : kLowestMaximum;
-        if (__any_sync(0xffffffffu, mx > m_used + kRescaleThreshold)) {
-          const float m_new = fmaxf(m_used, mx);
+        if (__any_sync(0xffffffffu, mx > m_used + (kLift + kRescaleThreshold))) {
+          const float m_new = fmaxf(m_used, mx - kLift);
           const float alpha = ex2(m_used - m_new);
           m_used = m_new;
           if (j > 0) {  // P and O are untouched by the tensor core before the first PV

@@ -304,3 +304,27 @@ def test_key_scales_of_any_sign(columns, rows, cap):
     k, v = cache.rows(0, 0), cache.rows(1, 0)
     want, size = attend(q, k, v, causal=True, cap=cap)
     assert ((out.double() - want).abs() <= allowed_of(want, size, 500, v.abs().amax(), extra=1e-4)).all()
+
+
+# ------------------------------------------------------------------ small weights
+@pytest.mark.parametrize("columns,rows,splits", [(8, 1, 1), (8, 1, 8), (16, 9, 2), (128, 9, 1), (128, 40, 4), (128, 100, 1)])
+def test_many_keys_of_little_weight_count(columns, rows, splits):
+    """One key 18 above 131071 others, whose weights, 2^-26 each, make 0.2 % together: they are all of the result where the
+    large one's value is zero."""
+    from tests.attention64 import attend
+
+    n = 131072
+    cache = Cache([n], 1, seed=27)
+    for which in range(2):
+        cache.codes[which].zero_()
+        cache.scales[which].fill_(1 / 128)
+    first = cache.table[0, 0].long()
+    cache.codes[0][first, 0, 0] = 64  # key 0: halves
+    cache.codes[1].fill_(100)
+    cache.codes[1][first, 0, 0] = 0
+    q = torch.full((rows, 1, 128), 18 * 2 * 128**-0.5, dtype=torch.bfloat16, device="cuda")
+    out = cached(cache, q, [0, rows], columns, splits)
+    k, v = cache.rows(0, 0), cache.rows(1, 0)
+    want, size = attend(q[-1:], k, v)
+    assert want.amin() > 0.0005
+    assert ((out[-1:].double() - want).abs() <= allowed_of(want, size, n, v.abs().amax())).all()
