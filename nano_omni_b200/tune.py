@@ -42,11 +42,14 @@ def _fill(desc: TensorDesc, generator: torch.Generator, scale: float) -> TensorD
 
 
 def address(arguments, seed: int = 0, scale: float = 1.0):
+    """``arguments`` with tensors in the place of empty descriptors; what has an address already is left as it is."""
     generator = torch.Generator(device="cuda").manual_seed(seed)
+    given = arguments
     arguments = arguments.map(lambda d: _fill(d, generator, scale) if d.kind == TensorKind.EMPTY else d)
     # kernels that follow indices in device memory say what makes sense there
     for name, values in getattr(arguments, "index_values", dict)().items():
-        getattr(arguments, name).tensor.copy_(torch.tensor(values, dtype=torch.int32))
+        if getattr(given, name).kind == TensorKind.EMPTY:
+            getattr(arguments, name).tensor.copy_(torch.tensor(values, dtype=torch.int32))
     return arguments
 
 

@@ -1,6 +1,8 @@
 """Edges of the ragged operators: bounds and lengths that cannot be right, caps and scales of any size, weights far below
 the largest."""
 
+import math
+
 import pytest
 import torch
 
@@ -328,3 +330,22 @@ def test_many_keys_of_little_weight_count(columns, rows, splits):
     want, size = attend(q[-1:], k, v)
     assert want.amin() > 0.0005
     assert ((out[-1:].double() - want).abs() <= allowed_of(want, size, n, v.abs().amax())).all()
+
+
+# ------------------------------------------------------------------ arguments for timing
+def test_addressing_arguments_leaves_given_tensors():
+    """What a caller has put in place, index tensors among it, is not written."""
+    import dataclasses
+
+    from nano_omni_b200 import tune
+    from nano_omni_b200.kernels.cache import CacheReadKernel, CacheReadWorkload
+    from tests.gpu_util import desc
+
+    empty = CacheReadKernel.make_arguments(CacheReadWorkload(capacity=90, sequences=2, max_blocks=3, num_blocks=9, kv_heads=1))
+    table, lengths = ints([[5, 6, 7], [1, 2, 3]]), ints([40, 50])
+    arguments = tune.address(dataclasses.replace(empty, table=desc(table), lengths=desc(lengths)))
+    assert table.tolist() == [[5, 6, 7], [1, 2, 3]] and lengths.tolist() == [40, 50]
+    assert arguments.bounds.as_torch().tolist() == [0, 0, 0] and arguments.table.as_torch() is table
+    filled = tune.address(empty)
+    assert filled.lengths.as_torch().tolist() == [192, 192] and filled.table.as_torch().tolist() == [[0, 1, 2], [3, 4, 5]]
+    assert not math.isnan(filled.key_scales.as_torch().sum().item())
