@@ -847,8 +847,18 @@ class MaskedBf16Attention(Op):
         assert self.rows > 0 and self.documents > 0, "no rows, or bounds of no document"
         self.causal, self.cap, self.scale = causal, cap, DEFAULT_SCALE if scale is None else scale
         self.key_bounds, self.prefix, self.slopes, self.rotation = key_bounds, prefix, slopes, rotation
-        self.units = plan_masked_units(self.rows, self.key_rows, self.documents, self.heads, causal, cap > 0)
+        self.chosen_units: MaskedUnits | None = None
         super().__init__(query, key, value, bounds, outputs=((DType.BF16, (self.rows, total_heads, 128)),))
+
+    @property
+    def units(self) -> MaskedUnits:
+        """Planned from the options as they are, unless set."""
+        planned = plan_masked_units(self.rows, self.key_rows, self.documents, self.heads, self.causal, self.cap > 0)
+        return planned if self.chosen_units is None else self.chosen_units
+
+    @units.setter
+    def units(self, units: MaskedUnits) -> None:
+        self.chosen_units = units
 
     def kernels(self, scratch: ScratchLayout) -> list[Kernel]:
         sequence = KernelSequence(scratch)

@@ -252,3 +252,19 @@ def test_a_scale_over_the_cap_outside_fp32_is_refused(lib, scale, cap):
         fn = getattr(lib, f"nob200_{name}_attention_d128")
         fn.restype = ctypes.c_int
         assert fn(*arguments) == -1 and b"scale / cap" in lib.nob200_last_error()
+
+
+def test_masked_units_follow_the_options():
+    """An option that is set later is planned for as if it had been given at construction; chosen units stay."""
+    from nano_omni_b200.kernels.masked import MaskedUnits
+
+    shape = {"heads": 28, "kv_heads": 28, "rows": 2100, "key_rows": 2100, "documents": 5, "total_heads": 28}
+    late, out = masked(**shape).to(at(DType.BF16, 2100, 28, 128)), at(DType.BF16, 2100, 28, 128)
+    plain = late.prepare()[0][-1].config
+    late.cap = 30.0
+    early = masked(**shape, cap=30.0).to(out)
+    assert late.prepare()[0][-1].config == early.prepare()[0][-1].config != plain
+    late.units = MaskedUnits(256, 2)
+    late.causal = True
+    call = late.prepare()[0][-1]
+    assert (call.config.unit_rows, call.config.kv_splits) == (256, 2) and call.arguments.workspace is not None
