@@ -92,7 +92,7 @@ struct MaskedParams {
   float* lse;
   uint32_t* status;
   int rows, key_rows, documents, heads, group, total_heads, head_offset;
-  int slots, unit_rows, splits, causal;
+  int unit_rows, splits, causal;
   float scale;    // of a raw score; CAP form: divided by the cap
   float to_log2;  // from a raw or capped score to log2 units
 };
@@ -691,7 +691,7 @@ extern "C" int nob200_masked_bf16_attention_d128(int num_rows, int num_key_rows,
   P.output = static_cast<__nv_bfloat16*>(output);
   P.rows = num_rows, P.key_rows = num_key_rows, P.documents = documents;
   P.heads = heads, P.group = heads / kv_heads, P.total_heads = total_heads, P.head_offset = head_offset;
-  P.slots = static_cast<int>(slots), P.unit_rows = unit_rows, P.splits = kv_splits, P.causal = causal != 0;
+  P.unit_rows = unit_rows, P.splits = kv_splits, P.causal = causal != 0;
   const float log2e = 1.4426950408889634f;
   P.scale = cap > 0.f ? scale / cap : scale;
   P.to_log2 = cap > 0.f ? cap * log2e : scale * log2e;

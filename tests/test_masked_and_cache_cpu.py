@@ -268,3 +268,52 @@ def test_masked_units_follow_the_options():
     late.causal = True
     call = late.prepare()[0][-1]
     assert (call.config.unit_rows, call.config.kv_splits) == (256, 2) and call.arguments.workspace is not None
+
+
+@pytest.mark.parametrize("sequences", [1, 2, 7, 64, 300])
+@pytest.mark.parametrize("heads,kv_heads", [(1, 1), (14, 14), (32, 8), (56, 8), (16, 1)])
+def test_cache_plans_can_be_launched(sequences, heads, kv_heads):
+    """Whatever the plan: shares within their limits, clusters of what a cluster holds, workspace where there is none."""
+    from nano_omni_b200.kernels.cache import MAX_CLUSTER, plan_cache_units
+    from nano_omni_b200.kernels.masked import share_workspace_bytes
+
+    for rows in (1, 2, 3, 8, 9, 16, 17, 24, 64, 65, 128, 129, 600, 4096):
+        for blocks in (1, 2, 4, 16, 100, 2048):
+            c = cache(blocks=sequences * blocks, kv_heads=kv_heads, sequences=sequences, max_blocks=blocks)
+            for tokens in (1, 65, c.capacity):
+                columns, splits, clusters = plan = plan_cache_units(rows, sequences, min(tokens, c.capacity), heads, kv_heads)
+                assert columns in (8, 16, 128) and 1 <= splits <= 64, plan
+                assert not clusters or (2 <= splits <= MAX_CLUSTER and columns < 128), plan
+                query, bounds = at(DType.BF16, rows, heads * 128), at(DType.I32, sequences + 1)
+                op = ops.CacheAttention(query, bounds, c, total_heads=heads, cached_tokens=tokens).to(at(DType.BF16, rows, heads, 128))
+                (call,), scratch = op.prepare()
+                assert (call.config.columns, call.config.kv_splits) == (columns, splits)
+                need = 0 if clusters else share_workspace_bytes(rows, heads, splits)
+                assert scratch == need == (call.arguments.workspace.num_bytes if call.arguments.workspace else 0)
+
+
+@pytest.mark.parametrize(
+    "call,plan",
+    [
+        # eight and nine, sixteen and seventeen rows of a sequence and key head
+        ((64, 64, 64 * 1021, 8, 1), (8, 7, True)),
+        ((64, 64, 64 * 1021, 9, 1), (16, 4, False)),
+        ((64, 64, 64 * 1021, 16, 1), (16, 4, False)),
+        ((64, 64, 64 * 1021, 17, 1), (8, 3, False)),
+        # 64 and 65: from there on tiles alone
+        ((64, 1, 300, 8, 8), (8, 2, True)),
+        ((65, 1, 300, 8, 8), (128, 1, False)),
+        # few rows against few keys and many: eights, tiles
+        ((24, 1, 1524, 8, 8), (8, 8, True)),
+        ((24, 1, 30000, 8, 8), (128, 18, False)),
+        # a token against keys of one share, of a cluster's, of more
+        ((1, 1, 128, 4, 4), (8, 1, False)),
+        ((1, 1, 256, 4, 4), (8, 2, True)),
+        ((1, 1, 1021, 14, 14), (8, 7, True)),
+        ((1, 1, 131072, 14, 14), (8, 42, False)),
+    ],
+)
+def test_cache_plans_on_both_sides_of_their_limits(call, plan):
+    from nano_omni_b200.kernels.cache import plan_cache_units
+
+    assert plan_cache_units(*call) == plan
