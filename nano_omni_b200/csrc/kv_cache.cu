@@ -73,6 +73,10 @@ __device__ __forceinline__ uint2 pack_codes(const int8_t (&c)[8]) {
   r.y = static_cast<uint8_t>(c[4]) | static_cast<uint8_t>(c[5]) << 8 | static_cast<uint8_t>(c[6]) << 16 | static_cast<uint32_t>(static_cast<uint8_t>(c[7])) << 24;
   return r;
 }
+// A code on the grid of another scale; of the magnitudes only 128 can leave the codes, on a grid that has turned.
+__device__ __forceinline__ int8_t again(int code, float ratio) {
+  return static_cast<int8_t>(__float2int_rn(fminf(__fmul_rn(static_cast<float>(code), ratio), 127.f)));
+}
 __device__ __forceinline__ int code_at(uint32_t word, int i) { return static_cast<int8_t>(word >> (8 * i)); }
 
 __global__ void __launch_bounds__(kAppendThreads)
@@ -151,7 +155,7 @@ cache_append_kernel(const AppendParams P) {
     __syncthreads();  // also: everyone has read the old scale
 #pragma unroll
     for (int w = 0; w < kAppendThreads / 32; ++w) top = max_nan(top, maxima[w]);
-    const float scale = max_nan(old, max_nan(__fmul_rn(top, 1.0f / 127.0f), 1e-10f));
+    const float scale = max_nan(fabsf(old), max_nan(__fmul_rn(top, 1.0f / 127.0f), 1e-10f));
     if (threadIdx.x == 0) scales[head] = scale;
     const float inverse = __frcp_rn(scale);
     const bool finite = scale <= 3.4e38f;  // else codes of 0, whose values are not numbers
@@ -171,7 +175,7 @@ cache_append_kernel(const AppendParams P) {
               finite ? codes_of<true>(*reinterpret_cast<const uint4*>(fresh + pitch * i), scale, inverse) : make_uint2(0, 0);
       }
     }
-    if (kept > 0 && scale != old) {  // the grid has grown: what was there is rounded again
+    if (kept > 0 && scale != old) {  // the grid has grown, or turned from a negative one: what was there is rounded again
       const float ratio = __fdiv_rn(old, scale);
 #pragma unroll
       for (int i = 0; i < kAppendPieces; ++i) {
@@ -179,8 +183,8 @@ cache_append_kernel(const AppendParams P) {
         int8_t c[8];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          c[k] = static_cast<int8_t>(__float2int_rn(__fmul_rn(static_cast<float>(code_at(x[i].x, k)), ratio)));
-          c[4 + k] = static_cast<int8_t>(__float2int_rn(__fmul_rn(static_cast<float>(code_at(x[i].y, k)), ratio)));
+          c[k] = again(code_at(x[i].x, k), ratio);
+          c[4 + k] = again(code_at(x[i].y, k), ratio);
         }
         *reinterpret_cast<uint2*>(mine + kAppendRows * kDim * i) = pack_codes(c);
       }

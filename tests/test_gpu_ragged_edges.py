@@ -99,6 +99,30 @@ def test_append_notes_bounds_behind_the_last_rows(bounds):
         assert torch.equal(cache.scales[which], want[1][which]) and torch.equal(cache.codes[which], want[0][which])
 
 
+@pytest.mark.parametrize("spread", [0.1, 30.0])
+def test_append_behind_a_negative_scale(spread):
+    """A block whose scale is negative, smaller or larger in magnitude than the new tokens need: its values stay, on a grid of
+    the larger magnitude."""
+    cache = Cache([50], 2, seed=38)
+    k, v = random_rows(39, 7, 2, spread), random_rows(40, 7, 2, spread)
+    block = cache.table[0, 0].long()
+    want = []
+    for which, x in enumerate((k, v)):
+        cache.scales[which][block, 0] *= -1
+        cache.codes[which][block, 0, 5, 7] = -128
+        old = cache.scales[which][block].clone()
+        scale = torch.maximum(old.abs(), x.float().abs().amax((0, 2)) * (1 / 127))
+        codes = cache.codes[which][block].clone()
+        held = torch.round(codes[:, :43].float() * (old / scale)[:, None, None]).clamp(-128, 127)
+        codes[:, :43] = torch.where((scale == old)[:, None, None], codes[:, :43].float(), held).to(torch.int8)
+        codes[:, 43:50] = torch.round(x.float().transpose(0, 1) / scale[:, None, None]).clamp(-127, 127).to(torch.int8)
+        want.append((scale, codes))
+    run_op(append_op(cache, k, v, ints([0, 7])))
+    for which in range(2):
+        assert torch.equal(cache.scales[which][block], want[which][0])
+        assert torch.equal(cache.codes[which][block], want[which][1])
+
+
 # ------------------------------------------------------------------ bounds of the attentions
 @pytest.mark.parametrize("columns,splits", [(8, 1), (8, 3), (16, 1), (128, 1), (128, 2)])
 @pytest.mark.parametrize("bounds", [[0, 30, 50], [-7, 20, 40], [0, 30, MOST], [LEAST, 25, 40], [0, 40, 41]], ids=str)
