@@ -32,9 +32,10 @@ __device__ __forceinline__ int2 document_rows(const int* bounds, int d, int rows
   return make_int2(begin, end);
 }
 
-// Whether document `d` begins and ends inside [0, rows], in this order.
+// Whether document `d` begins and ends inside [0, rows], in this order.  Both bounds are under way at once.
 __device__ __forceinline__ bool bounds_fit(const int* bounds, int d, int rows) {
-  return bounds[d] >= 0 && bounds[d] <= bounds[d + 1] && bounds[d + 1] <= rows;
+  const int begin = bounds[d], end = bounds[d + 1];
+  return (begin >= 0) & (begin <= end) & (end <= rows);
 }
 
 // Finds the `slot`-th unit of `count` documents with all THREADS threads of a CTA, a document each, so that what is to be known of

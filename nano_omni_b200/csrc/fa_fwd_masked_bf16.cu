@@ -114,7 +114,7 @@ __device__ __forceinline__ void find_own_unit(const MaskedParams& P, Shared<SMAL
           r.rows = document_rows(P.bounds, d, P.rows);
           r.units = (r.rows.y - r.rows.x + P.unit_rows - 1) / P.unit_rows;
           r.weight = r.keys.y - r.keys.x;
-          if (P.bounds[d + 1] < P.bounds[d] || P.key_bounds[d + 1] < P.key_bounds[d]) atomicOr(P.status, kBadIndex);
+          if ((P.bounds[d + 1] < P.bounds[d]) | (P.key_bounds[d + 1] < P.key_bounds[d])) atomicOr(P.status, kBadIndex);
         }
         return r;
       },

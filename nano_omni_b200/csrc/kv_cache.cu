@@ -102,11 +102,12 @@ cache_append_kernel(const AppendParams P) {
         if (live) {
           r.end = P.lengths[d];
           const bool fit = bounds_fit(P.bounds, d, P.rows);
-          const int fresh = fit ? P.bounds[d + 1] - P.bounds[d] : 0;
-          if (!fit || (fresh > 0 && (r.end < fresh || r.end > P.max_blocks * kBlock)))
-            atomicOr(P.status, kBadIndex);  // bounds or a length that cannot be right: no rows of it are appended
-          else if (fresh > 0)
-            r.first = P.bounds[d], r.before = r.end - fresh, r.units = (r.end + kBlock - 1) / kBlock - r.before / kBlock;
+          r.first = P.bounds[d];
+          const int fresh = P.bounds[d + 1] - r.first;  // of bounds that fit
+          r.before = r.end - fresh;
+          const bool right = fit && (fresh == 0 || (r.end >= fresh && r.end <= P.max_blocks * kBlock));
+          r.units = right && fresh > 0 ? (r.end + kBlock - 1) / kBlock - r.before / kBlock : 0;
+          if (!right) atomicOr(P.status, kBadIndex);  // bounds or a length that cannot be right: no rows of it are appended
         }
         return r;
       },
