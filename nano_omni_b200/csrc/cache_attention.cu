@@ -141,7 +141,6 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
           r.length = r.weight = P.lengths[d];
           r.prefix = P.prefix ? P.prefix[d] : 0;
           r.rows = document_rows(P.bounds, d, P.rows, &r.behind);
-          if (!bounds_fit(P.bounds, d, P.rows)) atomicOr(P.status, kBadIndex);
           r.units = ((r.rows.y - r.rows.x) * P.group + kColumns - 1) / kColumns;
         }
         return r;
@@ -150,7 +149,14 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
   pdl_release();
   const Unit unit = S.unit;
   const int sequence = unit.sequence;
-  if (sequence < 0) return;  // the whole cluster
+  auto note_bounds = [&] {
+    if (blockIdx.x == 0)
+      note_documents(threadIdx.x, P.sequences, kThreads, P.status, [&](int d) { return bounds_fit(P.bounds, d, P.rows); });
+  };
+  if (sequence < 0) {  // the whole cluster
+    note_bounds();
+    return;
+  }
 
   Sight sight;
   sight.keys = clamped(unit.length, 0, P.max_blocks * kBlock);
@@ -192,6 +198,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
   load(0, 0, e0);
   load(0, 1, e0);
   load(1, 0, e1);
+  note_bounds();
 
   // ---- the columns: a lane reads a quarter of column quad of each eight and works on columns 2 part and 2 part + 1
   uint32_t q[NT][kDim / 16][2];

@@ -98,7 +98,6 @@ __device__ __forceinline__ void find_own_unit(const CacheParams& P, Shared& S, i
           r.length = r.weight = P.lengths[d];
           r.prefix = P.prefix ? P.prefix[d] : 0;
           r.rows = document_rows(P.bounds, d, P.rows, &r.behind);
-          if (!bounds_fit(P.bounds, d, P.rows)) atomicOr(P.status, kBadIndex);
           r.units = ((r.rows.y - r.rows.x) * P.group + kTile - 1) / kTile;
         }
         return r;
@@ -210,6 +209,8 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
 
   if (warp >= kKeyWarp) {
     reg_dealloc<kServiceRegs>();
+    if (warp == kMmaWarp + 1 && blockIdx.x == 0)  // the value MMAs begin last
+      note_documents(lane, P.sequences, 32, status, [&](int d) { return bounds_fit(P.bounds, d, P.rows); });
     if (n_kv == 0) {
     } else if (warp == kKeyWarp || warp == kValueWarp) {
       // ------------------------------------------------------------ TMA producers, a block at a time

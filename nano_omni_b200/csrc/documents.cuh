@@ -38,10 +38,20 @@ __device__ __forceinline__ bool bounds_fit(const int* bounds, int d, int rows) {
   return (begin >= 0) & (begin <= end) & (end <= rows);
 }
 
+// Sets bit 6 of the status word if one of the documents first, first + step, .. is not right.  For a single CTA or warp of a launch,
+// beside its own work: noted by every CTA as it looks for its unit, one token of 1021 x 14 heads took 9.1 us instead of 8.95.
+template <typename Right>
+__device__ __forceinline__ void note_documents(int first, int count, int step, uint32_t* status, const Right& right) {
+  bool all = true;
+#pragma unroll 4
+  for (int d = first; d < count; d += step) all &= right(d);
+  if (!all) atomicOr(status, kBadIndex);
+}
+
 // Finds the `slot`-th unit of `count` documents with all THREADS threads of a CTA, a document each, so that what is to be known of
 // THREADS documents is one load's latency away: load(d, live) brings a document's record to its thread, with its `units` and
 // their `weight`, and found(record, document, unit) is called by the thread of the document that the unit is in, before the last
-// barrier.  load may note documents that cannot be right: between them the CTAs load every one.
+// barrier.
 // LONGEST_FIRST: up to THREADS documents are taken by falling weight (the longest key ranges), and a document's units from its
 // last one backwards (under a causal mask the longest again), so that short ones are left for the end of a launch; else, and
 // among more documents, they come in order.
@@ -101,11 +111,7 @@ __device__ __forceinline__ void find_unit(int count, int slot, FindScratch<THREA
       if (thread == S.hit[0]) found(record, d, S.hit[1]);
       __syncthreads();
     }
-    if (slot < total) {
-      if (blockIdx.x == 0)  // behind the last unit's documents nobody looks for one
-        for (base += THREADS; base < count; base += THREADS) load(base + thread, base + thread < count);
-      return;
-    }
+    if (slot < total) return;
     slot -= total;
   }
 }

@@ -114,7 +114,6 @@ __device__ __forceinline__ void find_own_unit(const MaskedParams& P, Shared<SMAL
           r.rows = document_rows(P.bounds, d, P.rows);
           r.units = (r.rows.y - r.rows.x + P.unit_rows - 1) / P.unit_rows;
           r.weight = r.keys.y - r.keys.x;
-          if ((P.bounds[d + 1] < P.bounds[d]) | (P.key_bounds[d + 1] < P.key_bounds[d])) atomicOr(P.status, kBadIndex);
         }
         return r;
       },
@@ -200,6 +199,9 @@ fa_fwd_masked_bf16_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
 
   if (warp >= F::kSoftmaxWarps) {
     reg_dealloc<F::kServiceRegs>();
+    if (warp == kCleanWarp && blockIdx.x == 0)  // the first V is a while away
+      note_documents(lane, P.documents, 32, status,
+                     [&](int d) { return (P.bounds[d] <= P.bounds[d + 1]) & (P.key_bounds[d] <= P.key_bounds[d + 1]); });
     if (n_kv == 0) {
     } else if (warp == kProducerWarp) {
       // ------------------------------------------------------------ TMA producer

@@ -112,6 +112,9 @@ cache_append_kernel(const AppendParams P) {
         return r;
       },
       [&](const Sequence& r, int d, int index) { own = r, own_index[0] = d, own_index[1] = index; });
+  if (blockIdx.x == 0)  // sequences that no CTA may come to as it looks for its block
+    note_documents(kAppendThreads + static_cast<int>(threadIdx.x), P.sequences, kAppendThreads, P.status,
+                   [&](int d) { return bounds_fit(P.bounds, d, P.rows); });
   const int sequence = own_index[0];
   if (sequence < 0) return;
   const int place = own.before / kBlock + own_index[1], token0 = place * kBlock;
