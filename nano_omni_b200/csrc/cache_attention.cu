@@ -586,6 +586,7 @@ extern "C" int nob200_int8_cache_attention_d128(int num_rows, int sequences, int
   const float log2e = 1.4426950408889634f;
   P.scale = cap > 0.f ? scale / cap : scale;
   P.to_log2 = cap > 0.f ? cap * log2e : log2e;
+  P.near = P.to_log2 <= kMostNearFactor ? 0.3f : -1.f;
   if (need) {
     P.partial = static_cast<float*>(workspace);
     P.lse = P.partial + static_cast<size_t>(kv_splits) * heads * num_rows * kDim;

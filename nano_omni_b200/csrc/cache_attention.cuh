@@ -28,6 +28,7 @@ struct CacheParams {
   int slots, splits, causal, joined;  // joined: the shares of a unit are a cluster, which joins them itself
   float scale;    // of a raw score; CAP form: divided by the cap
   float to_log2;  // from a (capped) scaled score to log2 units
+  float near;     // tiles, CAP form: the largest share of the cap for cap_scores' first way
 };
 
 // Units of 128 rows on the tensor cores' own instructions; slots counts such units.  Defined beside that kernel.

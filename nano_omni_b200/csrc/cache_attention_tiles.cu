@@ -329,7 +329,8 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
 #pragma unroll
         for (int i = 0; i < 4; ++i) top = fmaxf(top, fmaxf(fabsf(__uint_as_float(w[i] << 16)), fabsf(__uint_as_float(w[i] & 0xffff0000u))));
       }
-      const uint32_t exponent = min(max(__float_as_uint(top) >> 23, 1u), 253u);
+      // of a row that is none, or nothing, any; one that leaves cap_scores its shortest way
+      const uint32_t exponent = top == 0.f ? 127u : min(max(__float_as_uint(top) >> 23, 1u), 253u);
       const float down = __uint_as_float((254u - exponent) << 23);
       S.factor[thread] = __uint_as_float(exponent << 23);
 #pragma unroll 1
@@ -442,7 +443,11 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         const int valid = visible - tile_at(j) * kTile;
         // from a raw score to log2 units; a capped or biased one is turned into them at once
         const float unit = CAP || BIAS ? 1.f : key_scale * P.to_log2;
-        if constexpr (CAP) cap_scores(s, key_scale, P.to_log2);
+        if constexpr (CAP) {
+          const uint32_t least = __float_as_uint(kLeastNear);  // of positive numbers the order is that of their bits
+          const bool ordinary = __float_as_uint(key_scale) - least <= __float_as_uint(kMostNear) - least;
+          cap_scores(s, key_scale, P.to_log2, [&](float, float x) { return ordinary && x <= P.near; });
+        }
         if constexpr (BIAS) {
           const float from = static_cast<float>(position - tile_at(j) * kTile), f = CAP ? 1.f : key_scale * P.to_log2;
 #pragma unroll

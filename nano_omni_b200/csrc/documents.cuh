@@ -21,6 +21,15 @@ inline long long most_units(long long rows, long long documents, int unit) {
 // Scores are multiplied by scale / cap, which fp32 has to hold with all of its bits.
 inline bool cap_fits(float scale, float cap) { return cap == 0.f || (scale / cap >= 1e-35f && scale / cap <= 1e35f); }
 
+// For cap_scores: with c between 1e-7 and 1e5 and f up to 1e10 its coefficients stay in fp32; below, those past the first vanish, which
+// changes nothing for x up to 1e-3.
+constexpr float kLeastNear = 1e-7f, kMostNear = 1e5f, kMostNearFactor = 1e10f;
+inline float near_scores(float c, float f) {  // the largest score for the first way
+  if (c > kMostNear || f > kMostNearFactor) return -1.f;
+  const float top = (c >= kLeastNear ? 0.3f : 1e-3f) / c;
+  return top < 1e18f ? top : 1e18f;
+}
+
 #ifdef __CUDACC__
 
 __device__ __forceinline__ int clamped(int x, int low, int high) { return min(max(x, low), high); }

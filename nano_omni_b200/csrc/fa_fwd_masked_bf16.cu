@@ -95,6 +95,7 @@ struct MaskedParams {
   int unit_rows, splits, causal;
   float scale;    // of a raw score; CAP form: divided by the cap
   float to_log2;  // from a raw or capped score to log2 units
+  float near;     // near_scores
 };
 
 // The unit of this CTA, into shared memory.
@@ -404,7 +405,7 @@ fa_fwd_masked_bf16_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&S.s_taken[t]);
-        if constexpr (CAP) cap_scores(s, P.scale, P.to_log2);
+        if constexpr (CAP) cap_scores(s, P.scale, P.to_log2, [&](float top, float) { return top <= P.near; });
         [[maybe_unused]] float row_base = 0.f;
         if constexpr (BIAS) {
           const int key = tile_at(j) * kTile;
@@ -697,6 +698,7 @@ extern "C" int nob200_masked_bf16_attention_d128(int num_rows, int num_key_rows,
   const float log2e = 1.4426950408889634f;
   P.scale = cap > 0.f ? scale / cap : scale;
   P.to_log2 = cap > 0.f ? cap * log2e : scale * log2e;
+  P.near = near_scores(P.scale, P.to_log2);
   if (need) {
     P.partial = static_cast<float*>(workspace);
     P.lse = P.partial + static_cast<size_t>(kv_splits) * heads * num_rows * 128;
