@@ -209,8 +209,6 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
 
   if (warp >= kKeyWarp) {
     reg_dealloc<kServiceRegs>();
-    if (warp == kMmaWarp + 1 && blockIdx.x == 0)  // the value MMAs begin last
-      note_documents(lane, P.sequences, 32, status, [&](int d) { return bounds_fit(P.bounds, d, P.rows); });
     if (n_kv == 0) {
     } else if (warp == kKeyWarp || warp == kValueWarp) {
       // ------------------------------------------------------------ TMA producers, a block at a time
@@ -221,9 +219,10 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
       struct Blocks {
         int number;
         float key, value;
+        __half2 sign;
       };
       auto blocks_from = [&](int i) {
-        Blocks r = {-1, 0.f, 0.f};
+        Blocks r = {-1, 0.f, 0.f, __float2half2_rn(1.f)};
         if (i + lane < 2 * n_kv) {
           const int at = 2 * (kv_begin + tile_at((i + lane) >> 1)) + ((i + lane) & 1);
           r.number = block_of(P, table, at);
@@ -232,6 +231,7 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
             const size_t place = static_cast<size_t>(r.number) * P.kv_heads + key_head;
             r.key = P.key_scales[place];
             if (v) r.value = P.value_scales[place];
+            r.sign = __float2half2_rn(v && fabsf(r.value) < 1e-30f ? 0.f : (v ? r.value : r.key) < 0.f ? -1.f : 1.f);
           }
         }
         return r;
@@ -242,19 +242,19 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         const int st = i % kRawStages;
         if (i % 32 == 0) some = next;
         const int block = __shfl_sync(0xffffffffu, some.number, i % 32);
+        const __half2 sign = __shfl_sync(0xffffffffu, some.sign, i % 32);
         if (i >= kRawStages) ok = rest(&S.raw_empty[v][st], ((i / kRawStages) - 1) & 1, kWaitTimeoutRing);
         if (!ok) break;
-        const float key = __shfl_sync(0xffffffffu, some.key, i % 32), value = __shfl_sync(0xffffffffu, some.value, i % 32);
-        const bool none = v && fabsf(value) < 1e-30f;
         if (lane == 0) {
-          S.sign[v][st] = __float2half2_rn(none ? 0.f : (v ? value : key) < 0.f ? -1.f : 1.f);
+          S.sign[v][st] = sign;
           mbar_expect_tx(&S.raw_full[v][st], kRawBytes);
           // a block that is not there: any block, whose scores are masked
           tma_load_3d(S.raw[v][st], map, &S.raw_full[v][st], 0, (max(block, 0) * P.kv_heads + key_head) * kBlock, 0);
         }
         if (v) {
+          const float key = __shfl_sync(0xffffffffu, some.key, i % 32), value = __shfl_sync(0xffffffffu, some.value, i % 32);
           // V's is a summand of the exponent; of a block whose scale counts as 0 next to nothing is taken, of zeros
-          const float value_log2 = block < 0 ? kNotThere : log2f(none ? 1e-24f : fabsf(value));
+          const float value_log2 = block < 0 ? kNotThere : log2f(fabsf(value) < 1e-30f ? 1e-24f : fabsf(value));
           if (lane == 0) {
             S.scales[i % kScaleSlots] = make_float2(fabsf(key), value_log2);
             mbar_arrive(&S.scales_full[i % kScaleSlots]);
@@ -311,6 +311,8 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         }
       }
     }
+    if (warp == kMmaWarp && blockIdx.x == 0)  // through before the others
+      note_documents(lane, P.sequences, 32, status, [&](int d) { return bounds_fit(P.bounds, d, P.rows); });
   } else if (warp >= kWidenWarp) {
     // ------------------------------------------------- queries, then codes to f16 tiles
     reg_dealloc<kWidenRegs>();

@@ -200,9 +200,6 @@ fa_fwd_masked_bf16_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
 
   if (warp >= F::kSoftmaxWarps) {
     reg_dealloc<F::kServiceRegs>();
-    if (warp == kCleanWarp && blockIdx.x == 0)  // the first V is a while away
-      note_documents(lane, P.documents, 32, status,
-                     [&](int d) { return (P.bounds[d] <= P.bounds[d + 1]) & (P.key_bounds[d] <= P.key_bounds[d + 1]); });
     if (n_kv == 0) {
     } else if (warp == kProducerWarp) {
       // ------------------------------------------------------------ TMA producer
@@ -376,6 +373,9 @@ fa_fwd_masked_bf16_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
         }
       }
     }
+    if (warp == kCleanWarp && blockIdx.x == 0)  // through before the others
+      note_documents(lane, P.documents, 32, status,
+                     [&](int d) { return (P.bounds[d] <= P.bounds[d + 1]) & (P.key_bounds[d] <= P.key_bounds[d + 1]); });
   } else {
     // ------------------------------------------------- softmax + epilogue warps
     reg_alloc<F::kSoftmaxRegs>();
