@@ -60,8 +60,10 @@ def ptr(value) -> ctypes.c_void_p:
 def read_status(stream: int | None = None) -> int:
     """Synchronise ``stream`` and return-and-clear the device status word.
 
-    Non-zero means a bounded device-side wait gave up (the kernel returned
-    early and its outputs are not valid).
+    Bits 0 to 4 mean that a bounded device-side wait gave up (the kernel returned
+    early and its outputs are not valid), bit 5 a store outside its tensor that the
+    checked build skipped, bit 6 a bound, length or block number in device memory
+    that was not right and was skipped or clamped.
     """
     out = ctypes.c_uint32(0)
     code = symbol("nob200_read_status")(

@@ -8,16 +8,17 @@
 // HBM, and the kernel by the bytes it keeps in flight and the instructions it spends on a byte (an SM has some 700 cycles for
 // the 16 KiB of a block).  Keys are the 16 rows of the matrix instructions (mma.sync m16n8k16) and queries their 8 columns: the
 // query heads that share a key head, of all new tokens of a sequence, are 8 or 16 columns of a CTA.  (Queries as 16 rows took
-// twice the instructions for one token of up to eight heads, and 242 registers: 64 contexts x 32 heads 253 us.)
+// twice the instructions for one token of up to eight heads, and 242 registers: 64 contexts x 32 heads 253 us.)  Eight columns
+// spill 8 to 28 bytes of registers a thread, sixteen 36 to 140, which have three CTAs to an SM at 168 registers.
 //
 // A CTA's four warps take steps of 32 keys in turn from its share of the sequence, each with a running maximum, sum and
 // accumulator of its own, joined at the end.  A warp feeds itself: its lane 0 issues TMA loads of K and V (32 x 128 bytes,
 // 128-byte swizzle) into a ring of three, two of which are in flight while one is worked on; sixteen warps per SM make
-// 128 KiB in flight, well over the 45 KiB that latency x bandwidth asks for.  One token against 131072 x 14 heads 84-88 us (5.3-5.6
-// TB/s), 64 ragged contexts x 8 key heads 5.5 TB/s, of the 6.55 of a copy; the schedulers issue in 59 % of the cycles.
+// 128 KiB in flight, well over the 45 KiB that latency x bandwidth asks for.  One token against 131072 x 14 heads 84-90 us (5.2-5.6
+// TB/s), 64 ragged contexts x 8 key heads 5.5-6.2 TB/s, of the 6.55 of a copy; the schedulers issue in 59 % of the cycles.
 //  * scores: A = codes, which f16 holds exactly (byte -> f16 by a permute onto 1024 + (code + 128) and a subtraction); B = the
-//    queries as f16, scaled by a power of two to a row maximum in [1, 2) (exact down to 2^-24 of it).  The channels of an
-//    instruction's k index are chosen so that a lane reads 32 consecutive bytes of a key.
+//    queries as f16, scaled by a power of two to a row maximum in [1, 2): exact down to 2^-17 of it, what is smaller off by 2^-25
+//    of it at most.  The channels of an instruction's k index are chosen so that a lane reads 32 consecutive bytes of a key.
 //  * values: A = V transposed by ldmatrix.trans, which delivers two channels of two keys per register; a permute puts the even
 //    channels in rows 0-7 and the odd ones in rows 8-15.  B = the probabilities, from the scores' layout by movmatrix,
 //    rounded to f16 (2^-11, and 2^-32 of the largest: kLift; their sum is taken before); the block's scale of V multiplies the

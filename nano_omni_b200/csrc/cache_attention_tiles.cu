@@ -3,10 +3,11 @@
 //
 // A unit is up to 128 rows - (new token, head of the group) pairs of a sequence and key head - against 128 keys, two blocks, at a
 // time.  The scores and values are tcgen05 products of f16 operands, which hold an 8-bit code exactly (and take five instructions
-// for four codes, bf16 eight); queries are scaled by a power of two to a row maximum in [1, 2) (exact down to 2^-24 of it).  The
-// scales of K multiply the scores as they leave TMEM, those of V the probabilities before these are rounded to f16 (their
-// signs the codes, in the fused multiply-add that widens them), so nothing of K and V is rounded.  (Sixteen columns at a time by mma.sync widen every code once per sixteen rows: 1200 warp
-// instructions per 32 keys, 28 rows against 4000 keys x 8 heads x 16 sequences 102 us, here 60.)
+// for four codes, bf16 eight); queries are scaled by a power of two to a row maximum in [1, 2) (exact down to 2^-17 of it).  The
+// scales of K multiply the scores as they leave TMEM, those of V the probabilities before these are rounded to f16, and their
+// signs the codes, in the fused multiply-add that widens them, so nothing of K and V is rounded.  (Sixteen columns at a time by
+// mma.sync widen every code once per sixteen rows: 1200 warp instructions per 32 keys, 28 rows against 4000 keys x 8 heads x 16
+// sequences 102 us, here 60.)
 //   warps 16, 19  TMA producers: the blocks of K and of V as they are, 8 bits, into a ring of five blocks each (one producer for both,
 //                 whose K waited for V's places, held the kernel at 1.8 us a tile)
 //   warps 8-11    widen the blocks of K to f16 in the 128-byte-swizzled layout of the MMAs, warps 12-15 those of V, into a ring of

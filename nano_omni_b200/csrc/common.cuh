@@ -23,7 +23,7 @@ int fail(int code, const char* fmt, ...);
 // Converts a CUDA error after a launch into a status (0 when none).
 int check_launch(const char* what);
 
-// Status-word bits written by kernels whose bounded waits gave up.
+// Status-word bits written by kernels whose bounded waits gave up, or that met an index that cannot be right.
 enum StatusBit : uint32_t {
   kWaitTimeoutLoad = 1u << 0,     // waiting for a TMA tile
   kWaitTimeoutMma = 1u << 1,      // waiting for tensor-core completion

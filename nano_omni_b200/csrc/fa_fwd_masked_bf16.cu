@@ -17,9 +17,9 @@
 //  * capped scores: tanh by odd polynomials while all of a warp's rows stay within a third of the cap, or within the cap, else
 //    by 1 - 2 / (1 + e^2x) on the MUFU (cap_scores).
 // Bound by the softmax warps like the dense kernel, 3500 cycles per 256 rows x 128 keys of which the MMAs and the MUFU have 2048
-// each, and under long loads by the power cap: 32768 causal rows x 14 heads 3.24-3.52 ms (1.09-1.18 PFLOP/s), 15104 with a distance
-// bias 761 us, 9461 rows of nine documents 119-126 us (0.69), 4096 capped rows of three, 32 heads over 4, 134-138 us (104
-// without the cap).  Short documents pay a CTA's start and end, two to three tiles' time.
+// each, and under long loads by the power cap: 32768 causal rows x 14 heads 3.44-3.57 ms (1.08-1.12 PFLOP/s), 15104 with a distance
+// bias 800-857 us, 9461 rows of nine documents 114-125 us (0.70-0.77), 4096 capped rows of three, 32 heads over 4, 136-137 us
+// (107 without the cap).  Short documents pay a CTA's start and end, two to three tiles' time.
 #include <cuda.h>
 
 #include <type_traits>
@@ -714,7 +714,8 @@ extern "C" int nob200_masked_bf16_attention_d128(int num_rows, int num_key_rows,
   if ((rc = make_tensor_map_3d(&mv, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, value, 128, kv_heads, num_key_rows, 256, key_pitch, 64, 1, kTile)))
     return rc;
 
-  // CTAs of one query tile share an SM once there are more of them than SMs; alone on it a tile's scores need not wait
+  // CTAs of one query tile share an SM once there are more of them than SMs (148, as the planner counts them); alone on it a tile's
+  // scores need not wait
   const bool small = unit_rows == kTile && blocks > 148;
   auto launch = [&](auto small_form) -> int {
     constexpr bool kSmall = decltype(small_form)::value;

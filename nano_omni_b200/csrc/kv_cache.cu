@@ -294,7 +294,7 @@ cache_read_kernel(const ReadParams P) {
         if (first + 16 * i >= end || some + h >= last) continue;
         uint32_t o[4];
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {  // one rounding to bf16, of the exact product in fp32
+        for (int k = 0; k < 2; ++k) {  // the product of 7 and 24 bits is rounded to fp32, then to bf16
           o[k] = pack_bf16(code_at(c[h][i].x, 2 * k) * scale[h], code_at(c[h][i].x, 2 * k + 1) * scale[h]);
           o[2 + k] = pack_bf16(code_at(c[h][i].y, 2 * k) * scale[h], code_at(c[h][i].y, 2 * k + 1) * scale[h]);
         }
@@ -303,8 +303,9 @@ cache_read_kernel(const ReadParams P) {
   }
 }
 
-// Heads of a CTA: finding the block is two loads' latency, so that all CTAs have room at once where heads can make it so, eight
-// to an SM (64 short sequences x 8 heads read back in 12.9 us with a head each).
+// Heads of a CTA: finding the block is two loads' latency, so that a launch has some 1184 CTAs where heads can make it so (64
+// short sequences x 8 heads read back in 12.9 us with a head each).  An SM holds seven of the append's (72 registers) and four of
+// the read's (256 threads x 64); the last CTA of a block may have fewer heads than the others.
 int heads_each(int heads, long long all) {
   const long long each = (all + 8 * 148 - 1) / (8 * 148);
   return static_cast<int>(each > heads ? heads : each);

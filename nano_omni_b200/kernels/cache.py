@@ -243,7 +243,8 @@ def plan_cache_units(num_rows: int, sequences: int, cached_tokens: int, heads: i
     """Units of a launch whose sequences are taken to be of one length (the device alone knows).
 
     Up to sixteen rows of a sequence and key head are columns of the small kernel, eight where they do, of which an SM has room
-    for four CTAs, of sixteen for two (16 rows against 8192 x 4 x 16 sequences 34 us as columns, 37 in tiles).  More are eights
+    for four CTAs; of sixteen it has room for three and two are planned for (16 rows against 8192 x 4 x 16 sequences 34 us as
+    columns, 37 in tiles, measured so).  More are eights
     of columns or take the kernel of 128-row tiles, whichever is estimated to be faster: a CTA of eight columns 7.6 us and
     0.018 a key, of tiles 11.5 and 0.0081, a second launch 3 (64 sequences x 14 key heads, 30 rows: 100 keys 53 us in eights, 75
     in tiles, 276 72 and 84, 1005 154 and 121; 24 rows of one sequence x 8 key heads: 1524 keys 11 and 16, 30000 39 and 34)."""

@@ -898,8 +898,9 @@ class BlockCache:
     """Keys and values in 8 bits: codes I8 ``[blocks, kv_heads, 64, 128]`` and scales F32 ``[blocks, kv_heads]`` of K and V;
     ``table`` I32 ``[sequences, max_blocks]`` names the block of tokens ``64 b .. 64 b + 63`` of a sequence, ``lengths`` I32
     ``[sequences]`` how many tokens it holds.  Table and lengths are read when an operator runs: a program changes them in
-    place between runs.  Entries of the table past a sequence's length are not read; one that is and names no block counts as
-    a block without keys and sets bit 6 of the status word."""
+    place between runs.  Entries of the table past a sequence's length count for nothing; one before it that names no block is
+    skipped by the append, a block without keys to the attention, a block of zeros to the read, and sets bit 6 of the status
+    word."""
 
     key: TensorDesc
     value: TensorDesc

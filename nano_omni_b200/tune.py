@@ -68,7 +68,7 @@ def measure(kernel, repeat: int, warmup: int) -> list[float]:
         times.append(a.elapsed_time(b))
     status = _lib.read_status()
     if status:
-        raise RuntimeError(f"device status {status:#x}: a bounded wait gave up")
+        raise RuntimeError(f"device status {status:#x}: a bounded wait gave up or an index was not right")
     return times
 
 
