@@ -407,7 +407,7 @@ int nob200_int8_cache_read_d128(int capacity, int sequences, int max_blocks, int
  * Attention of the queries bounds[s] .. bounds[s + 1] over the cached tokens of sequence s, with positions, masks, cap and
  * slopes as nob200_masked_bf16_attention_d128 (a sequence is a document, lengths[s] its keys).  Bounds that leave the rows or
  * descend set bit 6: a row that is there keeps the position that its sequence's end gives it, whatever rows are not.
- * Scales may have any sign; one of V below 1e-30 in magnitude counts as 0.  query bf16 [num_rows, heads, 128], key / value
+ * Scales may have any sign; one of V below 1e-30 in magnitude may count as 0.  query bf16 [num_rows, heads, 128], key / value
  * codes int8 [num_blocks, kv_heads, 64, 128], output bf16 [num_rows, total_heads, 128] at head_offset.
  * Of the rows of a sequence and key head (new tokens x query heads of a key head) `columns` are a CTA's: 8 or
  * 16 for few, 128 for more, which take tcgen05 tiles.  kv_splits > 1 divides each sequence's keys over so many CTAs, whose

@@ -9,7 +9,7 @@
 // the 16 KiB of a block).  Keys are the 16 rows of the matrix instructions (mma.sync m16n8k16) and queries their 8 columns: the
 // query heads that share a key head, of all new tokens of a sequence, are 8 or 16 columns of a CTA.  (Queries as 16 rows took
 // twice the instructions for one token of up to eight heads, and 242 registers: 64 contexts x 32 heads 253 us.)  Eight columns
-// spill 8 to 28 bytes of registers a thread, sixteen 36 to 140, which have three CTAs to an SM at 168 registers.
+// spill 4 to 28 bytes of registers a thread, sixteen 36 to 116, which have three CTAs to an SM at 168 registers.
 //
 // A CTA's four warps take steps of 32 keys in turn from its share of the sequence, each with a running maximum, sum and
 // accumulator of its own, joined at the end.  A warp feeds itself: its lane 0 issues TMA loads of K and V (32 x 128 bytes,
@@ -199,7 +199,6 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
   load(0, 0, e0);
   load(0, 1, e0);
   load(1, 0, e1);
-  note_bounds();
 
   // ---- the columns: a lane reads a quarter of column quad of each eight and works on columns 2 part and 2 part + 1
   uint32_t q[NT][kDim / 16][2];
@@ -391,14 +390,11 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     // ---- values
     ok = warp_rest(&full[nv % kStages], (nv / kStages) & 1, abort_flag, P.status, kWaitTimeoutLoad);
     if (!ok) break;
-    // a column that sees nothing of the step has probabilities of 0 and takes 0 of it, whatever its scale is; one below 1e-30 is
-    // taken for 0, as in the tiles
-    float take[NT][2];
-    const float taken = fabsf(value_scale) < 1e-30f ? 0.f : value_scale;
+    float take[NT][2];  // a column that sees nothing of the step has probabilities of 0 and takes 0 of it, whatever its scale is
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int c = 0; c < 2; ++c) take[n][c] = e0 >= 0 && visible[n][c] > key0 ? taken : 0.f;
+      for (int c = 0; c < 2; ++c) take[n][c] = e0 >= 0 && visible[n][c] > key0 ? value_scale : 0.f;
     const uint32_t v_at = smem_u32(ring[nv % kStages]);
     const int v_key = ((lane >> 3) & 1) * 8 + (lane & 7);  // ldmatrix: the row whose address this lane gives
 #pragma unroll
@@ -440,6 +436,8 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     for (const uint64_t start = global_timer_ns(); global_timer_ns() - start < 1000000ull;) {
     }
   }
+
+  note_bounds();
 
   // ---- join of the four warps
   float* joined = reinterpret_cast<float*>(ring[0]);

@@ -200,6 +200,12 @@ fa_fwd_masked_bf16_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
 
   if (warp >= F::kSoftmaxWarps) {
     reg_dealloc<F::kServiceRegs>();
+    auto note_bounds = [&] {  // beside the others' work; at the start or at the end as the form's registers like it (1 to 2 %)
+      if (warp == kCleanWarp && blockIdx.x == 0)
+        note_documents(lane, P.documents, 32, status,
+                       [&](int d) { return (P.bounds[d] <= P.bounds[d + 1]) & (P.key_bounds[d] <= P.key_bounds[d + 1]); });
+    };
+    if (SMALL) note_bounds();
     if (n_kv == 0) {
     } else if (warp == kProducerWarp) {
       // ------------------------------------------------------------ TMA producer
@@ -373,9 +379,7 @@ fa_fwd_masked_bf16_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
         }
       }
     }
-    if (warp == kCleanWarp && blockIdx.x == 0)  // through before the others
-      note_documents(lane, P.documents, 32, status,
-                     [&](int d) { return (P.bounds[d] <= P.bounds[d + 1]) & (P.key_bounds[d] <= P.key_bounds[d + 1]); });
+    if (!SMALL) note_bounds();
   } else {
     // ------------------------------------------------- softmax + epilogue warps
     reg_alloc<F::kSoftmaxRegs>();
