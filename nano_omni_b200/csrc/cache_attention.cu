@@ -357,7 +357,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         mx[n][c] = fmaxf(fmaxf(s[0][n][c], s[0][n][2 + c]), fmaxf(s[1][n][c], s[1][n][2 + c]));
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) mx[n][c] = fmaxf(mx[n][c], __shfl_xor_sync(0xffffffffu, mx[n][c], d));
-        grown |= mx[n][c] > top[n][c] + (kLift + kRescaleThreshold);
+        grown |= mx[n][c] - top[n][c] > kLift + kRescaleThreshold;  // a difference of neighbours is exact, the sum would be rounded
       }
     if (__any_sync(0xffffffffu, grown)) {
 #pragma unroll

@@ -469,12 +469,15 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         }
         const bool sees = there && valid > 0;  // a row that sees nothing of the keys takes nothing of them, whatever their scales are
         const float value_log2 = sees ? value_scale : 0.f;
-        const float mx =
-            sees ? fmaf(max3(a, b, fmaxf(__uint_as_float(s[kKeys - 2]), __uint_as_float(s[kKeys - 1]))), unit, value_log2) : kLowestMaximum;
-        if (__any_sync(0xffffffffu, mx > m_used + (kLift + kRescaleThreshold))) {
-          const float m_new = fmaxf(m_used, mx - kLift);
+        const float most = max3(a, b, fmaxf(__uint_as_float(s[kKeys - 2]), __uint_as_float(s[kKeys - 1])));
+        // The largest exponent as the probabilities' are computed below: large scores and maxima are rounded by more than a unit.  Of a
+        // row that sees nothing it is -inf, or NaN under a scale that is: neither raises the maximum.
+        float offset = value_log2 - m_used;
+        if (__any_sync(0xffffffffu, fmaf(most, unit, offset) > kLift + kRescaleThreshold)) {
+          const float m_new = fmaxf(m_used, fmaf(most, unit, value_log2) - kLift);
           const float alpha = ex2(m_used - m_new);
           m_used = m_new;
+          offset = value_log2 - m_used;
           if (j > 0) {  // P and O are untouched by the tensor core before the first PV
             sum *= alpha;
             ok = spin(&S.pv_done[half], (j - 1) & 1, kWaitTimeoutMma);
@@ -486,7 +489,7 @@ cache_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         if (kCopies == 1 && j >= 1 - half && !(ok = rest(&S.turn[1 - half][quarter], (j - 1 + half) & 1, kWaitTimeoutSoftmax))) break;
         // Probabilities times V's scale at once: 2^(x + log2 scale - m), rounded to f16 for the value MMAs; the row sum is taken
         // before, and divided by the scale.
-        const float offset = value_log2 - m_used, f = sees ? unit : 1.f;
+        const float f = sees ? unit : 1.f;
         const uint64_t unit2 = pack2(f, f), offset2 = pack2(offset, offset);
         uint64_t la = 0ull, lb = 0ull;
         uint32_t p[kKeys / 2];

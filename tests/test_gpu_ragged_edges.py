@@ -356,6 +356,29 @@ def test_many_keys_of_little_weight_count(columns, rows, splits):
     assert ((out[-1:].double() - want).abs() <= allowed_of(want, size, n, v.abs().amax())).all()
 
 
+@pytest.mark.parametrize("columns,rows", [(8, 8), (16, 9), (128, 20), (128, 40), (128, 100)])
+@pytest.mark.parametrize("size", [5e6, 1.8e7, 5e7, 1.1e8])
+def test_large_scores_that_grow_slowly(columns, rows, size):
+    """Scores of `size` in log2 units, where a step of fp32 is 0.5 to 8 units, that grow from block to block by up to 60 such
+    steps: no probability leaves f16, so that equal values come back whatever the weights are."""
+    cache = Cache([640], 1, seed=41)
+    blocks = cache.table[0].long()
+    for which in range(2):
+        cache.scales[which].fill_(0.01)
+    cache.codes[1].fill_(100)
+    q = torch.zeros(rows, 1, 128, dtype=torch.bfloat16, device="cuda")
+    q[:, :, 0], q[:, :, 1:5] = 1.0, 2.0**-17  # 127 + code * 2^-17 is exact in fp32
+    for step in (*range(1, 13), 15, 20, 30, 60):
+        cache.codes[0].zero_()
+        for b in range(10):
+            cache.codes[0][blocks[b], 0, :, 0] = 127
+            for channel in range(1, 5):
+                cache.codes[0][blocks[b], 0, :, channel] = min(127, max(0, step * b - 127 * (channel - 1)))
+        out = cached(cache, q, [0, rows], columns, causal=False, scale=size / (127 * 0.01 * 1.4426950408889634))
+        off = (out.double() - 1.0).abs().amax().item()  # probabilities are rounded by 2^-11 beside their sum, the result by 2^-8
+        assert off <= 2.0**-8 + 2.0**-11, (step, off)
+
+
 # ------------------------------------------------------------------ arguments for timing
 def test_addressing_arguments_leaves_given_tensors():
     """What a caller has put in place, index tensors among it, is not written."""
